@@ -1,0 +1,458 @@
+"""Measured cases of the sequence-layer operators: the gated delta rule (whole sequences, their gradients, single
+tokens), the gated unit, and counter-based dropout.
+
+``listed()`` and ``draw()`` give cases as dicts of plain values, ``prepare()`` makes a case's inputs on the GPU from
+a seed, ``run()`` is one pass, ``work()`` what a pass cannot do without, ``exact()`` the outputs in 64 bits.  Where the
+module's ``own`` is false ``run()`` computes the operators in their plain form from elementary torch operations; where
+it is true it calls this package (``admm-lstm_amd`` on ``sys.path``).
+
+The operators, for one sequence and head with state S [K, V] (rows of q, k: length K; of v: length V):
+
+    S'  = exp(g_t) S_{t-1}
+    u_t = beta_t (v_t - S'^T k_t)
+    S_t = S' + k_t u_t^T
+    o_t = scale S_t^T q_t                         (gated delta rule; scale = K^-1/2)
+
+    y = act(x Wg) * (x Wu)                        (gated unit; weights [D, F])
+
+    y = residual + x keep / P(keep)               (dropout; keep from Philox4x32-10 at the element's index)
+"""
+import math
+import os
+import sys
+
+import numpy as np
+import torch
+
+own = False
+
+DTYPES = {'bf16': torch.bfloat16, 'fp16': torch.float16, 'fp32': torch.float32}
+CHUNK = 64   # rows of one block of the plain form's scan over a sequence
+
+
+# ----------------------------------------------------------------------------------------------------- cases
+
+def _rule(name, B, T, Hk, Hv, K, V, dtype, train, packed=0):
+    return dict(name=name, op='rule', B=B, T=T, Hk=Hk, Hv=Hv, K=K, V=V, dtype=dtype, train=train, packed=packed)
+
+
+def listed():
+    return [
+        # one long prompt read once (no gradients), grouped heads: query/key heads shared by two value heads
+        _rule('rule_long', 1, 8192, 16, 32, 128, 128, 'bf16', False),
+        # a batch of 9 prompts of different lengths packed one behind the other (T = rows in all), odd head sizes
+        _rule('rule_packed', 1, 5003, 8, 8, 72, 104, 'fp16', False, packed=9),
+        # a training step on ordinary sequences
+        _rule('rule_train', 4, 2048, 8, 8, 128, 128, 'bf16', True),
+        # a training step on many short windows: the batch and window length of the LSTM benchmark (8192 x 32, hidden
+        # 256 = 4 heads of 64), a quarter of its rows, in its type
+        _rule('rule_windows', 2048, 32, 4, 4, 64, 64, 'fp32', True),
+        # single-token serving: one stream, where only latency counts
+        dict(name='step_one', op='step', B=1, Hk=16, Hv=32, K=128, V=128, dtype='bf16'),
+        # single-token serving of 192 streams out of a pool of states
+        dict(name='step_many', op='step', B=192, Hk=16, Hv=32, K=128, V=128, dtype='bf16'),
+        # the gated unit on a handful of tokens: the weights are read once, nothing else matters
+        dict(name='unit_tokens', op='unit', M=5, D=2048, F=8192, act='silu', dtype='bf16', train=False),
+        # inference over the rows of the LSTM benchmark's batch, hidden 512, odd width, in its type
+        dict(name='unit_fp32', op='unit', M=8192, D=512, F=1365, act='gelu', dtype='fp32', train=False),
+        # a training step of a wide layer
+        dict(name='unit_train', op='unit', M=8192, D=2048, F=8192, act='silu', dtype='bf16', train=True),
+        # dropout of the LSTM benchmark's hidden state (8192 x 256) on its way to the output layer
+        dict(name='drop_hidden', op='drop', M=8192, N=256, p=0.2, dtype='fp32', residual=False),
+        # dropout of a wide layer's output, added to its residual stream
+        dict(name='drop_wide', op='drop', M=16384, N=8191, p=0.1, dtype='bf16', residual=True),
+    ]
+
+
+def _log(rng, lo, hi):
+    return max(lo, min(hi, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))))
+
+
+def draw(rng):
+    op = rng.choice(['rule', 'rule', 'rule', 'step', 'unit', 'unit', 'drop'])
+    dtype = rng.choice(['bf16', 'bf16', 'fp16', 'fp32'])
+    if op == 'drop':
+        return dict(op=op, M=_log(rng, 1, 8192), N=_log(rng, 1, 8192), p=round(rng.uniform(0.0, 0.9), 3), dtype=dtype,
+                    residual=rng.random() < 0.5)
+    if op == 'unit':
+        return dict(op=op, M=_log(rng, 1, 4096), D=_log(rng, 16, 2048), F=_log(rng, 16, 4096),
+                    act=rng.choice(['silu', 'gelu', 'sigmoid']), dtype=dtype, train=rng.random() < 0.5)
+    K, V = _log(rng, 8, 128), _log(rng, 8, 256)
+    if op == 'step':
+        Hk = _log(rng, 1, 16)
+        return dict(op=op, B=_log(rng, 1, 256), Hk=Hk, Hv=Hk * rng.choice([1, 2]), K=K, V=V, dtype=dtype)
+    train = rng.random() < 0.5
+    T = _log(rng, 1, 2048 if train else 4096)
+    Hk = _log(rng, 1, 8)
+    Hv = Hk * rng.choice([1, 1, 2, 3])
+    # rows in all stay below the largest listed case's, counted over heads
+    most = (65536 if train else 131072) // Hv
+    B = _log(rng, 1, max(1, min(512, most // T)))
+    packed = rng.choice([0, 0, _log(rng, 1, 40)])
+    if packed:
+        B, T = 1, max(packed, B * T)
+    return dict(op=op, B=B, T=T, Hk=Hk, Hv=Hv, K=K, V=V, dtype=dtype, train=train, packed=packed)
+
+
+# ---------------------------------------------------------------------------------------------------- inputs
+
+def _unit_rows(x):
+    return x / x.square().sum(-1, keepdim=True).add(1e-6).sqrt()
+
+
+def _recurrent_inputs(case, lead, gen):
+    """q, k (rows of length one, as layers make them), v, log decays from 1e-3 to 1, and write strengths in (0, 1)."""
+    dt = DTYPES[case['dtype']]
+
+    def randn(*s):
+        return torch.randn(*s, generator=gen, device='cuda')
+
+    Hk, Hv, K, V = case['Hk'], case['Hv'], case['K'], case['V']
+    s = dict(q=_unit_rows(randn(*lead, Hk, K)).to(dt), k=_unit_rows(randn(*lead, Hk, K)).to(dt),
+             v=randn(*lead, Hv, V).to(dt),
+             g=-torch.exp(math.log(1e-3) * torch.rand(*lead, Hv, generator=gen, device='cuda')),
+             beta=torch.sigmoid(randn(*lead, Hv)))
+    return s, randn
+
+
+def prepare(case, seed):
+    gen = torch.Generator(device='cuda').manual_seed(int(seed))
+    dt = DTYPES[case['dtype']]
+    op = case['op']
+    if op == 'rule':
+        s, randn = _recurrent_inputs(case, (case['B'], case['T']), gen)
+        N = case['packed'] or case['B']
+        s['initial'] = 0.5 * randn(N, case['Hv'], case['K'], case['V'])
+        s['offsets'] = s['longest'] = None
+        if case['packed']:
+            off = _offsets(case, seed)
+            s['offsets'] = torch.tensor(off, dtype=torch.int32, device='cuda')
+            s['longest'] = max(b - a for a, b in zip(off, off[1:]))   # the caller packed the rows: it knows
+        if case['train']:
+            s['do'] = randn(*s['v'].shape).to(dt)
+            s['dfinal'] = randn(*s['initial'].shape)
+            for n in ('q', 'k', 'v', 'g', 'beta', 'initial'):
+                s[n].requires_grad_()
+    elif op == 'step':
+        s, randn = _recurrent_inputs(case, (case['B'],), gen)
+        pool = case['B'] + 3
+        s['state'] = 0.5 * randn(pool, case['Hv'], case['K'], case['V'])
+        s['slots'] = torch.randperm(pool, generator=gen, device='cuda')[:case['B']].to(torch.int32)
+    elif op == 'unit':
+        M, D, F = case['M'], case['D'], case['F']
+        s = dict(x=torch.randn(M, D, generator=gen, device='cuda').to(dt))
+        for n in ('wg', 'wu'):
+            s[n] = (torch.randn(D, F, generator=gen, device='cuda') / math.sqrt(D)).to(dt)
+        if case['train']:
+            s['dy'] = torch.randn(M, F, generator=gen, device='cuda').to(dt)
+            for n in ('x', 'wg', 'wu'):
+                s[n].requires_grad_()
+    else:
+        M, N = case['M'], case['N']
+        s = dict(x=torch.randn(M, N, generator=gen, device='cuda').to(dt).requires_grad_(),
+                 dy=torch.randn(M, N, generator=gen, device='cuda').to(dt), residual=None,
+                 seed=int(torch.randint(1 << 62, (1,), generator=gen, device='cuda')),
+                 offset=int(torch.randint(1 << 40, (1,), generator=gen, device='cuda')))
+        if case['residual']:
+            s['residual'] = torch.randn(M, N, generator=gen, device='cuda').to(dt)
+    return dict(s, case=dict(case))
+
+
+def _offsets(case, seed):
+    """Where the packed sequences begin: random cuts, so that lengths from none to most of the rows occur."""
+    r = np.random.RandomState(int(seed) % (1 << 31))
+    return [0] + sorted(int(c) for c in r.randint(0, case['T'] + 1, case['packed'] - 1)) + [case['T']]
+
+
+# ------------------------------------------------------------------------------------------------ plain forms
+
+def _per_sequence(x, offsets, longest):
+    """Packed rows [1, R, ...] as [N, longest, ...], rows past a sequence's end zero; and the places they came from."""
+    lens = (offsets[1:] - offsets[:-1]).long()
+    at = torch.arange(longest, device=x.device)[None, :]
+    inside = at < lens[:, None]
+    src = torch.where(inside, offsets[:-1, None].long() + at, 0)
+    y = x[0][src]
+    return y * inside.reshape(inside.shape + (1,) * (y.dim() - 2)).to(y.dtype), inside
+
+
+def _plain_rule(q, k, v, g, beta, initial, offsets=None, longest=None):
+    """The recurrence in blocks of CHUNK rows: within a block the u of all rows solve one triangular system; the state
+    passes from block to block.  32 bits, the decays' exponents in 64 (they are differences of long sums)."""
+    out_type, rows = v.dtype, None
+    q, k, v, g, beta = (x.float() for x in (q, k, v, g, beta))
+    if offsets is not None:
+        (q, rows), k, v, g, beta = (_per_sequence(q, offsets, longest),
+                                    *(_per_sequence(x, offsets, longest)[0] for x in (k, v, g, beta)))
+    N, T, Hk, K = q.shape
+    Hv, V = v.shape[2:]
+    n = -(-T // CHUNK)
+
+    def blocks(x):   # [N, T, H, *] -> [N, Hv, n, CHUNK, *]; rows past T change nothing: k = 0, beta = 0, g = 0
+        x = torch.nn.functional.pad(x, (0, 0) * (x.dim() - 2) + (0, n * CHUNK - T))
+        x = x.reshape(N, n, CHUNK, *x.shape[2:]).movedim(3, 1)
+        return x.repeat_interleave(Hv // x.shape[1], 1)
+
+    q, k, v, g, beta = blocks(q) * K ** -0.5, blocks(k), blocks(v), blocks(g), blocks(beta)
+    lower = torch.ones(CHUNK, CHUNK, dtype=torch.bool, device=q.device).tril()
+    c = g.double().cumsum(-1)
+    decay = (c[..., :, None] - c[..., None, :]).masked_fill(~lower, -math.inf).exp().float()
+    into, left = c.exp().float()[..., None], (c[..., -1:] - c).exp().float()[..., None]
+    kt = k.transpose(-1, -2).contiguous()
+    A = (k @ kt) * decay * beta[..., None]
+    eye = torch.eye(CHUNK, device=q.device)
+    inv, i = eye, torch.arange(CHUNK, device=q.device)
+    for s in (1, 2, 4, 8, 16, 32):   # (I + strictly lower A)^-1, blocks of s rows joined in pairs
+        pair = (i[:, None] // (2 * s) == i[None, :] // (2 * s)) & (i[:, None] // s > i[None, :] // s)
+        inv = inv - inv @ (A * pair) @ inv
+    b = beta[..., None]
+    U, W = inv @ (b * v), inv @ (b * into * k)
+    P = (q @ kt) * decay
+    qi, kl = q * into, (k * left).transpose(-1, -2).contiguous()
+    S, o = initial, []
+    for m in range(n):
+        u = U[:, :, m] - W[:, :, m] @ S
+        o.append(qi[:, :, m] @ S + P[:, :, m] @ u)
+        S = into[:, :, m, -1:] * S + kl[:, :, m] @ u
+    o = torch.stack(o, 2).movedim(1, 3).reshape(N, n * CHUNK, Hv, V)[:, :T] if n else v.new_zeros(N, 0, Hv, V)
+    if rows is not None:
+        o = o[rows][None]   # the sequences lie one behind the other: their rows in order
+    return o.to(out_type), S
+
+
+def _plain_step(q, k, v, g, beta, state, slots):
+    at = slots.long()
+    r = v.shape[1] // k.shape[1]
+    qf, kf = (x.float().repeat_interleave(r, 1) for x in (q, k))
+    S = g.exp()[..., None, None] * state[at]
+    u = beta[..., None] * (v.float() - (S * kf[..., None]).sum(-2))
+    S = S + kf[..., None] * u[..., None, :]
+    state[at] = S
+    return (qf.shape[-1] ** -0.5 * (S * qf[..., None]).sum(-2)).to(v.dtype)
+
+
+def _act(name, z):
+    if name == 'silu':
+        return z * torch.sigmoid(z)
+    if name == 'gelu':
+        return 0.5 * z * (1 + torch.erf(z * 2 ** -0.5))
+    return torch.sigmoid(z)
+
+
+def _plain_unit(x, wg, wu, act):
+    xf = x.float()
+    return (_act(act, xf @ wg.float()) * (xf @ wu.float())).to(x.dtype)
+
+
+M32 = 0xffffffff
+
+
+def _mulhilo(a, b):
+    """High and low 32 bits of a * b for a constant and a tensor of 32-bit values held in 64 (no product overflows)."""
+    lo, hi = a * (b & 0xffff), a * (b >> 16)
+    mid = hi + (lo >> 16)
+    return mid >> 16, ((mid & 0xffff) << 16) | (lo & 0xffff)
+
+
+def _keep_bits(n, seed, offset, device):
+    """16 random bits for each of n elements: Philox4x32-10 (Salmon et al., 2011) at counter (element // 8, offset) under
+    key seed; element 8 c + 2 w + h takes half h of word w."""
+    c = torch.arange(-(-n // 8), device=device)
+    x = [c & M32, c >> 32, torch.full_like(c, offset & M32), torch.full_like(c, (offset >> 32) & M32)]
+    k0, k1 = seed & M32, (seed >> 32) & M32
+    for _ in range(10):
+        h0, l0 = _mulhilo(0xD2511F53, x[0])
+        h1, l1 = _mulhilo(0xCD9E8D57, x[2])
+        x = [h1 ^ x[1] ^ k0, l1, h0 ^ x[3] ^ k1, l0]
+        k0, k1 = (k0 + 0x9E3779B9) & M32, (k1 + 0xBB67AE85) & M32
+    w = torch.stack(x, 1)
+    return torch.stack([w & 0xffff, w >> 16], 2).reshape(-1)[:n]
+
+
+def _plain_dropout(x, p, seed, offset, residual):
+    drop = int(round(p * 65536))
+    keep = (_keep_bits(x.numel(), seed, offset, x.device) >= drop).reshape(x.shape)
+    y = torch.where(keep, x.float() * (65536 / (65536 - drop)), 0.0)
+    return (y if residual is None else y + residual.float()).to(x.dtype)
+
+
+# ------------------------------------------------------------------------------------------------- one pass
+
+def _package():
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), 'admm-lstm_amd')
+    if path not in sys.path:
+        sys.path.insert(0, path)
+    from blocks import delta_rule, dropout, gated_unit
+    return delta_rule, gated_unit, dropout
+
+
+def run(s):
+    case = s['case']
+    if own:
+        delta_rule, gated_unit, dropout = _package()
+    if case['op'] == 'rule':
+        args = [s[n] for n in ('q', 'k', 'v', 'g', 'beta')]
+        if own:
+            o, final = delta_rule.gated_delta_rule(*args, initial_state=s['initial'], offsets=s['offsets'])
+        else:
+            o, final = _plain_rule(*args, s['initial'], s['offsets'], s['longest'])
+        if not case['train']:
+            return dict(o=o, final=final)
+        names = ('q', 'k', 'v', 'g', 'beta', 'initial')
+        grads = torch.autograd.grad([o, final], [s[n] for n in names], [s['do'], s['dfinal']])
+        return dict(o=o.detach(), final=final.detach(), **{'d' + n: x for n, x in zip(names, grads)})
+    if case['op'] == 'step':
+        args = [s[n] for n in ('q', 'k', 'v', 'g', 'beta', 'state')]
+        if own:
+            o = delta_rule.gated_delta_step(*args, slots=s['slots'])
+        else:
+            o = _plain_step(*args, s['slots'])
+        return dict(o=o, state=s['state'])
+    if case['op'] == 'unit':
+        args = [s[n] for n in ('x', 'wg', 'wu')]
+        y = gated_unit.gated_unit(*args, activation=case['act']) if own else _plain_unit(*args, case['act'])
+        if not case['train']:
+            return dict(y=y)
+        dx, dwg, dwu = torch.autograd.grad(y, args, s['dy'])
+        return dict(y=y.detach(), dx=dx, dwg=dwg, dwu=dwu)
+    if own:
+        y = dropout.dropout(s['x'], case['p'], s['seed'], offset=s['offset'], residual=s['residual'])
+    else:
+        y = _plain_dropout(s['x'], case['p'], s['seed'], s['offset'], s['residual'])
+    return dict(y=y.detach(), dx=torch.autograd.grad(y, s['x'], s['dy'])[0])
+
+
+# ------------------------------------------------------------------------------------------------ what it takes
+
+def work(case):
+    size = 4 if case['dtype'] == 'fp32' else 2
+    if case['op'] in ('rule', 'step'):
+        Hk, Hv, K, V = case['Hk'], case['Hv'], case['K'], case['V']
+        rows = case['B'] * case.get('T', 1)
+        N = case.get('packed') or case['B']
+        io = rows * ((2 * Hk * K + Hv * V) * size + 2 * Hv * 4)      # q, k, v; g and beta in 32 bits
+        out = rows * Hv * V * size
+        state = N * Hv * K * V * 4
+        flops = 6 * rows * Hv * K * V                                # S'^T k, k u^T, S^T q
+        if not case.get('train'):
+            return dict(bytes=io + out + 2 * state, flops=flops)
+        return dict(bytes=2 * io + 2 * out + 4 * state, flops=3 * flops)
+    if case['op'] == 'unit':
+        M, D, F = case['M'], case['D'], case['F']
+        if not case['train']:
+            return dict(bytes=(M * D + 2 * D * F + M * F) * size, flops=4 * M * D * F)
+        return dict(bytes=(2 * M * D + 4 * D * F + 2 * M * F) * size, flops=12 * M * D * F)
+    n = case['M'] * case['N']
+    return dict(bytes=n * size * (5 if case['residual'] else 4), flops=4 * n)
+
+
+# -------------------------------------------------------------------------------------------- outputs in 64 bits
+
+def _exact_rule(q, k, v, g, beta, S0, do=None, dS=None):
+    """Token by token.  q, k, v, do [N, T, H, *], g, beta [N, T, H], S0 [N, H, K, V]; each row's state is kept where
+    gradients are asked for, and the gradients follow the recurrence backwards."""
+    N, T, H, K = q.shape
+    scale = K ** -0.5
+    S, o, kept = S0.clone(), torch.zeros_like(v), []
+    for t in range(T):
+        if do is not None:
+            kept.append(S)
+        S = S * g[:, t].exp()[..., None, None]
+        u = beta[:, t, :, None] * (v[:, t] - torch.einsum('nhkv,nhk->nhv', S, k[:, t]))
+        S = S + k[:, t, :, :, None] * u[:, :, None, :]
+        o[:, t] = scale * torch.einsum('nhkv,nhk->nhv', S, q[:, t])
+    if do is None:
+        return o, S
+    grads = [torch.zeros_like(x) for x in (q, k, v, g, beta)]
+    dq, dk, dv, dg, db = grads
+    for t in range(T - 1, -1, -1):
+        decayed = kept.pop() * g[:, t].exp()[..., None, None]
+        err = v[:, t] - torch.einsum('nhkv,nhk->nhv', decayed, k[:, t])
+        u = beta[:, t, :, None] * err
+        now = decayed + k[:, t, :, :, None] * u[:, :, None, :]
+        dq[:, t] = scale * torch.einsum('nhkv,nhv->nhk', now, do[:, t])
+        dS = dS + scale * q[:, t, :, :, None] * do[:, t, :, None, :]
+        du = torch.einsum('nhkv,nhk->nhv', dS, k[:, t])
+        dv[:, t] = beta[:, t, :, None] * du
+        dk[:, t] = torch.einsum('nhkv,nhv->nhk', dS, u) - torch.einsum('nhkv,nhv->nhk', decayed, dv[:, t])
+        db[:, t] = (du * err).sum(-1)
+        dS = dS - k[:, t, :, :, None] * dv[:, t, :, None, :]
+        dg[:, t] = (dS * decayed).sum((-1, -2))
+        dS = dS * g[:, t].exp()[..., None, None]
+    return o, S, *grads, dS
+
+
+def exact(case, seed):
+    s = {n: x.detach() if isinstance(x, torch.Tensor) else x for n, x in prepare(case, seed).items()}
+    d = {n: x.double() for n, x in s.items() if isinstance(x, torch.Tensor) and x.is_floating_point()}
+    if case['op'] == 'rule':
+        N = case['packed'] or case['B']
+        steps = s['longest'] if case['packed'] else case['T']
+        per_step = N * case['Hv'] * case['K'] * case['V']
+        if case['train'] and steps * per_step * 8 > 60e9 or steps * (2e-4 + 4e-11 * per_step) * (3 if case['train'] else 1) > 18:
+            return None
+        r = case['Hv'] // case['Hk']
+        rows = {n: d[n] for n in ('q', 'k', 'v', 'g', 'beta', 'do') if n in d}
+        if case['packed']:
+            off = _offsets(case, seed)
+            rows = {n: torch.stack([torch.cat([x[0, a:b], x.new_zeros(steps - (b - a), *x.shape[2:])])
+                                    for a, b in zip(off, off[1:])]) for n, x in rows.items()}
+        q, k = (rows[n].repeat_interleave(r, 2) for n in 'qk')
+        got = _exact_rule(q, k, rows['v'], rows['g'], rows['beta'], d['initial'], rows.get('do'), d.get('dfinal'))
+
+        def back(x):
+            if case['packed']:
+                x = torch.cat([x[i, :b - a] for i, (a, b) in enumerate(zip(off, off[1:]))])[None]
+            return x
+
+        def grouped(x):
+            return back(x.reshape(*x.shape[:2], case['Hk'], r, -1).sum(3))
+
+        if not case['train']:
+            return dict(o=back(got[0]), final=got[1])
+        o, final, dq, dk, dv, dg, db, d0 = got
+        return dict(o=back(o), final=final, dq=grouped(dq), dk=grouped(dk), dv=back(dv), dg=back(dg), dbeta=back(db),
+                    dinitial=d0)
+    if case['op'] == 'step':
+        r, at = case['Hv'] // case['Hk'], s['slots'].long()
+        one = [d['q'].repeat_interleave(r, 1), d['k'].repeat_interleave(r, 1), d['v'], d['g'], d['beta']]
+        o, S = _exact_rule(*(x[:, None] for x in one), d['state'][at])
+        d['state'][at] = S
+        return dict(o=o[:, 0], state=d['state'])
+    if case['op'] == 'unit':
+        a, b = d['x'] @ d['wg'], d['x'] @ d['wu']
+        sig = 1 / (1 + (-a).exp())
+        if case['act'] == 'silu':
+            f, df = a * sig, sig * (1 + a * (1 - sig))
+        elif case['act'] == 'gelu':
+            phi = 0.5 * torch.special.erfc(-a / math.sqrt(2))
+            f, df = a * phi, phi + a * (-a * a / 2).exp() / math.sqrt(2 * math.pi)
+        else:
+            f, df = sig, sig * (1 - sig)
+        if not case['train']:
+            return dict(y=f * b)
+        da, db = d['dy'] * b * df, d['dy'] * f
+        return dict(y=f * b, dx=da @ d['wg'].T + db @ d['wu'].T, dwg=d['x'].T @ da, dwu=d['x'].T @ db)
+    n = case['M'] * case['N']
+    drop = int(round(case['p'] * 65536))
+    kept = torch.from_numpy(_philox_host(n, s['seed'], s['offset']) >= drop).cuda().reshape(case['M'], case['N'])
+    factor = 65536 / (65536 - drop)
+    y = kept * d['x'] * factor
+    return dict(y=y + d['residual'] if case['residual'] else y, dx=kept * d['dy'] * factor)
+
+
+def _philox_host(n, seed, offset):
+    """_keep_bits() once more, in unsigned 64-bit numpy."""
+    u = np.uint64
+    m, low = u(32), u(M32)
+    c = np.arange(-(-n // 8), dtype=u)
+    a, b, e, f = c & low, c >> m, np.full_like(c, offset & M32), np.full_like(c, (offset >> 32) & M32)
+    key = [seed & M32, (seed >> 32) & M32]
+    for _ in range(10):
+        p, r = a * u(0xD2511F53), e * u(0xCD9E8D57)
+        a, b, e, f = (r >> m) ^ b ^ u(key[0]), r & low, (p >> m) ^ f ^ u(key[1]), p & low
+        key = [(key[0] + 0x9E3779B9) & M32, (key[1] + 0xBB67AE85) & M32]
+    out = np.empty((len(c), 4, 2), np.uint16)
+    for w, x in enumerate((a, b, e, f)):
+        out[:, w, 0], out[:, w, 1] = x & u(0xffff), x >> u(16)
+    return out.reshape(-1)[:n]
