@@ -1,0 +1,114 @@
+"""ctypes binding of libseqops.so (the C ABI declared in include/seq_ops.h): the sequence-layer operators.
+
+Like libadmmlstm.so (``_native``) it is built in-tree by ``csrc/Makefile`` and is the only compute path of its operators:
+loading fails loudly when it is missing, and host tensors are refused.
+"""
+from __future__ import annotations
+
+import ctypes
+import os
+from ctypes import POINTER, Structure, c_char_p, c_float, c_int, c_int32, c_int64, c_void_p
+
+import torch  # noqa: F401  (must precede the CDLL load: one HIP runtime per process)
+
+from ._native import AdmmError, NativeUnavailable
+
+LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), 'libseqops.so')
+ABI_VERSION = 1
+DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+class SeqDelta(Structure):
+    _fields_ = [('batch', c_int64), ('T', c_int64), ('sequences', c_int64),
+                ('Hk', c_int32), ('Hv', c_int32), ('K', c_int32), ('V', c_int32),
+                ('dtype', c_int32), ('offsets_64', c_int32), ('scale', c_float), ('device', c_int32),
+                ('q', c_void_p), ('k', c_void_p), ('v', c_void_p), ('g', c_void_p), ('beta', c_void_p),
+                ('q_stride', c_int64 * 3), ('k_stride', c_int64 * 3), ('v_stride', c_int64 * 3),
+                ('g_stride', c_int64 * 3), ('beta_stride', c_int64 * 3),
+                ('offsets', c_void_p), ('initial', c_void_p)]
+
+
+class SeqDeltaStep(Structure):
+    _fields_ = [('batch', c_int64), ('pool', c_int64),
+                ('Hk', c_int32), ('Hv', c_int32), ('K', c_int32), ('V', c_int32),
+                ('dtype', c_int32), ('slots_64', c_int32), ('scale', c_float), ('device', c_int32),
+                ('q', c_void_p), ('k', c_void_p), ('v', c_void_p), ('g', c_void_p), ('beta', c_void_p),
+                ('q_stride', c_int64 * 2), ('k_stride', c_int64 * 2), ('v_stride', c_int64 * 2),
+                ('g_stride', c_int64 * 2), ('beta_stride', c_int64 * 2), ('state_stride', c_int64 * 2),
+                ('slots', c_void_p), ('state', c_void_p), ('o', c_void_p)]
+
+
+# name -> (restype, argtypes)
+_SIGNATURES = {
+    'seq_abi_version': (c_int32, []),
+    'seq_last_error': (c_char_p, []),
+    'seq_delta_workspace': (c_int, [POINTER(SeqDelta), c_int32, POINTER(c_int64)]),
+    'seq_delta_forward': (c_int, [POINTER(SeqDelta), c_int32, c_void_p, c_int64, c_void_p, c_void_p, c_void_p]),
+    'seq_delta_step': (c_int, [POINTER(SeqDeltaStep), c_void_p]),
+}
+EXPORTS = tuple(_SIGNATURES)
+
+_lib = None
+
+
+def load() -> ctypes.CDLL:
+    """Load (once) and return the library, with argtypes/restype declared."""
+    global _lib
+    if _lib is not None:
+        return _lib
+    if not os.path.exists(LIB_PATH):
+        raise NativeUnavailable(f'{LIB_PATH} not found: build it with `make -C admm-lstm_amd/admm_amd/csrc` '
+                                f'(or __graft_entry__.build()). There is no CPU fallback.')
+    try:
+        lib = ctypes.CDLL(LIB_PATH)
+    except OSError as e:  # pragma: no cover - environment dependent
+        raise NativeUnavailable(f'cannot load {LIB_PATH}: {e}') from e
+    for name, (res, args) in _SIGNATURES.items():
+        fn = getattr(lib, name)
+        fn.restype, fn.argtypes = res, args
+    if lib.seq_abi_version() != ABI_VERSION:
+        raise NativeUnavailable(f'{LIB_PATH}: ABI {lib.seq_abi_version()} != expected {ABI_VERSION}')
+    _lib = lib
+    return lib
+
+
+def check(rc: int, what: str) -> None:
+    if rc != 0:
+        raise AdmmError(f'{what} failed (code {rc}): {_lib.seq_last_error().decode(errors="replace")}', rc)
+
+
+def stream(device: torch.device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def require(cond: bool, msg: str) -> None:
+    if not cond:
+        raise ValueError(msg)
+
+
+def require_tensors(**tensors) -> None:
+    """All of them tensors (None is skipped)."""
+    for name, t in tensors.items():
+        if t is not None and not isinstance(t, torch.Tensor):
+            raise TypeError(f'{name} must be a tensor (got {type(t).__name__})')
+
+
+def require_device(**tensors) -> torch.device:
+    """All of them HIP tensors on one device (None is skipped); returns it."""
+    dev = None
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError(f'{name} must be a HIP device tensor (got {t.device}); '
+                               'admm-lstm_amd has no CPU execution path')
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise ValueError(f'{name} is on {t.device}, the other tensors on {dev}')
+    return dev
+
+
+def rows_last(t: torch.Tensor) -> torch.Tensor:
+    """The tensor itself where its last axis is contiguous, else a contiguous copy."""
+    return t if t.stride(-1) == 1 or t.size(-1) == 1 else t.contiguous()
