@@ -44,6 +44,8 @@ _SIGNATURES = {
     'seq_last_error': (c_char_p, []),
     'seq_delta_workspace': (c_int, [POINTER(SeqDelta), c_int32, POINTER(c_int64)]),
     'seq_delta_forward': (c_int, [POINTER(SeqDelta), c_int32, c_void_p, c_int64, c_void_p, c_void_p, c_void_p]),
+    'seq_delta_backward_scratch': (c_int, [POINTER(SeqDelta), POINTER(c_int64)]),
+    'seq_delta_backward': (c_int, [POINTER(SeqDelta), c_void_p, c_int64, c_void_p, c_int64] + [c_void_p] * 9),
     'seq_delta_step': (c_int, [POINTER(SeqDeltaStep), c_void_p]),
 }
 EXPORTS = tuple(_SIGNATURES)

@@ -1,39 +1,17 @@
 // seq_delta.hip -- the gated delta rule over whole sequences (seq_delta.hpp has the mathematics).
-#include "seq_delta.hpp"
+#include "seq_delta_dev.hpp"
 
 namespace seq {
 namespace {
-
-__device__ __forceinline__ int perm_row(int t, int m) { return 32 * (t >> 1) + 8 * (m >> 2) + 4 * (t & 1) + (m & 3); }
-
-// operand A of tile t: the lane's row, values 8 (4 s + g)..+7
-template <int W, int NP, int TILE>
-__device__ __forceinline__ void frag(const __bf16* base, int row, int s, int g, bf16x8 (&a)[NP]) {
-  const int at = tile_at<W>(row, 4 * s + g);
-#pragma unroll
-  for (int i = 0; i < NP; ++i) a[i] = *reinterpret_cast<const bf16x8*>(base + i * TILE + at);
-}
-
-// operand A of tile t of the transposed tile: the lane's column perm_row(t, l % 16), rows 32 s + 8 g..+7
-template <int W, int NP, int TILE>
-__device__ __forceinline__ void frag_t(const __bf16* base, int t, int s, int g, int x, bf16x8 (&a)[NP]) {
-  const int r = 32 * s + 8 * g + (x >> 2), c = 4 * (t >> 1) + (x & 3), h = 4 * (t & 1);
-  const int lo = tile_at<W>(r, c) + h, hi = tile_at<W>(r + 4, c) + h;
-#pragma unroll
-  for (int i = 0; i < NP; ++i) {
-    const bf16x4 u = tr4(base + i * TILE + lo), v = tr4(base + i * TILE + hi);
-    a[i] = __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7);
-  }
-}
 
 // ------------------------------------------------------------------------------------------------- per chunk: X, P
 
 constexpr int kLd = kC + 4;   // row length of the f32 64 x 64 tiles in LDS
 constexpr int kLdY = 36;
 
-template <int DT, int KP>
+template <int DT, int KP, bool SAVE>
 constexpr int prep_lds() {
-  using S = DeltaShape<DT, KP>;
+  using S = DeltaShape<DT, KP, SAVE>;
   const int mats = 2 * kC * kLd * 4 + 32 * kLdY * 4 + S::kXP;
   return (S::kKQ > mats ? S::kKQ : mats) + 4 * kC * 4;
 }
@@ -46,9 +24,9 @@ __device__ __forceinline__ f32x4 mm16(const float* a, int lda, const float* b, i
   return acc;
 }
 
-template <int DT, int KP>
+template <int DT, int KP, bool SAVE>
 __global__ __launch_bounds__(256) void k_delta_prep(DeltaArgs a) {
-  using S = DeltaShape<DT, KP>;
+  using S = DeltaShape<DT, KP, SAVE>;
   using T = typename Elem<DT>::T;
   constexpr int NP = S::NP;
   extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -57,7 +35,7 @@ __global__ __launch_bounds__(256) void k_delta_prep(DeltaArgs a) {
   float* const X = A + kC * kLd;
   float* const Y = X + kC * kLd;
   __bf16* const xp = reinterpret_cast<__bf16*>(Y + 32 * kLdY);
-  float* const ghi = reinterpret_cast<float*>(lds + prep_lds<DT, KP>() - 4 * kC * 4);
+  float* const ghi = reinterpret_cast<float*>(lds + prep_lds<DT, KP, SAVE>() - 4 * kC * 4);
   float* const glo = ghi + kC;
   float* const bet = glo + kC;
   int* const kbad = reinterpret_cast<int*>(bet + kC);   // rows of k that hold a NaN or infinity
@@ -135,15 +113,8 @@ __global__ __launch_bounds__(256) void k_delta_prep(DeltaArgs a) {
       const uint64_t odd = __ballot((gv - gv) + (bv - bv) != 0.f || kbad[lane]);
       const int bad = odd ? __ffsll((unsigned long long)odd) - 1 : kC;
       if (lane >= bad) gv = bv = 0.f;
-      // running sum in f64, kept as hi + lo: the exponents are differences of it, and have to be right to 1e-7 where
-      // the sum is large
-      double sum = gv;
-#pragma unroll
-      for (int d = 1; d < 64; d *= 2) {
-        const double up = __shfl_up(sum, d);
-        if (lane >= d) sum += up;
-      }
-      const double last = __shfl(sum, 63);
+      double last;
+      const double sum = running_sum(gv, lane, last);
       const float hi = (float)sum;
       ghi[lane] = hi;
       glo[lane] = (float)(sum - (double)hi);
@@ -165,14 +136,15 @@ __global__ __launch_bounds__(256) void k_delta_prep(DeltaArgs a) {
         const float d = lower ? expf((ghi[row] - ghi[col]) + (glo[row] - glo[col])) : 0.f;
         A[row * kLd + col] = col < row ? bet[row] * d * kk[j][r] : 0.f;
         const float p = lower ? a.scale * d * qk[j][r] : 0.f;
-        const int at = tile_at<kC>(row, col >> 3) + (col & 7);
-        __bf16* pp = xp + 3 * kC * kC + at;
-        const __bf16 p0 = (__bf16)p;
-        const float q1 = p - (float)p0;
-        const __bf16 p1 = (__bf16)q1;
-        pp[0] = p0;
-        pp[kC * kC] = p1;
-        if constexpr (S::NO > 2) pp[2 * kC * kC] = (__bf16)(q1 - (float)p1);
+        if (row >= 32 || col < 32) {
+          __bf16* pp = xp + 3 * kTri + tri_at(row, col >> 3) + (col & 7);
+          const __bf16 p0 = (__bf16)p;
+          const float q1 = p - (float)p0;
+          const __bf16 p1 = (__bf16)q1;
+          pp[0] = p0;
+          pp[kTri] = p1;
+          if constexpr (S::NPP > 2) pp[2 * kTri] = (__bf16)(q1 - (float)p1);
+        }
       }
     }
     __syncthreads();
@@ -220,11 +192,12 @@ __global__ __launch_bounds__(256) void k_delta_prep(DeltaArgs a) {
     __syncthreads();
     for (int i = tid; i < kC * kC / 8; i += 256) {
       const int r = i >> 3, p = i & 7;
+      if (r < 32 && p >= 4) continue;
       const f32x4* src = reinterpret_cast<const f32x4*>(X + r * kLd + 8 * p);
       bf16x8 pl[3];
       planes8<3>(cat8(src[0], src[1]), pl);
 #pragma unroll
-      for (int j = 0; j < 3; ++j) *reinterpret_cast<bf16x8*>(xp + j * kC * kC + tile_at<kC>(r, p)) = pl[j];
+      for (int j = 0; j < 3; ++j) *reinterpret_cast<bf16x8*>(xp + j * kTri + tri_at(r, p)) = pl[j];
     }
     __syncthreads();
     u32x4* dst = reinterpret_cast<u32x4*>(a.xp + ch * (int64_t)S::kXP);
@@ -234,27 +207,11 @@ __global__ __launch_bounds__(256) void k_delta_prep(DeltaArgs a) {
 
 // --------------------------------------------------------------------------------------------- chunk after chunk
 
-template <int DT, int KP> constexpr int scan_bufs() { return 2 * DeltaShape<DT, KP>::kStage <= 160 * 1024 ? 2 : 1; }
-
-// linear copy of a chunk's planes and vectors into LDS, 1 KB a wave at a time
-template <int DT, int KP, int WAVES>
-__device__ __forceinline__ void stage_chunk(const DeltaArgs& a, int64_t c, int hk, int h, char* lds, int wave, int lane) {
-  using S = DeltaShape<DT, KP>;
-  const char* kq = a.kq + (c * a.Hk + hk) * (int64_t)S::kKQ;
-  const char* xp = a.xp + (c * a.Hv + h) * (int64_t)S::kXP;
-  const char* vec = a.vec + (c * a.Hv + h) * (int64_t)S::kVec;
-  for (int i = wave; i < S::kStage / 1024; i += WAVES) {
-    const char* src = i < S::kKQ / 1024 ? kq + i * 1024
-                      : i < (S::kKQ + S::kXP) / 1024 ? xp + (i * 1024 - S::kKQ) : vec;
-    glds16(src + lane * 16, lds + i * 1024);
-  }
-}
-
 template <int DT, int KP, int WAVES, bool SAVE>
 __global__ __launch_bounds__(64 * WAVES) void k_delta_scan(DeltaArgs a) {
-  using S = DeltaShape<DT, KP>;
+  using S = DeltaShape<DT, KP, SAVE>;
   using T = typename Elem<DT>::T;
-  constexpr int NP = S::NP, NO = S::NO, LO = S::LO, NB = scan_bufs<DT, KP>(), KS = KP / 32;
+  constexpr int NP = S::NP, NO = S::NO, NB = scan_bufs<DT, KP, SAVE>(), KS = KP / 32;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, x = lane & 15, g = lane >> 4;
   // workgroups go to the eight XCDs in turn: those of one head (which read the same planes) share one XCD's L2
@@ -293,7 +250,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_delta_scan(DeltaArgs a) {
       }
   };
   if (nc > 0) {
-    stage_chunk<DT, KP, WAVES>(a, c0, hk, h, lds, wave, lane);
+    stage_chunk<S, WAVES>(a, c0, hk, h, lds, wave, lane);
     load_v(0);
   }
   for (int64_t ci = 0; ci < nc; ++ci) {
@@ -304,13 +261,13 @@ __global__ __launch_bounds__(64 * WAVES) void k_delta_scan(DeltaArgs a) {
 #pragma unroll
     for (int t = 0; t < 4; ++t) vc[t] = v[t];
     if (ci + 1 < nc) {
-      if (NB == 2) stage_chunk<DT, KP, WAVES>(a, c0 + ci + 1, hk, h, lds + ((ci + 1) & 1) * S::kStage, wave, lane);
+      if (NB == 2) stage_chunk<S, WAVES>(a, c0 + ci + 1, hk, h, lds + ((ci + 1) & 1) * S::kStage, wave, lane);
       load_v((ci + 1) * kC);
     }
     const __bf16* Kt = reinterpret_cast<const __bf16*>(buf);
     const __bf16* Qt = Kt + NP * S::kTile;
     const __bf16* Xt = reinterpret_cast<const __bf16*>(buf + S::kKQ);
-    const __bf16* Pt = Xt + 3 * kC * kC;
+    const __bf16* Pt = Xt + 3 * kTri;
     const float* vec = reinterpret_cast<const float*>(buf + S::kKQ + S::kXP);
     const int64_t ch = (c0 + ci) * a.Hv + h;
     if (SAVE && col < a.VP) {
@@ -337,7 +294,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_delta_scan(DeltaArgs a) {
         frag<KP, NP, S::kTile>(Kt, perm_row(t, x), s, g, fa);
         ks[t] = mfma_planes<NP, 3, 3>(fa, sp, ks[t]);
         frag<KP, NP, S::kTile>(Qt, perm_row(t, x), s, g, fa);
-        o[t] = mfma_planes<NP, NO, LO>(fa, so, o[t]);
+        o[t] = mfma_planes<NP, NO, NO>(fa, so, o[t]);
       }
     }
     // beta (v - exp(G) K S), and u = X of it
@@ -374,7 +331,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_delta_scan(DeltaArgs a) {
 #pragma unroll
       for (int s = 0; s <= t / 2; ++s) {
         bf16x8 fa[3];
-        frag<kC, 3, kC * kC>(Xt, perm_row(t, x), s, g, fa);
+        frag_tri(Xt, t, s, g, x, fa);
         u[t] = mfma_planes<3, 3, 3>(fa, rp[s], u[t]);
       }
     }
@@ -394,8 +351,8 @@ __global__ __launch_bounds__(64 * WAVES) void k_delta_scan(DeltaArgs a) {
 #pragma unroll
       for (int t = 2 * s; t < 4; ++t) {
         bf16x8 fa[NO];
-        frag<kC, NO, kC * kC>(Pt, perm_row(t, x), s, g, fa);
-        o[t] = mfma_planes<NO, NO, LO>(fa, up, o[t]);
+        frag_tri(Pt, t, s, g, x, fa);
+        o[t] = mfma_planes<NO, NO, NO>(fa, up, o[t]);
       }
     }
     // S <- exp(G_63) S + K^T (exp(G_63 - G) u)
@@ -428,7 +385,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_delta_scan(DeltaArgs a) {
     }
     if (NB == 1 && ci + 1 < nc) {
       __syncthreads();
-      stage_chunk<DT, KP, WAVES>(a, c0 + ci + 1, hk, h, lds, wave, lane);
+      stage_chunk<S, WAVES>(a, c0 + ci + 1, hk, h, lds, wave, lane);
     }
   }
   if (in) {
@@ -454,21 +411,16 @@ __global__ void k_delta_outside(DeltaRows rows, void* p, int64_t row) {
   }
 }
 
-template <class F>
-hipError_t allow_lds(F* f, int bytes) {
-  return hipFuncSetAttribute(reinterpret_cast<const void*>(f), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-}
-
 template <int DT, int KP, bool SAVE>
 hipError_t forward(const DeltaArgs& a, hipStream_t s) {
-  using S = DeltaShape<DT, KP>;
+  using S = DeltaShape<DT, KP, SAVE>;
   constexpr int W = 4;
-  hipError_t e = allow_lds(k_delta_prep<DT, KP>, prep_lds<DT, KP>());
+  hipError_t e = allow_lds(k_delta_prep<DT, KP, SAVE>, prep_lds<DT, KP, SAVE>());
   if (e != hipSuccess) return e;
-  constexpr int bytes = scan_bufs<DT, KP>() * S::kStage;
+  constexpr int bytes = scan_bufs<DT, KP, SAVE>() * S::kStage;
   e = allow_lds(k_delta_scan<DT, KP, W, SAVE>, bytes);
   if (e != hipSuccess) return e;
-  if (a.chunks) k_delta_prep<DT, KP><<<(unsigned)(a.chunks * a.Hk), 256, (unsigned)prep_lds<DT, KP>(), s>>>(a);
+  if (a.chunks) k_delta_prep<DT, KP, SAVE><<<(unsigned)(a.chunks * a.Hk), 256, (unsigned)prep_lds<DT, KP, SAVE>(), s>>>(a);
   const int64_t vg = (a.VP / 16 + W - 1) / W, heads = (a.rows.N * a.Hv + 7) / 8 * 8;
   k_delta_scan<DT, KP, W, SAVE><<<(unsigned)(heads * vg), 64 * W, bytes, s>>>(a);
   return hipGetLastError();

@@ -17,16 +17,21 @@
 namespace seq {
 
 constexpr int kC = 64;          // rows of a chunk
+// X and P are lower triangular: a plane is rows 0..31 of 32 values, then rows 32..63 of 64
+constexpr int kTri = 32 * 32 + 32 * 64;
+__device__ __forceinline__ int tri_at(int r, int c) { return r < 32 ? tile_at<32>(r, c) : 32 * 32 + tile_at<64>(r - 32, c); }
+
 constexpr float kMinG = -200.f;  // exp(g) is zero in f32 far above this: lower values (-inf too) act the same
 
-template <int DT, int KP>
+// SAVE: gradients follow, and f32 gradients (of g, beta and the state) are made of P too
+template <int DT, int KP, bool SAVE>
 struct DeltaShape {
   static constexpr int NP = Elem<DT>::kPlanes;
-  static constexpr int NO = DT == SEQ_FP32 ? 3 : 2;    // planes of S, u and P in what only o (of type DT) is made of
-  static constexpr int LO = DT == SEQ_FP32 ? 3 : 2;
+  static constexpr int NO = DT == SEQ_FP32 ? 3 : 2;    // planes of what only values of type DT are made of
+  static constexpr int NPP = SAVE ? 3 : NO;            // planes of P
   static constexpr int kTile = kC * KP;                // values of one plane of K or Q
   static constexpr int kKQ = 2 * NP * kTile * 2;       // bytes of a chunk's K planes and Q planes
-  static constexpr int kXP = (3 + NO) * kC * kC * 2;   // bytes of a chunk's X and P planes
+  static constexpr int kXP = (3 + NPP) * kTri * 2;     // bytes of a chunk's X and P planes
   static constexpr int kVec = 4 * kC * 4;              // exp(G); exp(G_63 - G); beta; exp(G_63), first row not finite
   static constexpr int kStage = kKQ + kXP + kVec;
 };

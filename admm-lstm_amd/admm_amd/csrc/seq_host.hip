@@ -10,6 +10,7 @@
 
 namespace seq {
 hipError_t delta_forward(const DeltaArgs& a, int dtype, int KP, bool save, hipStream_t s);
+hipError_t delta_backward(const DeltaGradArgs& ga, int dtype, int KP, bool wide_v, bool wide_o, hipStream_t s);
 hipError_t delta_outside(const DeltaRows& rows, void* p, int64_t row_bytes, hipStream_t s);
 hipError_t delta_step(const SeqDeltaStep& d, hipStream_t s);
 }  // namespace seq
@@ -67,12 +68,12 @@ int check_heads(int Hk, int Hv, int K, int V, int dtype) {
 
 struct DeltaSizes {
   int KP, NP, NO;
-  int64_t per, chunks, VP, kq, xp, vec, s0, u, saved, plain;
+  int64_t per, chunks, VP, kq, xp, vec, s0, u, heads, need;
 };
 
 int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
 
-int delta_sizes(const SeqDelta* d, DeltaSizes& z) {
+int delta_sizes(const SeqDelta* d, bool saved, DeltaSizes& z) {
   if (!d) return fail(SEQ_EINVAL, "NULL argument");
   const int rc = check_heads(d->Hk, d->Hv, d->K, d->V, d->dtype);
   if (rc) return rc;
@@ -89,19 +90,27 @@ int delta_sizes(const SeqDelta* d, DeltaSizes& z) {
   if (z.chunks > kMaxBlocks / d->Hv || (d->sequences + 8) > kMaxBlocks / (d->Hv * blocks))
     return fail(SEQ_EINVAL, "too many sequences, rows or heads for one launch");
   z.kq = up256(z.chunks * d->Hk * (4LL * z.NP * kC * z.KP));
-  z.xp = up256(z.chunks * d->Hv * (2LL * (3 + z.NO) * kC * kC));
+  z.xp = up256(z.chunks * d->Hv * (2LL * (3 + (saved ? 3 : z.NO)) * kTri));
   z.vec = up256(z.chunks * d->Hv * (4LL * kC * 4));
   z.s0 = up256(z.chunks * d->Hv * 4 * z.KP * z.VP);
   z.u = up256(z.chunks * d->Hv * 4 * kC * z.VP);
-  z.plain = z.kq + z.xp + z.vec;
-  z.saved = z.plain + z.s0 + z.u;
+  const int64_t rows = d->batch * d->T;
+  z.heads = d->Hv > d->Hk ? up256(rows * d->Hv * d->K * 4) : 0;
+  z.need = z.kq + z.xp + z.vec + (saved ? z.s0 + z.u : 0);
   return SEQ_OK;
 }
 
+int check_memory(const char* name, const void* p, int64_t bytes, int64_t need) {
+  if (bytes < need) return fail(SEQ_EINVAL, "%s memory of %lld bytes: %lld are needed", name, (long long)bytes, (long long)need);
+  if (need && (!p || !aligned16(p))) return fail(SEQ_EINVAL, "%s memory is NULL or not 16-byte aligned", name);
+  return SEQ_OK;
+}
+
+// whether 16 bytes at a time may be read from rows of n values
 template <class S>
-bool wide_rows(const SeqDelta* d, const void* p, const S& stride) {
+bool wide_rows(const SeqDelta* d, int len, const void* p, const S& stride) {
   const int n = 16 / elem_size(d->dtype);
-  return aligned16(p) && d->K % 8 == 0 && stride[0] % n == 0 && stride[1] % n == 0 && stride[2] % n == 0;
+  return aligned16(p) && len % 8 == 0 && stride[0] % n == 0 && stride[1] % n == 0 && stride[2] % n == 0;
 }
 
 void delta_args(const SeqDelta* d, const DeltaSizes& z, void* work, DeltaArgs& a) {
@@ -119,8 +128,8 @@ void delta_args(const SeqDelta* d, const DeltaSizes& z, void* work, DeltaArgs& a
   memcpy(a.vs, d->v_stride, sizeof a.vs);
   memcpy(a.gs, d->g_stride, sizeof a.gs);
   memcpy(a.bs, d->beta_stride, sizeof a.bs);
-  a.wide_q = wide_rows(d, d->q, d->q_stride);
-  a.wide_k = wide_rows(d, d->k, d->k_stride);
+  a.wide_q = wide_rows(d, d->K, d->q, d->q_stride);
+  a.wide_k = wide_rows(d, d->K, d->k, d->k_stride);
   a.initial = d->initial;
   a.chunks = z.chunks;
   char* w = static_cast<char*>(work);
@@ -142,21 +151,19 @@ const char* seq_last_error(void) { return g_error; }
 
 int seq_delta_workspace(const SeqDelta* d, int32_t saved, int64_t* bytes) {
   DeltaSizes z;
-  const int rc = delta_sizes(d, z);
+  const int rc = delta_sizes(d, saved != 0, z);
   if (rc) return rc;
   if (!bytes) return fail(SEQ_EINVAL, "NULL argument");
-  *bytes = saved ? z.saved : z.plain;
+  *bytes = z.need;
   return SEQ_OK;
 }
 
 int seq_delta_forward(const SeqDelta* d, int32_t saved, void* work, int64_t work_bytes, void* o, float* final_state,
                       void* stream) {
   DeltaSizes z;
-  const int rc = delta_sizes(d, z);
+  int rc = delta_sizes(d, saved != 0, z);
+  if (!rc) rc = check_memory("work", work, work_bytes, z.need);
   if (rc) return rc;
-  const int64_t need = saved ? z.saved : z.plain;
-  if (work_bytes < need) return fail(SEQ_EINVAL, "work memory of %lld bytes: %lld are needed", (long long)work_bytes, (long long)need);
-  if (need && (!work || !aligned16(work))) return fail(SEQ_EINVAL, "work memory is NULL or not 16-byte aligned");
   if (!delta_inputs(d) || (d->batch * d->T && !o) || (d->sequences && !final_state)) return fail(SEQ_EINVAL, "NULL buffer");
   ON_DEVICE(d->device);
   DeltaArgs a;
@@ -170,6 +177,51 @@ int seq_delta_forward(const SeqDelta* d, int32_t saved, void* work, int64_t work
   }
   if (!d->sequences) return SEQ_OK;
   return hip_result(delta_forward(a, d->dtype, z.KP, saved != 0, s), "delta_rule");
+}
+
+int seq_delta_backward_scratch(const SeqDelta* d, int64_t* bytes) {
+  DeltaSizes z;
+  const int rc = delta_sizes(d, true, z);
+  if (rc) return rc;
+  if (!bytes) return fail(SEQ_EINVAL, "NULL argument");
+  *bytes = z.s0 + z.u + 2 * z.heads;
+  return SEQ_OK;
+}
+
+int seq_delta_backward(const SeqDelta* d, const void* work, int64_t work_bytes, void* scratch, int64_t scratch_bytes,
+                       const void* d_o, const float* d_final, void* dq, void* dk, void* dv, float* dg, float* dbeta,
+                       float* d_initial, void* stream) {
+  DeltaSizes z;
+  int rc = delta_sizes(d, true, z);
+  if (!rc) rc = check_memory("work", work, work_bytes, z.need);
+  if (!rc) rc = check_memory("scratch", scratch, scratch_bytes, z.s0 + z.u + 2 * z.heads);
+  if (rc) return rc;
+  const bool some = d->batch * d->T != 0;
+  if (!delta_inputs(d) || (some && (!d_o || !dq || !dk || !dv || !dg || !dbeta))) return fail(SEQ_EINVAL, "NULL buffer");
+  ON_DEVICE(d->device);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  DeltaGradArgs ga;
+  memset(&ga, 0, sizeof ga);
+  delta_args(d, z, const_cast<void*>(work), ga.f);   // read only
+  char* p = static_cast<char*>(scratch);
+  ga.ds = reinterpret_cast<float*>(p);
+  ga.dr = reinterpret_cast<float*>(p + z.s0);
+  if (z.heads) {
+    ga.dq32 = reinterpret_cast<float*>(p + z.s0 + z.u);
+    ga.dk32 = reinterpret_cast<float*>(p + z.s0 + z.u + z.heads);
+  }
+  ga.d_o = d_o, ga.d_final = d_final;
+  ga.dq = dq, ga.dk = dk, ga.dv = dv, ga.dg = dg, ga.dbeta = dbeta, ga.d_initial = d_initial;
+  if (d->sequences) {
+    const bool wide_o = aligned16(d_o) && d->V % 8 == 0;
+    rc = hip_result(delta_backward(ga, d->dtype, z.KP, wide_rows(d, d->V, d->v, d->v_stride), wide_o, s), "delta_rule backward");
+  }
+  if (rc || !d->offsets || !some) return rc;
+  const int64_t size = elem_size(d->dtype), kb = (int64_t)d->Hk * d->K * size, vb = (int64_t)d->Hv * d->V * size, hb = (int64_t)d->Hv * 4;
+  void* const out[5] = {dq, dk, dv, dg, dbeta};
+  const int64_t row[5] = {kb, kb, vb, hb, hb};
+  for (int i = 0; i < 5 && !rc; ++i) rc = hip_result(delta_outside(ga.f.rows, out[i], row[i], s), "delta_rule backward");
+  return rc;
 }
 
 int seq_delta_step(const SeqDeltaStep* d, void* stream) {

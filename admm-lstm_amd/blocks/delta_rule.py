@@ -14,6 +14,7 @@ import ctypes
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from admm_amd import _seq_native as N
 
@@ -80,6 +81,34 @@ class _Call:
         return o, final, work
 
 
+class _GatedDeltaRule(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, g, beta, initial, offsets, scale):
+        call = _Call(q, k, v, g, beta, initial, offsets, scale)
+        o, final, work = call.forward(True)
+        ctx.save_for_backward(q, k, v, g, beta, initial, offsets)
+        ctx.work, ctx.scale = work, scale
+        return o, final
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_o, d_final):
+        q, k, v, g, beta, initial, offsets = ctx.saved_tensors
+        call = _Call(q, k, v, g, beta, initial, offsets, ctx.scale)
+        lib, need, dev = N.load(), ctypes.c_int64(), q.device
+        N.check(lib.seq_delta_backward_scratch(ctypes.byref(call.d), ctypes.byref(need)), 'gated_delta_rule')
+        scratch = torch.empty(need.value, dtype=torch.uint8, device=dev)
+        d_o, d_final = d_o.contiguous(), d_final.contiguous()
+        dq, dk, dv, dg, dbeta = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v, g, beta))
+        d_initial = torch.empty_like(d_final) if ctx.needs_input_grad[5] else None
+        N.check(lib.seq_delta_backward(ctypes.byref(call.d), ctx.work.data_ptr(), ctx.work.numel(), scratch.data_ptr(),
+                                       need.value, d_o.data_ptr(), d_final.data_ptr(),
+                                       *(t.data_ptr() for t in (dq, dk, dv, dg, dbeta)),
+                                       d_initial.data_ptr() if d_initial is not None else None, N.stream(dev)),
+                'gated_delta_rule backward')
+        return dq, dk, dv, dg, dbeta, d_initial, None, None
+
+
 def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor, *,
                      scale: Optional[float] = None, initial_state: Optional[torch.Tensor] = None,
                      offsets: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -114,6 +143,8 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
         initial_state = initial_state.contiguous()
     N.require_device(q=q, k=k, v=v, g=g, beta=beta, initial_state=initial_state, offsets=offsets)
     scale = q.size(3) ** -0.5 if scale is None else float(scale)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, g, beta, initial_state)):
+        return _GatedDeltaRule.apply(q, k, v, g, beta, initial_state, offsets, scale)
     return _Call(q, k, v, g, beta, initial_state, offsets, scale).forward(False)[:2]
 
 

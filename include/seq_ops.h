@@ -64,6 +64,14 @@ int seq_delta_workspace(const SeqDelta* d, int32_t saved, int64_t* bytes);
 int seq_delta_forward(const SeqDelta* d, int32_t saved, void* work, int64_t work_bytes, void* o, float* final_state,
                       void* stream);
 
+/* Gradients.  `work` as the forward with saved = 1 left it; `scratch` is more work memory.  d_o contiguous like o, d_final
+ * like final (NULL: zeros).  dq, dk, dv contiguous and of `dtype`, dg, dbeta contiguous float32, d_initial like
+ * initial (NULL: not wanted).  Rows that belong to no sequence get zero gradients. */
+int seq_delta_backward_scratch(const SeqDelta* d, int64_t* bytes);
+int seq_delta_backward(const SeqDelta* d, const void* work, int64_t work_bytes, void* scratch, int64_t scratch_bytes,
+                       const void* d_o, const float* d_final, void* dq, void* dk, void* dv, float* dg, float* dbeta,
+                       float* d_initial, void* stream);
+
 /* One token of each of `batch` streams; the state of row b is state[slots[b]] (slots NULL: state[b]) and is replaced.
  * q, k [batch, Hk, K], v, o [batch, Hv, V], g, beta [batch, Hv]; strides (batch, head) in elements, o contiguous.
  * state: `pool` states with the strides (slot, head) in elements, [K, V] contiguous.  A row whose slot is negative is idle: its

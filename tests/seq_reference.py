@@ -26,6 +26,13 @@ def o_atol(dtype, K):
     return 3 * 2.0 ** -17 * math.sqrt(K + 64) + f32_atol(K + 128)
 
 
+def grad_atol(dtype, K, V):
+    """Gradients: sums over K, V and the chunk's 64 rows several times over.  dbeta and dg add up to six such sums that partly
+    cancel, each of up to the size of the tensor's larger values: four times the bound of one."""
+    atol = 4 * f32_atol(K + V + 256)
+    return atol if dtype == torch.float32 else atol + 3 * 2.0 ** -17 * math.sqrt(K + 64)
+
+
 def assert_close(name, got, want, atol):
     """|got - want| <= half a step of got's type + atol * rms(want), element by element; NaN and inf in the same places."""
     assert got.shape == want.shape, f'{name}: shape {tuple(got.shape)} != {tuple(want.shape)}'

@@ -153,6 +153,147 @@ def test_a_sequence_in_two_calls_is_the_sequence_in_one(rule):
     assert torch.equal(torch.cat([a[0], b[0]], 1), whole[0]) and torch.equal(b[1], whole[1])   # cut on a chunk's edge
 
 
+# ---------------------------------------------------------------------------------------------------- gradients
+
+NAMES = ('q', 'k', 'v', 'g', 'beta', 'initial')
+
+
+def _grads(rule, ins, do, dfinal, **kw):
+    """Gradients of <o, do> + <final, dfinal> from the kernels and from the float64 recurrence."""
+    leaves = [x.detach().requires_grad_() for x in ins]
+    o, final = rule.gated_delta_rule(*leaves[:5], initial_state=leaves[5], **kw)
+    got = torch.autograd.grad([o, final], leaves, [do, dfinal])
+    ref = [x.detach().cpu().double().requires_grad_() for x in ins]
+    wo, wf = R.delta_rule(*ref[:5], initial=ref[5], **{n: x.cpu() for n, x in kw.items()})
+    want = torch.autograd.grad([wo, wf], ref, [do.cpu().double(), dfinal.cpu().double()], allow_unused=True)
+    return o, final, wo, wf, got, [torch.zeros_like(r) if w is None else w for r, w in zip(ref, want)]
+
+
+def _check_grads(rule, ins, dtype, **kw):
+    gen = torch.Generator(device='cuda').manual_seed(99)
+    K, V = ins[5].shape[2:]
+    do = torch.randn(ins[2].shape, generator=gen, device='cuda').to(dtype)
+    dfinal = torch.randn(ins[5].shape, generator=gen, device='cuda')
+    o, final, wo, wf, got, want = _grads(rule, ins, do, dfinal, **kw)
+    R.assert_close('o', o.detach(), wo.detach(), R.o_atol(dtype, K))
+    R.assert_close('final', final.detach(), wf.detach(), R.f32_atol(K + 128))
+    for n, a, b, leaf in zip(NAMES, got, want, ins):
+        assert a.dtype == leaf.dtype and a.shape == leaf.shape
+        R.assert_close('d' + n, a, b, R.grad_atol(a.dtype, K, V))
+
+
+@pytest.mark.parametrize('dtype', [BF16, FP16, FP32])
+@pytest.mark.parametrize('shape', SHAPES)
+def test_gradients(rule, shape, dtype):
+    B, T, Hk, Hv, K, V = shape
+    _check_grads(rule, R.delta_inputs(B, T, Hk, Hv, K, V, dtype, seed=21), dtype)
+
+
+@pytest.mark.parametrize('dtype', [BF16, FP32])
+def test_gradients_of_packed_sequences(rule, dtype):
+    off = torch.tensor([0, 0, 1, 65, 65, 193, 194, 260, 260], dtype=torch.int32, device='cuda')
+    _check_grads(rule, R.delta_inputs(1, 260, 2, 4, 40, 24, dtype, seed=22, n=8), dtype, offsets=off)
+
+
+def test_rows_outside_the_packed_sequences_get_zero_gradients(rule):
+    off = torch.tensor([5, 70, 90], dtype=torch.int32, device='cuda')
+    ins = R.delta_inputs(1, 200, 1, 2, 16, 24, BF16, seed=23, n=2)
+    leaves = [x.requires_grad_() for x in ins]
+    o, final = rule.gated_delta_rule(*leaves[:5], initial_state=leaves[5], offsets=off)
+    do = torch.full_like(o, math.nan)
+    do[:, 5:90] = 1.0
+    for n, d in zip(NAMES[:5], torch.autograd.grad([o, final], leaves, [do, torch.ones_like(final)])):
+        assert torch.isfinite(d).all(), n
+        assert (d[:, :5] == 0).all() and (d[:, 90:] == 0).all() and (d[:, 5:90] != 0).any(), n
+
+
+def test_gradients_with_strong_decay_and_resets(rule):
+    ins = R.delta_inputs(1, 150, 1, 2, 32, 32, FP32, seed=24)
+    ins[3][:, 10:140] -= 30.0
+    _check_grads(rule, ins, FP32)
+    ins[3][:, 20] = -math.inf
+    leaves = [x.requires_grad_() for x in ins]
+    o, final = rule.gated_delta_rule(*leaves[:5], initial_state=leaves[5])
+    grads = torch.autograd.grad([o, final], leaves, [torch.ones_like(o), torch.ones_like(final)])
+    assert all(torch.isfinite(x).all() for x in grads) and (grads[3][:, 20] == 0).all()
+
+
+def test_gradients_of_strided_inputs_and_without_an_initial_state(rule):
+    q, k, v, g, beta, _ = R.delta_inputs(2, 70, 2, 2, 24, 40, FP32, seed=25)
+    fused = torch.cat([q, k, v], -1).requires_grad_()
+    o, final = rule.gated_delta_rule(fused[..., :24], fused[..., 24:48], fused[..., 48:], g, beta)
+    (d,) = torch.autograd.grad(o.sum() + final.sum(), fused)
+    ref = fused.detach().cpu().double().requires_grad_()
+    wo, wf = R.delta_rule(ref[..., :24], ref[..., 24:48], ref[..., 48:], g.cpu(), beta.cpu())
+    (w,) = torch.autograd.grad(wo.sum() + wf.sum(), ref)
+    R.assert_close('d', d, w, R.grad_atol(FP32, 24, 40))
+
+
+def test_gradients_against_differences(rule):
+    """Along one direction: (L(x + h d) - L(x - h d)) / 2h.  L is a sum of ~1e4 f32 terms of size ~1 (error ~1e-4 in L, 1e-2
+    after division by 2h = 0.02), the third derivative adds ~h^2 relative: 2 % of the gradient's size is allowed."""
+    ins = R.delta_inputs(2, 100, 1, 2, 32, 24, FP32, seed=26)
+    gen = torch.Generator(device='cuda').manual_seed(5)
+    do = torch.randn(ins[2].shape, generator=gen, device='cuda')
+    df = torch.randn(ins[5].shape, generator=gen, device='cuda')
+
+    def loss(xs):
+        o, f = rule.gated_delta_rule(*xs[:5], initial_state=xs[5])
+        return float((o.double() * do).sum() + (f.double() * df).sum())
+
+    leaves = [x.detach().requires_grad_() for x in ins]
+    o, f = rule.gated_delta_rule(*leaves[:5], initial_state=leaves[5])
+    grads = torch.autograd.grad([o, f], leaves, [do, df])
+    for i, n in enumerate(NAMES):
+        d = grads[i] / grads[i].norm()
+        h = 1e-2 * float(ins[i].norm()) / 10
+        up = [x + h * d if j == i else x for j, x in enumerate(ins)]
+        dn = [x - h * d if j == i else x for j, x in enumerate(ins)]
+        slope = (loss(up) - loss(dn)) / (2 * h)
+        assert abs(slope - float(grads[i].norm())) <= 0.02 * float(grads[i].norm()), n
+
+
+def test_gradients_twice_and_after_an_edit(rule):
+    ins = [x.requires_grad_() for x in R.delta_inputs(1, 80, 1, 1, 16, 16, FP32, seed=27)]
+    o, _ = rule.gated_delta_rule(*ins[:5], initial_state=ins[5])
+    a = torch.autograd.grad(o.sum(), ins, retain_graph=True)
+    b = torch.autograd.grad(o.sum(), ins)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    o, _ = rule.gated_delta_rule(*ins[:5], initial_state=ins[5])
+    with torch.no_grad():
+        ins[2].add_(1.0)
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        o.sum().backward()
+
+
+def test_captured_training_step(rule):
+    """Forward and backward in one graph, replayed on new values in the same places."""
+    ins = [x.requires_grad_() for x in R.delta_inputs(2, 100, 1, 2, 32, 32, BF16, seed=28)]
+    do = torch.randn_like(ins[2])
+
+    def step():
+        o, f = rule.gated_delta_rule(*ins[:5], initial_state=ins[5])
+        return (o, f, *torch.autograd.grad([o, f], ins, [do, torch.ones_like(f)]))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for i in range(3):
+        with torch.no_grad():
+            do.mul_(-0.5)
+            ins[2].add_(0.25)
+        graph.replay()
+        got = [x.clone() for x in out]
+        want = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got, want)), i
+
+
 # ------------------------------------------------------------------------------------------------ single tokens
 
 STEPS = [(1, 1, 1, 1, 1), (3, 2, 4, 32, 32), (2, 1, 3, 33, 30), (5, 2, 2, 64, 65), (4, 1, 2, 100, 36), (7, 2, 2, 128, 128)]
