@@ -7,7 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import POINTER, Structure, c_char_p, c_float, c_int, c_int32, c_int64, c_void_p
+from ctypes import POINTER, Structure, c_char_p, c_float, c_int, c_int32, c_int64, c_uint64, c_void_p
 
 import torch  # noqa: F401  (must precede the CDLL load: one HIP runtime per process)
 
@@ -38,6 +38,12 @@ class SeqDeltaStep(Structure):
                 ('slots', c_void_p), ('state', c_void_p), ('o', c_void_p)]
 
 
+class SeqUnit(Structure):
+    _fields_ = [('M', c_int64), ('D', c_int32), ('F', c_int32), ('act', c_int32), ('dtype', c_int32), ('device', c_int32),
+                ('x', c_void_p), ('wg', c_void_p), ('wu', c_void_p),
+                ('x_ld', c_int64), ('wg_ld', c_int64), ('wu_ld', c_int64)]
+
+
 # name -> (restype, argtypes)
 _SIGNATURES = {
     'seq_abi_version': (c_int32, []),
@@ -47,6 +53,11 @@ _SIGNATURES = {
     'seq_delta_backward_scratch': (c_int, [POINTER(SeqDelta), POINTER(c_int64)]),
     'seq_delta_backward': (c_int, [POINTER(SeqDelta), c_void_p, c_int64, c_void_p, c_int64] + [c_void_p] * 9),
     'seq_delta_step': (c_int, [POINTER(SeqDeltaStep), c_void_p]),
+    'seq_dropout': (c_int, [c_int32, c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_uint64, c_uint64, c_void_p, c_int32,
+                            c_void_p]),
+    'seq_unit_workspace': (c_int, [POINTER(SeqUnit), c_int32, POINTER(c_int64)]),
+    'seq_unit_forward': (c_int, [POINTER(SeqUnit), c_void_p, c_int64, c_void_p, c_void_p, c_void_p]),
+    'seq_unit_backward': (c_int, [POINTER(SeqUnit), c_void_p, c_int64, c_void_p, c_void_p, c_int64] + [c_void_p] * 4),
 }
 EXPORTS = tuple(_SIGNATURES)
 

@@ -7,12 +7,17 @@
 #include <cstring>
 
 #include "seq_delta.hpp"
+#include "seq_unit.hpp"
 
 namespace seq {
 hipError_t delta_forward(const DeltaArgs& a, int dtype, int KP, bool save, hipStream_t s);
 hipError_t delta_backward(const DeltaGradArgs& ga, int dtype, int KP, bool wide_v, bool wide_o, hipStream_t s);
 hipError_t delta_outside(const DeltaRows& rows, void* p, int64_t row_bytes, hipStream_t s);
 hipError_t delta_step(const SeqDeltaStep& d, hipStream_t s);
+hipError_t dropout(int dtype, const void* x, const void* res, void* y, int64_t n, uint32_t below, uint64_t seed, uint64_t offset,
+                   const int64_t* seed_dev, hipStream_t s);
+hipError_t unit_forward(const UnitArgs& u, hipStream_t s);
+hipError_t unit_backward(const UnitArgs& u, hipStream_t s);
 }  // namespace seq
 
 using namespace seq;
@@ -142,6 +147,48 @@ void delta_args(const SeqDelta* d, const DeltaSizes& z, void* work, DeltaArgs& a
 
 bool delta_inputs(const SeqDelta* d) { return d->batch * d->T == 0 || (d->q && d->k && d->v && d->g && d->beta); }
 
+// ------------------------------------------------------------------------------------------------------ gated unit
+
+struct UnitSizes {
+  bool copy_x, copy_w;
+  int64_t D8, F8, x, w, da, need;
+};
+
+int unit_sizes(const SeqUnit* u, bool backward, UnitSizes& z) {
+  if (!u) return fail(SEQ_EINVAL, "NULL argument");
+  if (u->dtype < SEQ_BF16 || u->dtype > SEQ_FP32) return fail(SEQ_EINVAL, "unknown dtype %d", u->dtype);
+  if (u->act < SEQ_SILU || u->act > SEQ_SIGMOID) return fail(SEQ_EINVAL, "unknown activation %d", u->act);
+  if (u->M < 0 || u->M > kMaxBlocks) return fail(SEQ_EINVAL, "%lld rows: 0 to %lld are supported", (long long)u->M, (long long)kMaxBlocks);
+  if (u->D < 1 || u->D > SEQ_UNIT_MAX || u->F < 1 || u->F > SEQ_UNIT_MAX)
+    return fail(SEQ_EINVAL, "weights of %d x %d: 1 to %d are supported", u->D, u->F, SEQ_UNIT_MAX);
+  if (u->M / 64 + 1 > kMaxBlocks / (u->F / 64 + 1) || u->M / 64 + 1 > kMaxBlocks / (u->D / 64 + 1))
+    return fail(SEQ_EINVAL, "too many rows for one launch");
+  const int np = u->dtype == SEQ_FP32 ? 3 : 1;
+  z.D8 = (u->D + 7) / 8 * 8;
+  z.F8 = (u->F + 7) / 8 * 8;
+  z.copy_x = np == 3 || !aligned16(u->x) || u->x_ld % 8 || u->D % 8;
+  z.copy_w = np == 3 || !aligned16(u->wg) || !aligned16(u->wu) || u->wg_ld % 8 || u->wu_ld != u->wg_ld || u->F % 8;
+  z.x = z.copy_x ? up256(u->M * z.D8 * 2 * np) : 0;
+  z.w = z.copy_w ? up256(u->D * z.F8 * 2 * np) : 0;
+  z.da = backward ? up256(u->M * z.F8 * 2 * np) : 0;
+  z.need = z.x + 2 * z.w + 2 * z.da;
+  return SEQ_OK;
+}
+
+void unit_args(const SeqUnit* u, const UnitSizes& z, void* work, UnitArgs& a) {
+  memset(&a, 0, sizeof a);
+  a.M = (int)u->M, a.D = u->D, a.F = u->F, a.act = u->act, a.dtype = u->dtype;
+  a.x = u->x, a.wg = u->wg, a.wu = u->wu;
+  a.x_ld = u->x_ld, a.w_ld = u->wg_ld, a.wu_ld = u->wu_ld;
+  a.copy_x = z.copy_x, a.copy_w = z.copy_w, a.D8 = z.D8, a.F8 = z.F8;
+  char* w = static_cast<char*>(work);
+  a.xp = w;
+  a.wgp = w + z.x;
+  a.wup = a.wgp + z.w;
+  a.dap = a.wup + z.w;
+  a.dbp = a.dap + z.da;
+}
+
 }  // namespace
 
 extern "C" {
@@ -235,6 +282,57 @@ int seq_delta_step(const SeqDeltaStep* d, void* stream) {
   if (!d->q || !d->k || !d->v || !d->g || !d->beta || !d->o || (d->pool && !d->state)) return fail(SEQ_EINVAL, "NULL buffer");
   ON_DEVICE(d->device);
   return hip_result(delta_step(*d, static_cast<hipStream_t>(stream)), "delta_step");
+}
+
+int seq_dropout(int32_t dtype, const void* x, const void* residual, void* y, int64_t n, int32_t below, uint64_t seed,
+                uint64_t offset, const int64_t* seed_device, int32_t device, void* stream) {
+  if (dtype < SEQ_BF16 || dtype > SEQ_FP32) return fail(SEQ_EINVAL, "unknown dtype %d", dtype);
+  if (n < 0) return fail(SEQ_EINVAL, "negative size");
+  if (below < 0 || below > 65536) return fail(SEQ_EINVAL, "below must be 0 to 65536 (got %d)", below);
+  if (!n) return SEQ_OK;
+  if (!x || !y) return fail(SEQ_EINVAL, "NULL buffer");
+  ON_DEVICE(device);
+  return hip_result(dropout(dtype, x, residual, y, n, (uint32_t)below, seed, offset, seed_device, static_cast<hipStream_t>(stream)),
+                    "dropout");
+}
+
+int seq_unit_workspace(const SeqUnit* u, int32_t backward, int64_t* bytes) {
+  UnitSizes z;
+  const int rc = unit_sizes(u, backward != 0, z);
+  if (rc) return rc;
+  if (!bytes) return fail(SEQ_EINVAL, "NULL argument");
+  *bytes = z.need;
+  return SEQ_OK;
+}
+
+int seq_unit_forward(const SeqUnit* u, void* work, int64_t work_bytes, void* y, float* pre, void* stream) {
+  UnitSizes z;
+  int rc = unit_sizes(u, false, z);
+  if (!rc) rc = check_memory("work", work, work_bytes, z.need);
+  if (rc) return rc;
+  if (!u->M) return SEQ_OK;
+  if (!u->x || !u->wg || !u->wu || !y) return fail(SEQ_EINVAL, "NULL buffer");
+  ON_DEVICE(u->device);
+  UnitArgs a;
+  unit_args(u, z, work, a);
+  a.y = y, a.pre = pre;
+  return hip_result(unit_forward(a, static_cast<hipStream_t>(stream)), "gated_unit");
+}
+
+int seq_unit_backward(const SeqUnit* u, void* work, int64_t work_bytes, const float* pre, const void* dy, int64_t dy_ld,
+                      void* dx, void* dwg, void* dwu, void* stream) {
+  UnitSizes z;
+  int rc = unit_sizes(u, true, z);
+  if (!rc) rc = check_memory("work", work, work_bytes, z.need);
+  if (rc) return rc;
+  if (!u->wg || !u->wu || (u->M && (!u->x || !pre || !dy)) || !dwg != !dwu) return fail(SEQ_EINVAL, "NULL buffer");
+  ON_DEVICE(u->device);
+  UnitArgs a;
+  unit_args(u, z, work, a);
+  a.pre = const_cast<float*>(pre);   // read only
+  a.dy = dy, a.dy_ld = dy_ld;
+  a.dx = u->M ? dx : nullptr, a.dwg = dwg, a.dwu = dwu;
+  return hip_result(unit_backward(a, static_cast<hipStream_t>(stream)), "gated_unit backward");
 }
 
 }  // extern "C"

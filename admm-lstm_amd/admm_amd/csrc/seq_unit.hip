@@ -1,0 +1,304 @@
+// seq_unit.hip -- the gated unit y = act(x Wg) * (x Wu): both projections, the activation and the product in one kernel,
+// and its gradients.
+//
+// Forward: a workgroup forms the same tile of both projections (one tile of x in LDS serves both) and only their product
+// leaves it; where gradients follow, the projections a = x Wg and b = x Wu are kept too, in f32 (rounded to 16 bits they would
+// cost the gradients more than their own rounding).  Backward: da = dy b act'(a) and db = dy act(a) elementwise, rounded to
+// the inputs' type (one rounding more than the result's own), then dx = da Wg^T + db Wu^T as one product over both, and
+// dWg = x^T da, dWu = x^T db in one launch.
+//
+// Bound by the matrix cores where the layer is wide (12 M D F operations a training step), by the weights where there are few
+// rows.  f32 operands are split into three bf16 planes by a pass before (six products, seq_dev.hpp), and 16-bit operands whose
+// rows are not 16-byte aligned are copied to padded rows.
+#include "seq_gemm.hpp"
+#include "seq_unit.hpp"
+
+namespace seq {
+
+namespace {
+
+__device__ __forceinline__ float sigmoid(float z) { return admm::sigm(z); }
+
+// act(z), and its derivative
+__device__ __forceinline__ float act(int kind, float z) {
+  if (kind == SEQ_SILU) return z * sigmoid(z);
+  if (kind == SEQ_GELU) return 0.5f * z * erfcf(-0.70710678118654752f * z);
+  return sigmoid(z);
+}
+__device__ __forceinline__ void act_grad(int kind, float z, float& f, float& df) {
+  if (kind == SEQ_GELU) {
+    const float phi = 0.5f * erfcf(-0.70710678118654752f * z);
+    f = z * phi;
+    df = fmaf(z, 0.39894228040143268f * expf(-0.5f * z * z), phi);
+  } else {
+    const admm::SigPair s = admm::sig_pair(z);
+    if (kind == SEQ_SILU) {
+      f = z * s.s;
+      df = s.s * fmaf(z, s.sc, 1.f);
+    } else {
+      f = s.s;
+      df = s.s * s.sc;
+    }
+  }
+}
+
+// rows of n values with the stride ld, as rows of n8 >= n values, the rest zero: 16-bit values as they are, f32 as three planes
+// (`plane` elements apart)
+template <int DT>
+__global__ __launch_bounds__(256) void k_unit_copy(const void* src, int64_t ld, int64_t rows, int n, int64_t n8, __bf16* dst, int64_t plane) {
+  using T = typename Elem<DT>::T;
+  const T* s = static_cast<const T*>(src);
+  const int64_t pieces = n8 / 8, all = rows * pieces;
+  const bool wide = reinterpret_cast<uintptr_t>(src) % 16 == 0 && ld * (int)sizeof(T) % 16 == 0;
+  for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / pieces, p = i % pieces;
+    const int left = n - (int)(8 * p);
+    __bf16* d = dst + r * n8 + 8 * p;
+    if constexpr (DT == SEQ_FP32) {
+      f32x8 v = {};
+      if (left > 0) v = load8(s + r * ld + 8 * p, left, wide);
+      bf16x8 pl[3];
+      planes8<3>(v, pl);
+#pragma unroll
+      for (int j = 0; j < 3; ++j) *reinterpret_cast<bf16x8*>(d + j * plane) = pl[j];
+    } else {
+      const uint16_t* h = reinterpret_cast<const uint16_t*>(s) + r * ld + 8 * p;
+      uint16_t v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = j < left ? h[j] : 0;
+      *reinterpret_cast<u32x4*>(d) = *reinterpret_cast<const u32x4*>(v);
+    }
+  }
+}
+
+// four neighbouring values of a row, n of them inside it
+template <class T>
+__device__ __forceinline__ void store4(T* p, f32x4 v, int n, bool wide) {
+  typedef T T4 __attribute__((ext_vector_type(4)));
+  if (wide && n >= 4) {
+    T4 t;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t[i] = (T)v[i];
+    *reinterpret_cast<T4*>(p) = t;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < n) p[i] = (T)v[i];
+  }
+}
+
+template <int DT, int WM, int WN, int MT, int NT, bool KEEP>
+__global__ __launch_bounds__(64 * WM * WN) void k_unit(GemmArgs g, int kind, typename Elem<DT>::T* y, float* pre, bool wide) {
+  using G = Gemm<DT, WM, WN, MT, NT, true, false, true, false>;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, x = lane & 15, q = lane >> 4, wm = wave / WN, wn = wave % WN;
+  int tm, tn;
+  G::place(g, tm, tn);
+  f32x4 acc[MT][NT];
+  G::run(g, tm, tn, 0, lds, acc);
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    const int row = tm * G::BM + 16 * (wm * MT + i) + x;
+    if (row >= g.M) continue;
+#pragma unroll
+    for (int j = 0; j < NT / 2; ++j) {
+      const int col = tn * G::BH + 16 * (wn * (NT / 2) + j) + 4 * q, n = g.N - col;
+      if (n <= 0) continue;
+      const f32x4 a = acc[i][j], b = acc[i][j + NT / 2];
+      f32x4 r;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) r[e] = act(kind, a[e]) * b[e];
+      const int64_t at = (int64_t)row * g.N + col;
+      store4(y + at, r, n, wide);
+      if (KEEP) {
+        store4(pre + at, a, n, wide);
+        store4(pre + (int64_t)g.M * g.N + at, b, n, wide);
+      }
+    }
+  }
+}
+
+// AI, BI, SPLIT as in Gemm; otherwise blockIdx.y picks the matrix B and the result
+template <int DT, int WM, int WN, int MT, int NT, bool AI, bool BI, bool SPLIT>
+__global__ __launch_bounds__(64 * WM * WN) void k_unit_gemm(GemmArgs g, typename Elem<DT>::T* c0, typename Elem<DT>::T* c1, bool wide) {
+  using G = Gemm<DT, WM, WN, MT, NT, AI, BI, false, SPLIT>;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, x = lane & 15, q = lane >> 4, wm = wave / WN, wn = wave % WN;
+  int tm, tn;
+  G::place(g, tm, tn);
+  f32x4 acc[MT][NT];
+  G::run(g, tm, tn, blockIdx.y, lds, acc);
+  typename Elem<DT>::T* c = blockIdx.y ? c1 : c0;
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    const int row = tm * G::BM + 16 * (wm * MT + i) + x;
+    if (row >= g.M) continue;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      const int col = tn * G::BN + 16 * (wn * NT + j) + 4 * q, n = g.N - col;
+      if (n > 0) store4(c + (int64_t)row * g.N + col, acc[i][j], n, wide);
+    }
+  }
+}
+
+// da = dy b act'(a), db = dy act(a), as rows of F8 values (f32: planes)
+template <int DT>
+__global__ __launch_bounds__(256) void k_unit_back(UnitArgs u) {
+  using T = typename Elem<DT>::T;
+  const int64_t pieces = u.F8 / 8, all = u.M * pieces, plane = u.M * u.F8, MF = (int64_t)u.M * u.F;
+  const T* dy = static_cast<const T*>(u.dy);
+  const bool wide = u.F % 8 == 0, wide_dy = reinterpret_cast<uintptr_t>(dy) % 16 == 0 && u.dy_ld * (int)sizeof(T) % 16 == 0;
+  for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / pieces, p = i % pieces;
+    const int left = u.F - (int)(8 * p);
+    const f32x8 a = load8(u.pre + r * u.F + 8 * p, left, wide), b = load8(u.pre + MF + r * u.F + 8 * p, left, wide);
+    const f32x8 d = load8(dy + r * u.dy_ld + 8 * p, left, wide_dy);
+    f32x8 da, db;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float f, df;
+      act_grad(u.act, a[j], f, df);
+      da[j] = j < left ? d[j] * b[j] * df : 0.f;
+      db[j] = j < left ? d[j] * f : 0.f;
+    }
+    const int64_t at = r * u.F8 + 8 * p;
+    if constexpr (DT == SEQ_FP32) {
+      bf16x8 pa[3], pb[3];
+      planes8<3>(da, pa);
+      planes8<3>(db, pb);
+#pragma unroll
+      for (int j = 0; j < 3; ++j) {
+        *reinterpret_cast<bf16x8*>(reinterpret_cast<__bf16*>(u.dap) + j * plane + at) = pa[j];
+        *reinterpret_cast<bf16x8*>(reinterpret_cast<__bf16*>(u.dbp) + j * plane + at) = pb[j];
+      }
+    } else {
+      typedef T T8 __attribute__((ext_vector_type(8)));
+      *reinterpret_cast<T8*>(reinterpret_cast<T*>(u.dap) + at) = __builtin_convertvector(da, T8);
+      *reinterpret_cast<T8*>(reinterpret_cast<T*>(u.dbp) + at) = __builtin_convertvector(db, T8);
+    }
+  }
+}
+
+unsigned blocks_for(int64_t n) {
+  const int64_t want = (n + 255) / 256;
+  return (unsigned)(want < 256 * 32 ? want : 256 * 32);
+}
+
+template <int DT>
+void copy(const void* src, int64_t ld, int64_t rows, int n, int64_t n8, char* dst, hipStream_t s) {
+  if (rows && n8) k_unit_copy<DT><<<blocks_for(rows * n8 / 8), 256, 0, s>>>(src, ld, rows, n, n8, reinterpret_cast<__bf16*>(dst), rows * n8);
+}
+
+template <class F>
+hipError_t lds_for(F* f, int bytes) {
+  return hipFuncSetAttribute(reinterpret_cast<const void*>(f), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+}
+
+// planes of an operand: the tensor itself, or its copy
+void planes(const char* (&p)[3], bool copied, const void* x, const char* copy, int64_t plane) {
+  for (int i = 0; i < 3; ++i) p[i] = copied ? copy + i * plane * 2 : static_cast<const char*>(x);
+}
+
+void tiles(GemmArgs& g, int BM, int BN) {
+  g.tiles_m = (g.M + BM - 1) / BM;
+  g.tiles_n = (g.N + BN - 1) / BN;
+}
+
+template <int DT, int WM, int WN, int MT, int NT>
+hipError_t launch_unit(GemmArgs g, const UnitArgs& u, hipStream_t s) {
+  using T = typename Elem<DT>::T;
+  using G = Gemm<DT, WM, WN, MT, NT, true, false, true, false>;
+  tiles(g, G::BM, G::BH);
+  const bool wide = u.F % 4 == 0;
+  auto go = [&](auto* f) {
+    const hipError_t e = lds_for(f, G::kLds);
+    if (e == hipSuccess) f<<<(unsigned)(g.tiles_m * g.tiles_n), G::kThreads, G::kLds, s>>>(g, u.act, static_cast<T*>(u.y), u.pre, wide);
+    return e;
+  };
+  return u.pre ? go(k_unit<DT, WM, WN, MT, NT, true>) : go(k_unit<DT, WM, WN, MT, NT, false>);
+}
+
+template <int DT, int WM, int WN, int MT, int NT, bool AI, bool BI, bool SPLIT>
+hipError_t launch_gemm(GemmArgs g, void* c0, void* c1, hipStream_t s) {
+  using T = typename Elem<DT>::T;
+  using G = Gemm<DT, WM, WN, MT, NT, AI, BI, false, SPLIT>;
+  tiles(g, G::BM, G::BN);
+  auto* f = k_unit_gemm<DT, WM, WN, MT, NT, AI, BI, SPLIT>;
+  const hipError_t e = lds_for(f, G::kLds);
+  if (e != hipSuccess) return e;
+  f<<<dim3((unsigned)(g.tiles_m * g.tiles_n), c1 ? 2 : 1), G::kThreads, G::kLds, s>>>(g, static_cast<T*>(c0), static_cast<T*>(c1), g.N % 4 == 0);
+  return hipSuccess;
+}
+
+// tiles of 256 x 256 where they make work for most of the 256 compute units, else 64 x 64
+bool big(int64_t m, int64_t n) { return ((m + 255) / 256) * ((n + 255) / 256) >= 128; }
+
+template <int DT>
+hipError_t forward(const UnitArgs& u, hipStream_t s) {
+  if (u.copy_x) copy<DT>(u.x, u.x_ld, u.M, u.D, u.D8, u.xp, s);
+  if (u.copy_w) {
+    copy<DT>(u.wg, u.w_ld, u.D, u.F, u.F8, u.wgp, s);
+    copy<DT>(u.wu, u.wu_ld, u.D, u.F, u.F8, u.wup, s);
+  }
+  GemmArgs g = {};
+  g.M = u.M, g.N = u.F, g.K = u.D;
+  g.planes = DT == SEQ_FP32 ? 3 : 1;
+  g.lda = u.copy_x ? u.D8 : u.x_ld;
+  g.ldb = u.copy_w ? u.F8 : u.w_ld;
+  planes(g.a[0], u.copy_x, u.x, u.xp, u.M * u.D8);
+  planes(g.b[0], u.copy_w, u.wg, u.wgp, u.D * u.F8);
+  planes(g.b[1], u.copy_w, u.wu, u.wup, u.D * u.F8);
+  const hipError_t e = big(u.M, 2 * (int64_t)u.F) ? launch_unit<DT, 2, 4, 8, 4>(g, u, s) : launch_unit<DT, 2, 2, 2, 4>(g, u, s);
+  return e != hipSuccess ? e : hipGetLastError();
+}
+
+template <int DT>
+hipError_t backward(const UnitArgs& u, hipStream_t s) {
+  constexpr int np = DT == SEQ_FP32 ? 3 : 1;
+  if (u.M) k_unit_back<DT><<<blocks_for(u.M * u.F8 / 8), 256, 0, s>>>(u);
+  if (u.copy_x) copy<DT>(u.x, u.x_ld, u.M, u.D, u.D8, u.xp, s);
+  if (u.copy_w) {
+    copy<DT>(u.wg, u.w_ld, u.D, u.F, u.F8, u.wgp, s);
+    copy<DT>(u.wu, u.wu_ld, u.D, u.F, u.F8, u.wup, s);
+  }
+  hipError_t e = hipSuccess;
+  if (u.dx) {
+    GemmArgs g = {};
+    g.M = u.M, g.N = u.D, g.K = u.F;
+    g.planes = np;
+    g.lda = u.F8;
+    g.ldb = u.copy_w ? u.F8 : u.w_ld;
+    planes(g.a[0], true, nullptr, u.dap, u.M * u.F8);
+    planes(g.a[1], true, nullptr, u.dbp, u.M * u.F8);
+    planes(g.b[0], u.copy_w, u.wg, u.wgp, u.D * u.F8);
+    planes(g.b[1], u.copy_w, u.wu, u.wup, u.D * u.F8);
+    e = big(u.M, u.D) ? launch_gemm<DT, 2, 4, 8, 4, true, true, true>(g, u.dx, nullptr, s)
+                      : launch_gemm<DT, 2, 2, 2, 2, true, true, true>(g, u.dx, nullptr, s);
+    if (e != hipSuccess) return e;
+  }
+  if (u.dwg) {
+    GemmArgs g = {};
+    g.M = u.D, g.N = u.F, g.K = u.M;
+    g.planes = np;
+    g.lda = u.copy_x ? u.D8 : u.x_ld;
+    g.ldb = u.F8;
+    planes(g.a[0], u.copy_x, u.x, u.xp, u.M * u.D8);
+    planes(g.b[0], true, nullptr, u.dap, u.M * u.F8);
+    planes(g.b[1], true, nullptr, u.dbp, u.M * u.F8);
+    e = big(u.D, 2 * (int64_t)u.F) ? launch_gemm<DT, 2, 4, 8, 4, false, false, false>(g, u.dwg, u.dwu, s)
+                                   : launch_gemm<DT, 2, 2, 2, 2, false, false, false>(g, u.dwg, u.dwu, s);
+    if (e != hipSuccess) return e;
+  }
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t unit_forward(const UnitArgs& u, hipStream_t s) {
+  return u.dtype == SEQ_BF16 ? forward<SEQ_BF16>(u, s) : u.dtype == SEQ_FP16 ? forward<SEQ_FP16>(u, s) : forward<SEQ_FP32>(u, s);
+}
+hipError_t unit_backward(const UnitArgs& u, hipStream_t s) {
+  return u.dtype == SEQ_BF16 ? backward<SEQ_BF16>(u, s) : u.dtype == SEQ_FP16 ? backward<SEQ_FP16>(u, s) : backward<SEQ_FP32>(u, s);
+}
+
+}  // namespace seq

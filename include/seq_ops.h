@@ -92,6 +92,33 @@ typedef struct SeqDeltaStep {
 } SeqDeltaStep;
 int seq_delta_step(const SeqDeltaStep* d, void* stream);
 
+/* Dropout: y_i = residual_i + (keep_i ? x_i * 65536 / (65536 - below) : 0) for n contiguous values, residual may be NULL, y may
+ * be x or residual.  keep_i: 16 bits of Philox4x32-10 at counter (i / 8 in the low, offset in the high 64 bits) under the key
+ * seed -- half (i % 2) of word (i % 8) / 2 -- are not below `below` (0..65536).  seed_device (NULL: `seed` counts): one
+ * value on the device, read by the kernel. */
+int seq_dropout(int32_t dtype, const void* x, const void* residual, void* y, int64_t n, int32_t below, uint64_t seed,
+                uint64_t offset, const int64_t* seed_device, int32_t device, void* stream);
+
+/* The gated unit y = act(x Wg) * (x Wu): x [M, D] with the row stride x_ld, Wg and Wu [D, F] with the row strides wg_ld and
+ * wu_ld, y [M, F] contiguous, all of `dtype`; act: SEQ_SILU (z / (1 + exp(-z))), SEQ_GELU (the exact one, z Phi(z)) or
+ * SEQ_SIGMOID. */
+typedef struct SeqUnit {
+  int64_t M;
+  int32_t D, F, act, dtype, device;
+  const void *x, *wg, *wu;
+  int64_t x_ld, wg_ld, wu_ld;
+} SeqUnit;
+
+#define SEQ_UNIT_MAX 1048576     /* largest D and F */
+
+/* Work memory of the forward (backward = 0) or the backward.  `pre` [2, M, F] float32 receives x Wg and x Wu for the
+ * gradients, or is NULL.  dy [M, F] with the row stride dy_ld; dx [M, D], dwg and dwu [D, F] contiguous, dx and the pair dwg, dwu
+ * may be NULL where they are not wanted. */
+int seq_unit_workspace(const SeqUnit* u, int32_t backward, int64_t* bytes);
+int seq_unit_forward(const SeqUnit* u, void* work, int64_t work_bytes, void* y, float* pre, void* stream);
+int seq_unit_backward(const SeqUnit* u, void* work, int64_t work_bytes, const float* pre, const void* dy, int64_t dy_ld,
+                      void* dx, void* dwg, void* dwu, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

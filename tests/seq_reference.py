@@ -13,6 +13,7 @@ Tolerances, from the arithmetic:
 """
 import math
 
+import numpy as np
 import torch
 
 
@@ -33,8 +34,9 @@ def grad_atol(dtype, K, V):
     return atol if dtype == torch.float32 else atol + 3 * 2.0 ** -17 * math.sqrt(K + 64)
 
 
-def assert_close(name, got, want, atol):
-    """|got - want| <= half a step of got's type + atol * rms(want), element by element; NaN and inf in the same places."""
+def assert_close(name, got, want, atol, more=None):
+    """|got - want| <= half a step of got's type + atol * rms(want) (+ more), element by element; NaN and inf in the same
+    places."""
     assert got.shape == want.shape, f'{name}: shape {tuple(got.shape)} != {tuple(want.shape)}'
     g, w = got.double().cpu(), want.double().cpu()
     assert torch.equal(torch.isfinite(g), torch.isfinite(w)), f'{name}: non-finite values in other places'
@@ -45,6 +47,8 @@ def assert_close(name, got, want, atol):
         return
     rms = float(w.square().mean().sqrt())
     bound = torch.finfo(got.dtype).eps / 2 * w.abs() + atol * rms
+    if more is not None:   # half a step of a value that is off by `more` itself
+        bound = bound + more.double().cpu()[fin] * (1 + torch.finfo(got.dtype).eps / 2)
     over = ((g - w).abs() - bound).max()
     assert float(over) <= 0, (f'{name}: off by up to {float((g - w).abs().max()):.3e} (rms {rms:.3e}), '
                               f'{float(over):.3e} more than allowed')
@@ -96,3 +100,51 @@ def delta_inputs(B, T, Hk, Hv, K, V, dtype, seed=0, n=None, device='cuda'):
     beta = torch.sigmoid(randn(B, T, Hv))
     s0 = 0.5 * randn(B if n is None else n, Hv, K, V)
     return [x.to(device) for x in (q.to(dtype), k.to(dtype), v.to(dtype), g, beta, s0)]
+
+
+def philox_bits(n, seed, offset):
+    """16 random bits for each of n elements as blocks/dropout.py defines them: Philox4x32-10 in unsigned 64-bit numpy."""
+    u, low, half = np.uint64, np.uint64(0xffffffff), np.uint64(32)
+    c = np.arange(-(-n // 8), dtype=u)
+    x = [c & low, c >> half, np.full_like(c, offset & 0xffffffff), np.full_like(c, (offset >> 32) & 0xffffffff)]
+    k = [seed & 0xffffffff, (seed >> 32) & 0xffffffff]
+    for _ in range(10):
+        a, b = x[0] * u(0xD2511F53), x[2] * u(0xCD9E8D57)
+        x = [(b >> half) ^ x[1] ^ u(k[0]), b & low, (a >> half) ^ x[3] ^ u(k[1]), a & low]
+        k = [(k[0] + 0x9E3779B9) & 0xffffffff, (k[1] + 0xBB67AE85) & 0xffffffff]
+    return np.stack([v >> s & u(0xffff) for v in x for s in (u(0), u(16))], 1).reshape(-1)[:n]
+
+
+def dropout(x, p, seed, offset=0, residual=None):
+    below = int(round(p * 65536))
+    keep = torch.from_numpy(philox_bits(x.numel(), seed, offset).astype(np.int64) >= below).reshape(x.shape)
+    y = torch.where(keep, x.double().cpu() * (65536 / max(65536 - below, 1)), 0.0)
+    return (y if residual is None else y + residual.double().cpu()), keep
+
+
+def gated_unit(x, wg, wu, activation):
+    x, wg, wu = x.double(), wg.double(), wu.double()
+    a, b = x @ wg, x @ wu
+    f = {'silu': torch.nn.functional.silu, 'gelu': torch.nn.functional.gelu, 'sigmoid': torch.sigmoid}[activation]
+    return f(a) * b
+
+
+def unit_atol(n):
+    """y: two f32 sums of n products, an activation with slope at most 1.13 and size at most |a|, and their product, whose size the
+    two sums' root mean squares bound: three times the bound of one sum."""
+    return 3 * f32_atol(n)
+
+
+def unit_grad_bounds(x, wg, wu, dy, activation):
+    """What dx, dwg and dwu may be off by, element by element, beyond their own rounding.  They are sums of products whose operands
+    da and db were rounded to the type, half a step h relative each: at most h times the sum of the terms' sizes, which is formed here
+    (|da| |Wg|^T + |db| |Wu|^T, |x|^T |da|, |x|^T |db|).  The f32 sums of n terms add n 2^-24 of the same, and the projections' errors
+    (f32 sums over D) 2^-24 (n + D) of the gradients' root mean square, three times (as for y)."""
+    half = torch.finfo(x.dtype).eps / 2 if x.dtype != torch.float32 else 0.0
+    x, wg, wu, dy = (t.detach().double().cpu() for t in (x, wg, wu, dy))
+    a, b = (x @ wg).requires_grad_(), (x @ wu).requires_grad_()
+    f = {'silu': torch.nn.functional.silu, 'gelu': torch.nn.functional.gelu, 'sigmoid': torch.sigmoid}[activation]
+    da, db = (t.abs() for t in torch.autograd.grad(f(a) * b, (a, b), dy))
+    sizes = (da @ wg.abs().t() + db @ wu.abs().t(), x.abs().t() @ da, x.abs().t() @ db)
+    terms = (2 * wg.size(1), x.size(0), x.size(0))
+    return [((half + n * 2.0 ** -24) * s, 3 * f32_atol(n + x.size(1))) for s, n in zip(sizes, terms)]

@@ -107,3 +107,79 @@ def test_step_refusals(state, slots, said):
     from blocks.delta_rule import gated_delta_step
     with pytest.raises(ValueError, match=said):
         gated_delta_step(*(x[:, 0] for x in _rule_args().values()), state, slots=slots)
+
+
+def test_philox_reference_has_the_published_vectors():
+    """Random123's known answers for philox4x32-10: counter and key all zeros, and all ones."""
+    import seq_reference as R
+
+    def words(bits):
+        return [int(bits[2 * i]) | int(bits[2 * i + 1]) << 16 for i in range(4)]
+
+    assert words(R.philox_bits(8, 0, 0)) == [0x6627e8d5, 0xe169c58d, 0xbc57ac4c, 0x9b00dbd8]
+
+
+@pytest.mark.parametrize('args, kw, said', [
+    ((torch.zeros(3, dtype=torch.int32), 0.5, 1), {}, 'x must be'), ((torch.zeros(3), -0.1, 1), {}, 'p must'),
+    ((torch.zeros(3), 1.1, 1), {}, 'p must'), ((torch.zeros(3), float('nan'), 1), {}, 'p must'),
+    ((torch.zeros(3), 0.5, 1), dict(residual=torch.zeros(4)), 'residual'),
+    ((torch.zeros(3), 0.5, 1), dict(residual=torch.zeros(3).half()), 'residual'),
+    ((torch.zeros(3), 0.5, torch.zeros(2, dtype=torch.int64)), {}, 'seed'), ((torch.zeros(3), 0.5, torch.zeros(1)), {}, 'seed')])
+def test_dropout_refusals(args, kw, said):
+    from blocks.dropout import dropout
+    with pytest.raises(ValueError, match=said):
+        dropout(*args, **kw)
+
+
+def test_dropout_refuses_host_tensors_and_bad_c_calls():
+    from admm_amd import _seq_native as N
+    from blocks.dropout import dropout
+    with pytest.raises(RuntimeError, match='HIP device'):
+        dropout(torch.zeros(3), 0.5, 1)
+    lib = N.load()
+    assert lib.seq_dropout(5, 1, None, 1, 4, 0, 0, 0, None, 0, None) == -1
+    assert lib.seq_dropout(0, 1, None, 1, -4, 0, 0, 0, None, 0, None) == -1
+    assert lib.seq_dropout(0, 1, None, 1, 4, 65537, 0, 0, None, 0, None) == -1
+    assert lib.seq_dropout(0, None, None, 1, 4, 0, 0, 0, None, 0, None) == -1
+    assert lib.seq_dropout(0, None, None, None, 0, 0, 0, 0, None, 0, None) == 0
+
+
+@pytest.mark.parametrize('x, wg, wu, kw, said', [
+    (torch.zeros(2, 4).double(), torch.zeros(4, 3).double(), torch.zeros(4, 3).double(), {}, 'x must be'),
+    (torch.zeros(2, 4), torch.zeros(4, 3).half(), torch.zeros(4, 3), {}, 'w_gate must have'),
+    (torch.zeros(2, 4), torch.zeros(5, 3), torch.zeros(4, 3), {}, 'w_gate must be'),
+    (torch.zeros(2, 4), torch.zeros(4, 3), torch.zeros(4), {}, 'w_up must be'),
+    (torch.zeros(2, 4), torch.zeros(4, 3), torch.zeros(4, 2), {}, 'differ in shape'),
+    (torch.zeros(2, 4), torch.zeros(4, 0), torch.zeros(4, 0), {}, 'between 1 x 1'),
+    (torch.zeros(2, 0), torch.zeros(0, 3), torch.zeros(0, 3), {}, 'between 1 x 1'),
+    (torch.zeros(()), torch.zeros(4, 3), torch.zeros(4, 3), {}, 'one axis'),
+    (torch.zeros(2, 4), torch.zeros(4, 3), torch.zeros(4, 3), dict(activation='relu'), 'activation')])
+def test_unit_refusals(x, wg, wu, kw, said):
+    from blocks.gated_unit import gated_unit
+    with pytest.raises(ValueError, match=said):
+        gated_unit(x, wg, wu, **kw)
+
+
+def test_unit_refuses_host_tensors_and_bad_c_calls():
+    from admm_amd import _seq_native as N
+    from blocks.gated_unit import gated_unit
+    with pytest.raises(RuntimeError, match='HIP device'):
+        gated_unit(torch.zeros(2, 4), torch.zeros(4, 3), torch.zeros(4, 3))
+    lib, n = N.load(), ctypes.c_int64()
+
+    def bad(said, **kw):
+        u = N.SeqUnit(M=4, D=8, F=8, x_ld=8, wg_ld=8, wu_ld=8)
+        for name, v in kw.items():
+            setattr(u, name, v)
+        assert lib.seq_unit_workspace(ctypes.byref(u), 0, ctypes.byref(n)) == -1 and said in lib.seq_last_error()
+
+    bad(b'dtype', dtype=7)
+    bad(b'activation', act=3)
+    bad(b'rows', M=-1)
+    bad(b'weights', D=0)
+    bad(b'weights', F=(1 << 20) + 1)
+    bad(b'too many', M=(1 << 31) - 1, F=1 << 20)
+    u = N.SeqUnit(M=4, D=7, F=7, x_ld=7, wg_ld=7, wu_ld=7)
+    assert lib.seq_unit_workspace(ctypes.byref(u), 1, ctypes.byref(n)) == 0 and n.value > 0
+    assert lib.seq_unit_forward(ctypes.byref(u), None, 0, None, None, None) == -1 and b'work memory' in lib.seq_last_error()
+    assert lib.seq_unit_backward(ctypes.byref(u), 256, n.value, None, None, 7, None, None, None, None) == -1
