@@ -6,59 +6,64 @@ namespace {
 
 // ------------------------------------------------------------------------------------------------- per chunk: X, P
 
-constexpr int kLd = kC + 4;   // row length of the f32 64 x 64 tiles in LDS
 constexpr int kLdY = 36;
 
-template <int DT, int KP, bool SAVE>
-constexpr int prep_lds() {
-  using S = DeltaShape<DT, KP, SAVE>;
-  const int mats = 2 * kC * kLd * 4 + 32 * kLdY * 4 + S::kXP;
-  return (S::kKQ > mats ? S::kKQ : mats) + 4 * kC * 4;
-}
+template <int DT, int KP, int C, bool SAVE>
+struct PrepLds {
+  using S = DeltaShape<DT, KP, C, SAVE>;
+  static constexpr int ld = C + 4;                 // row length of the f32 tiles
+  static constexpr int kq = 2 * S::NP * C * KP * 2;
+  static constexpr int xp = 2 * C * ld * 4 + (C / 2) * kLdY * 4;
+  static constexpr int mats = xp + (3 + S::NPP) * C * C * 2;
+  static constexpr int vec = kq > mats ? kq : mats;
+  static constexpr int bytes = vec + 4 * C * 4;
+};
 
-// f32 product of 16 x 16 tiles, inner length 16 n: C += A B with A(m, k) = a[m * lda + k], B(k, n) = b[k * ldb + n]
-__device__ __forceinline__ f32x4 mm16(const float* a, int lda, const float* b, int ldb, int n, int lane, f32x4 acc) {
+// f32 product of 16 x 16 tiles, inner length 16 n: A(m, k) = a[m * lda + k], B(k, n) = b[k * ldb + n]
+__device__ __forceinline__ f32x4 mm16(const float* a, int lda, const float* b, int ldb, int n, int lane) {
   const int m = lane & 15, g = lane >> 4;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   for (int k = 0; k < 16 * n; k += 4)
     acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[m * lda + k + g], b[(k + g) * ldb + m], acc, 0, 0, 0);
   return acc;
 }
 
-template <int DT, int KP, bool SAVE>
-__global__ __launch_bounds__(256) void k_delta_prep(DeltaArgs a) {
-  using S = DeltaShape<DT, KP, SAVE>;
+template <int DT, int KP, int C, bool SAVE>
+__global__ __launch_bounds__(4 * C) void k_delta_prep(DeltaArgs a) {
+  using S = DeltaShape<DT, KP, C, SAVE>;
+  using L = PrepLds<DT, KP, C, SAVE>;
   using T = typename Elem<DT>::T;
-  constexpr int NP = S::NP;
+  constexpr int NP = S::NP, W = S::RT, kThreads = 64 * W, kLd = L::ld, kTile = C * KP, kMat = C * C;
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  __bf16* kq = reinterpret_cast<__bf16*>(lds);
+  __bf16* const kq = reinterpret_cast<__bf16*>(lds);
   float* const A = reinterpret_cast<float*>(lds);           // after the Gram products: over K and Q
-  float* const X = A + kC * kLd;
-  float* const Y = X + kC * kLd;
-  __bf16* const xp = reinterpret_cast<__bf16*>(Y + 32 * kLdY);
-  float* const ghi = reinterpret_cast<float*>(lds + prep_lds<DT, KP, SAVE>() - 4 * kC * 4);
-  float* const glo = ghi + kC;
-  float* const bet = glo + kC;
-  int* const kbad = reinterpret_cast<int*>(bet + kC);   // rows of k that hold a NaN or infinity
+  float* const X = A + C * kLd;
+  float* const Y = X + C * kLd;
+  __bf16* const xp = reinterpret_cast<__bf16*>(lds + L::xp);   // planes of X, then of P
+  float* const ghi = reinterpret_cast<float*>(lds + L::vec);
+  float* const glo = ghi + C;
+  float* const bet = glo + C;
+  int* const kbad = reinterpret_cast<int*>(bet + C);   // rows of k that hold a NaN or infinity
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, m = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, wave = wave_id(), m = lane & 15, g = lane >> 4;
   const int64_t c = blockIdx.x / a.Hk;
   const int hk = (int)(blockIdx.x % a.Hk);
   const int64_t n = a.rows.find(c);
   int64_t begin, len, chunk0;
   a.rows.range(n, begin, len, chunk0);
-  const int64_t t0 = (c - chunk0) * kC;
+  const int64_t t0 = (c - chunk0) * C;
   if (t0 < 0 || t0 >= len) return;
-  const int rows = (int)(len - t0 < kC ? len - t0 : kC);
+  const int rows = (int)(len - t0 < C ? len - t0 : C);
   const int64_t bt = a.rows.batch(n), r0 = begin + t0;
 
-  // K and Q rows as planes, in LDS and in the work memory
-  if (tid < kC) kbad[tid] = 0;
+  // K and Q rows as planes in LDS
+  if (tid < C) kbad[tid] = 0;
   __syncthreads();
   {
     const T* kp = static_cast<const T*>(a.k) + bt * a.ks[0] + r0 * a.ks[1] + hk * a.ks[2];
     const T* qp = static_cast<const T*>(a.q) + bt * a.qs[0] + r0 * a.qs[1] + hk * a.qs[2];
-    for (int i = tid; i < 2 * kC * (KP / 8); i += 256) {
-      const int w = i / (kC * (KP / 8)), r = i / (KP / 8) % kC, p = i % (KP / 8);
+    for (int i = tid; i < 2 * C * (KP / 8); i += kThreads) {
+      const int w = i / (C * (KP / 8)), r = i / (KP / 8) % C, p = i % (KP / 8);
       const T* src = w ? qp + (int64_t)r * a.qs[1] : kp + (int64_t)r * a.ks[1];
       f32x8 x = {};
       const int left = a.K - 8 * p;
@@ -67,34 +72,46 @@ __global__ __launch_bounds__(256) void k_delta_prep(DeltaArgs a) {
       bf16x8 pl[NP];
       planes8<NP>(x, pl);
 #pragma unroll
-      for (int j = 0; j < NP; ++j)
-        *reinterpret_cast<bf16x8*>(kq + (w * NP + j) * S::kTile + tile_at<KP>(r, p)) = pl[j];
+      for (int j = 0; j < NP; ++j) *reinterpret_cast<bf16x8*>(kq + (w * NP + j) * kTile + tile_at<KP>(r, p)) = pl[j];
     }
   }
   __syncthreads();
-  for (int i = tid; i < kC * NP * (KP / 8); i += 256) {
+  for (int i = tid; i < C * NP * (KP / 8); i += kThreads) {
     const int r = i / (NP * (KP / 8)), j = i / (KP / 8) % NP;
-    if (kbad[r]) *reinterpret_cast<u32x4*>(kq + j * S::kTile + tile_at<KP>(r, i % (KP / 8))) = u32x4{0, 0, 0, 0};
+    if (kbad[r]) *reinterpret_cast<u32x4*>(kq + j * kTile + tile_at<KP>(r, i % (KP / 8))) = u32x4{0, 0, 0, 0};
   }
   __syncthreads();
+  // their fragments
   {
-    u32x4* dst = reinterpret_cast<u32x4*>(a.kq + (c * a.Hk + hk) * (int64_t)S::kKQ);
-    for (int i = tid; i < S::kKQ / 16; i += 256) dst[i] = reinterpret_cast<const u32x4*>(lds)[i];
+    char* dst = a.kq + (c * a.Hk + hk) * (int64_t)S::kKQ + lane * 16;
+#pragma unroll 1
+    for (int f = wave; f < S::fEnd; f += W) {
+      bf16x8 v[NP];
+      if (f < S::fKT) {
+        const int e = f < S::fQ ? f : f - S::fQ;
+        frag<KP, NP, kTile>(kq + (f < S::fQ ? 0 : NP * kTile), perm_row(e / S::KS, m), e % S::KS, g, v);
+      } else {
+        const int e = f < S::fQT ? f - S::fKT : f - S::fQT;
+        frag_t<KP, NP, kTile>(kq + (f < S::fQT ? 0 : NP * kTile), e / S::CS, e % S::CS, g, m, v);
+      }
+#pragma unroll
+      for (int j = 0; j < NP; ++j) *reinterpret_cast<bf16x8*>(dst + (f * NP + j) * 1024) = v[j];
+    }
   }
   // k_i . k_j and q_i . k_j, rows 16 wave..+15, columns up to the diagonal tile
-  f32x4 kk[4], qk[4];
+  f32x4 kk[S::RT], qk[S::RT];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) kk[j] = qk[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int j = 0; j < S::RT; ++j) kk[j] = qk[j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int s = 0; s < KP / 32; ++s) {
+  for (int s = 0; s < S::KS; ++s) {
     bf16x8 ka[NP], qa[NP];
-    frag<KP, NP, S::kTile>(kq, 16 * wave + m, s, g, ka);
-    frag<KP, NP, S::kTile>(kq + NP * S::kTile, 16 * wave + m, s, g, qa);
+    frag<KP, NP, kTile>(kq, 16 * wave + m, s, g, ka);
+    frag<KP, NP, kTile>(kq + NP * kTile, 16 * wave + m, s, g, qa);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < S::RT; ++j) {
       if (j > wave) continue;
       bf16x8 kb[NP];
-      frag<KP, NP, S::kTile>(kq, 16 * j + m, s, g, kb);
+      frag<KP, NP, kTile>(kq, 16 * j + m, s, g, kb);
       kk[j] = mfma_planes<NP, NP, 3>(ka, kb, kk[j]);
       qk[j] = mfma_planes<NP, NP, 3>(qa, kb, qk[j]);
     }
@@ -110,25 +127,27 @@ __global__ __launch_bounds__(256) void k_delta_prep(DeltaArgs a) {
       float gv = in ? a.g[bt * a.gs[0] + (r0 + lane) * a.gs[1] + h * a.gs[2]] : 0.f;
       float bv = in ? a.beta[bt * a.bs[0] + (r0 + lane) * a.bs[1] + h * a.bs[2]] : 0.f;
       gv = gv < kMinG ? kMinG : gv;
-      const uint64_t odd = __ballot((gv - gv) + (bv - bv) != 0.f || kbad[lane]);
-      const int bad = odd ? __ffsll((unsigned long long)odd) - 1 : kC;
+      const uint64_t odd = __ballot((gv - gv) + (bv - bv) != 0.f || (lane < C && kbad[lane < C ? lane : 0]));
+      const int bad = odd ? __ffsll((unsigned long long)odd) - 1 : C;
       if (lane >= bad) gv = bv = 0.f;
       double last;
       const double sum = running_sum(gv, lane, last);
       const float hi = (float)sum;
-      ghi[lane] = hi;
-      glo[lane] = (float)(sum - (double)hi);
-      bet[lane] = bv;
-      float* vec = reinterpret_cast<float*>(a.vec + ch * (int64_t)S::kVec);
+      if (lane < C) {
+        ghi[lane] = hi;
+        glo[lane] = (float)(sum - (double)hi);
+        bet[lane] = bv;
+      }
+      float* vec = reinterpret_cast<float*>(a.vec + ch * (int64_t)kVec);
       vec[lane] = expf((float)sum);
-      vec[kC + lane] = expf((float)(last - sum));
-      vec[2 * kC + lane] = bv;
-      vec[3 * kC + lane] = lane == 1 ? (float)bad : expf((float)last);
+      vec[64 + lane] = expf((float)(last - sum));
+      vec[128 + lane] = bv;
+      vec[192 + lane] = lane == 1 ? (float)bad : expf((float)last);
     }
     __syncthreads();
-    for (int i = tid; i < kC * kLd; i += 256) X[i] = 0.f;
+    for (int i = tid; i < C * kLd; i += kThreads) X[i] = 0.f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < S::RT; ++j) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int row = 16 * wave + 4 * g + r, col = 16 * j + m;
@@ -136,20 +155,18 @@ __global__ __launch_bounds__(256) void k_delta_prep(DeltaArgs a) {
         const float d = lower ? expf((ghi[row] - ghi[col]) + (glo[row] - glo[col])) : 0.f;
         A[row * kLd + col] = col < row ? bet[row] * d * kk[j][r] : 0.f;
         const float p = lower ? a.scale * d * qk[j][r] : 0.f;
-        if (row >= 32 || col < 32) {
-          __bf16* pp = xp + 3 * kTri + tri_at(row, col >> 3) + (col & 7);
-          const __bf16 p0 = (__bf16)p;
-          const float q1 = p - (float)p0;
-          const __bf16 p1 = (__bf16)q1;
-          pp[0] = p0;
-          pp[kTri] = p1;
-          if constexpr (S::NPP > 2) pp[2 * kTri] = (__bf16)(q1 - (float)p1);
-        }
+        __bf16* pp = xp + 3 * kMat + tile_at<C>(row, col >> 3) + (col & 7);
+        const __bf16 p0 = (__bf16)p;
+        const float q1 = p - (float)p0;
+        const __bf16 p1 = (__bf16)q1;
+        pp[0] = p0;
+        pp[kMat] = p1;
+        if constexpr (S::NPP > 2) pp[2 * kMat] = (__bf16)(q1 - (float)p1);
       }
     }
     __syncthreads();
-    // X = (I + A)^-1: the four diagonal 16 x 16 blocks by substitution (a lane has one column), then joined in pairs
-    if (wave == 0) {
+    // X = (I + A)^-1: the diagonal 16 x 16 blocks by substitution (a lane has one column), then joined in pairs
+    if (wave == 0 && g < S::RT) {
       float x[16];
       const float* blk = A + (16 * g) * kLd + 16 * g;
 #pragma unroll
@@ -163,239 +180,330 @@ __global__ __launch_bounds__(256) void k_delta_prep(DeltaArgs a) {
       for (int i = 0; i < 16; ++i) X[(16 * g + i) * kLd + 16 * g + m] = x[i];
     }
     __syncthreads();
-    const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-    if (wave < 2) {   // [X11 0; -X22 A21 X11  X22], 16 rows each
-      const float* a21 = A + (32 * wave + 16) * kLd + 32 * wave;
-      const f32x4 y = mm16(a21, kLd, X + 32 * wave * kLd + 32 * wave, kLd, 1, lane, zero);
+    if (wave < C / 32) {   // [X11 0; -X22 A21 X11  X22], 16 rows each
+      const f32x4 y = mm16(A + (32 * wave + 16) * kLd + 32 * wave, kLd, X + 32 * wave * kLd + 32 * wave, kLd, 1, lane);
 #pragma unroll
       for (int r = 0; r < 4; ++r) Y[(16 * wave + 4 * g + r) * kLdY + m] = y[r];
     }
     __syncthreads();
-    if (wave < 2) {
-      const f32x4 z = mm16(X + (32 * wave + 16) * kLd + 32 * wave + 16, kLd, Y + 16 * wave * kLdY, kLdY, 1, lane, zero);
+    if (wave < C / 32) {
+      const f32x4 z = mm16(X + (32 * wave + 16) * kLd + 32 * wave + 16, kLd, Y + 16 * wave * kLdY, kLdY, 1, lane);
 #pragma unroll
       for (int r = 0; r < 4; ++r) X[(32 * wave + 16 + 4 * g + r) * kLd + 32 * wave + m] = -z[r];
     }
     __syncthreads();
-    const int ti = wave >> 1, tj = wave & 1;
-    {
-      const f32x4 y = mm16(A + (32 + 16 * ti) * kLd, kLd, X + 16 * tj, kLd, 2, lane, zero);
+    if constexpr (C == 64) {   // the same of 32 rows each, a wave has one 16 x 16 tile
+      const int ti = wave >> 1, tj = wave & 1;
+      const f32x4 y = mm16(A + (32 + 16 * ti) * kLd, kLd, X + 16 * tj, kLd, 2, lane);
 #pragma unroll
       for (int r = 0; r < 4; ++r) Y[(16 * ti + 4 * g + r) * kLdY + 16 * tj + m] = y[r];
-    }
-    __syncthreads();
-    {
-      const f32x4 z = mm16(X + (32 + 16 * ti) * kLd + 32, kLd, Y + 16 * tj, kLdY, 2, lane, zero);
+      __syncthreads();
+      const f32x4 z = mm16(X + (32 + 16 * ti) * kLd + 32, kLd, Y + 16 * tj, kLdY, 2, lane);
 #pragma unroll
       for (int r = 0; r < 4; ++r) X[(32 + 16 * ti + 4 * g + r) * kLd + 16 * tj + m] = -z[r];
+      __syncthreads();
     }
-    __syncthreads();
-    for (int i = tid; i < kC * kC / 8; i += 256) {
-      const int r = i >> 3, p = i & 7;
-      if (r < 32 && p >= 4) continue;
+    for (int i = tid; i < C * C / 8; i += kThreads) {
+      const int r = i / (C / 8), p = i % (C / 8);
       const f32x4* src = reinterpret_cast<const f32x4*>(X + r * kLd + 8 * p);
       bf16x8 pl[3];
       planes8<3>(cat8(src[0], src[1]), pl);
 #pragma unroll
-      for (int j = 0; j < 3; ++j) *reinterpret_cast<bf16x8*>(xp + j * kTri + tri_at(r, p)) = pl[j];
+      for (int j = 0; j < 3; ++j) *reinterpret_cast<bf16x8*>(xp + j * kMat + tile_at<C>(r, p)) = pl[j];
     }
     __syncthreads();
-    u32x4* dst = reinterpret_cast<u32x4*>(a.xp + ch * (int64_t)S::kXP);
-    for (int i = tid; i < S::kXP / 16; i += 256) dst[i] = reinterpret_cast<const u32x4*>(xp)[i];
+    char* dst = a.xp + ch * (int64_t)S::kXP + lane * 16;
+#pragma unroll 1
+    for (int f = wave; f < (SAVE ? 4 : 2) * S::TRI; f += W) {
+      const int kind = f / S::TRI, e = f % S::TRI;   // X, P, X^T, P^T
+      const int np = kind & 1 ? S::NPP : 3;
+      const __bf16* src = xp + (kind & 1 ? 3 * kMat : 0);
+      char* p = dst + (kind == 0 ? S::pX : kind == 1 ? S::pP : kind == 2 ? S::pXT : S::pPT) * 1024 + e * np * 1024;
+      for (int j = 0; j < np; ++j) {
+        bf16x8 v[1];
+        if (kind < 2) {
+          const int t = e < 2 ? e : 2 + ((e - 2) >> 1), s = e < 2 ? 0 : (e - 2) & 1;
+          frag<C, 1, kMat>(src + j * kMat, perm_row(t, m), s, g, v);
+        } else {
+          const int t = C == 32 || e >= 4 ? (C == 32 ? e : e - 2) : e >> 1, s = C == 32 ? 0 : e >= 4 ? 1 : e & 1;
+          frag_t<C, 1, kMat>(src + j * kMat, t, s, g, m, v);
+        }
+        *reinterpret_cast<bf16x8*>(p + j * 1024) = v[0];
+      }
+    }
   }
 }
 
 // --------------------------------------------------------------------------------------------- chunk after chunk
 
-template <int DT, int KP, int WAVES, bool SAVE>
-__global__ __launch_bounds__(64 * WAVES) void k_delta_scan(DeltaArgs a) {
-  using S = DeltaShape<DT, KP, SAVE>;
+// A workgroup owns NC tiles of 16 columns, from the first chunk to the last; its C / 16 waves share the rows.  Wave w forms rows
+// perm_row(w, .) of K S, Q S, u and o, and keeps TW tiles of the state in registers; what a product needs of the other waves'
+// results (S, beta (v - exp(G_i) K S), u) goes through LDS as planes in operand order, three barriers a chunk.  The fragments of
+// the next chunk are loaded as soon as those of this one are used.  Bound by the chain of products and exchanges of a chunk
+// (with few heads) or by issue and LDS (with many): one wave for all rows took four times as long for a chunk.
+template <int DT, int KP, int C, int NC, bool SAVE>
+struct Scan {
+  using S = DeltaShape<DT, KP, C, SAVE>;
+  static constexpr int TW = S::KT >= S::RT ? S::KT / S::RT : 1;
+  static constexpr int bS = 0, bR = S::KS * 3, bU = bR + S::CS * 3, bL = bU + S::CS * S::NO, bEnd = bL + S::CS * 3;   // KB
+  static constexpr int bad = NC * bEnd * 1024, bytes = bad + NC * 16 * S::RT * 4;
+};
+
+template <int DT, int KP, int C, int NC, bool SAVE>
+__global__ __launch_bounds__(4 * C) void k_delta_scan(DeltaArgs a) {
+  using S = DeltaShape<DT, KP, C, SAVE>;
+  using Sc = Scan<DT, KP, C, NC, SAVE>;
   using T = typename Elem<DT>::T;
-  constexpr int NP = S::NP, NO = S::NO, NB = scan_bufs<DT, KP, SAVE>(), KS = KP / 32;
+  constexpr int NP = S::NP, NO = S::NO, TW = Sc::TW;
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, x = lane & 15, g = lane >> 4;
-  // workgroups go to the eight XCDs in turn: those of one head (which read the same planes) share one XCD's L2
-  const int vg = (a.VP / 16 + WAVES - 1) / WAVES;
-  const int64_t heads = a.rows.N * a.Hv;
-  const int64_t head = (int64_t)(blockIdx.x / 8 / vg) * 8 + blockIdx.x % 8;
-  if (head >= heads) return;
+  const int lane = threadIdx.x & 63, w = wave_id(), x = lane & 15, g = lane >> 4;
+  const int groups = (a.VP / 16 + NC - 1) / NC;
+  int64_t head;
+  int group;
+  if (!place_columns(a.rows.N * a.Hv, groups, head, group)) return;
   const int64_t n = head / a.Hv;
   const int h = (int)(head % a.Hv), hk = h / (a.Hv / a.Hk);
-  const int col = ((int)(blockIdx.x / 8 % vg) * WAVES + wave) * 16 + x;   // the lane's column
-  const bool in = col < a.V;
+  const int col0 = group * NC * 16 + x;   // the lane's column in the first tile
   int64_t begin, len, c0;
   a.rows.range(n, begin, len, c0);
-  const int64_t nc = (len + kC - 1) / kC;
+  const int64_t nc = (len + C - 1) / C;
+  const bool holds = w * TW < S::KT;      // whether this wave has tiles of the state
+  const int row0 = perm_row(w, 4 * g);    // its rows of a chunk: row0..row0 + 3
+  const float nan = __builtin_nanf("");
 
-  f32x4 st[KP / 16];   // tile t, register r: row perm_row(t, 4 g + r) of the state
+  f32x4 st[NC][TW];
 #pragma unroll
-  for (int t = 0; t < KP / 16; ++t)
+  for (int i = 0; i < NC; ++i)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int kd = perm_row(t, 4 * g + r);
-      st[t][r] = a.initial && in && kd < a.K ? a.initial[(head * a.K + kd) * a.V + col] : 0.f;
-    }
+    for (int t = 0; t < TW; ++t)
+      st[i][t] = load_state(a.initial && holds ? a.initial + head * a.K * a.V : nullptr, a.K, a.V, col0 + 16 * i, w * TW + t, g);
 
-  const T* vp = static_cast<const T*>(a.v) + a.rows.batch(n) * a.vs[0] + begin * a.vs[1] + h * a.vs[2] + col;
-  T* op = static_cast<T*>(a.o) + ((a.rows.batch(n) * a.rows.T + begin) * a.Hv + h) * (int64_t)a.V + col;
+  const char* kq = a.kq + (c0 * a.Hk + hk) * (int64_t)S::kKQ;
+  const char* xp = a.xp + (c0 * a.Hv + h) * (int64_t)S::kXP;
+  const float* vec = reinterpret_cast<const float*>(a.vec + (c0 * a.Hv + h) * (int64_t)kVec);
+  const int64_t kq_step = (int64_t)a.Hk * S::kKQ, xp_step = (int64_t)a.Hv * S::kXP, vec_step = (int64_t)a.Hv * (kVec / 4);
+  const T* vp[NC];
+  T* op[NC];
+  bool in[NC];
   const int64_t orow = (int64_t)a.Hv * a.V;
-  f32x4 v[4];   // rows perm_row(t, 4 g + r) of the chunk
-  auto load_v = [&](int64_t t0) {
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+  for (int i = 0; i < NC; ++i) {
+    const int col = col0 + 16 * i;
+    in[i] = col < a.V;
+    vp[i] = static_cast<const T*>(a.v) + a.rows.batch(n) * a.vs[0] + begin * a.vs[1] + h * a.vs[2] + (in[i] ? col : a.V - 1);
+    op[i] = static_cast<T*>(a.o) + ((a.rows.batch(n) * a.rows.T + begin) * a.Hv + h) * (int64_t)a.V + col + row0 * orow;
+  }
+
+  bf16x8 fk[S::KS][NP], fq[S::KS][NP], fx[S::CS][3], fp[S::CS][NO], ft[TW][S::CS][NP];
+  f32x4 into, left, beta;
+  float all = 0.f, first_bad = 0.f;
+  ColumnRows<T> v[NC];
+  auto load_kq = [&](const char* p) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int64_t row = t0 + perm_row(t, 4 * g + r);
-        v[t][r] = in && row < len ? (float)vp[row * a.vs[1]] : 0.f;
+    for (int s = 0; s < S::KS; ++s) {
+      load_frag<NP>(p, (S::fK + w * S::KS + s) * NP, lane, fk[s]);
+      load_frag<NP>(p, (S::fQ + w * S::KS + s) * NP, lane, fq[s]);
+    }
+  };
+  auto load_x = [&](const char* p) {   // (rows of the upper half have no second inner step: theirs is loaded, not used)
+#pragma unroll
+    for (int s = 0; s < S::CS; ++s) load_frag<3>(p, S::pX + 3 * tri_frag(w, s <= w / 2 ? s : 0), lane, fx[s]);
+  };
+  auto load_pt = [&](const char* p, const char* k) {
+#pragma unroll
+    for (int s = 0; s < S::CS; ++s) load_frag<NO>(p, S::pP + S::NPP * tri_frag(w, s <= w / 2 ? s : 0), lane, fp[s]);
+    if (holds) {
+#pragma unroll
+      for (int t = 0; t < TW; ++t)
+#pragma unroll
+        for (int s = 0; s < S::CS; ++s) load_frag<NP>(k, (S::fKT + (w * TW + t) * S::CS + s) * NP, lane, ft[t][s]);
+    }
+  };
+  auto load_v = [&](int64_t ci) {
+    const int rows = (int)(len - ci * C < C ? len - ci * C : C);
+#pragma unroll
+    for (int i = 0; i < NC; ++i) v[i].load(vp[i] + ci * C * a.vs[1], a.vs[1], rows, row0);
+  };
+  auto load_vec = [&](const float* p) {
+    into = *reinterpret_cast<const f32x4*>(p + row0);
+    left = *reinterpret_cast<const f32x4*>(p + 64 + row0);
+    beta = *reinterpret_cast<const f32x4*>(p + 128 + row0);
+    all = p[192];
+    first_bad = p[193];
+  };
+  auto put_state = [&]() {
+    if (!holds) return;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      char* b = lds + (i * Sc::bEnd + Sc::bS) * 1024;
+      if constexpr (TW >= 2) {
+#pragma unroll
+        for (int t = 0; t < TW; t += 2) put_whole<3>(b, (w * TW + t) / 2, lane, cat8(st[i][t], st[i][t + 1]));
+      } else {
+        put_half<3>(b, w / 2, w & 1, lane, st[i][0]);
       }
+    }
   };
   if (nc > 0) {
-    stage_chunk<S, WAVES>(a, c0, hk, h, lds, wave, lane);
+    load_kq(kq);
     load_v(0);
+    load_vec(vec);
+    load_x(xp);
+    load_pt(xp, kq);
+    put_state();
   }
+  int* const bads = reinterpret_cast<int*>(lds + Sc::bad);
   for (int64_t ci = 0; ci < nc; ++ci) {
-    const char* buf = lds + (NB == 2 ? (ci & 1) * S::kStage : 0);
-    vm_wait();
-    __syncthreads();
-    f32x4 vc[4];
-#pragma unroll
-    for (int t = 0; t < 4; ++t) vc[t] = v[t];
-    if (ci + 1 < nc) {
-      if (NB == 2) stage_chunk<S, WAVES>(a, c0 + ci + 1, hk, h, lds + ((ci + 1) & 1) * S::kStage, wave, lane);
-      load_v((ci + 1) * kC);
-    }
-    const __bf16* Kt = reinterpret_cast<const __bf16*>(buf);
-    const __bf16* Qt = Kt + NP * S::kTile;
-    const __bf16* Xt = reinterpret_cast<const __bf16*>(buf + S::kKQ);
-    const __bf16* Pt = Xt + 3 * kTri;
-    const float* vec = reinterpret_cast<const float*>(buf + S::kKQ + S::kXP);
+    const bool more = ci + 1 < nc;   // behind the last chunk its own values are loaded again, and not used
     const int64_t ch = (c0 + ci) * a.Hv + h;
-    if (SAVE && col < a.VP) {
-      float* s0 = a.s0 + ch * (int64_t)KP * a.VP + col;
+    const int rows = (int)(len - ci * C < C ? len - ci * C : C);
+    f32x4 vc[NC];
 #pragma unroll
-      for (int t = 0; t < KP / 16; ++t)
+    for (int i = 0; i < NC; ++i) vc[i] = v[i].get(in[i], row0);
+    lds_barrier();   // the state is in LDS
+    if (SAVE && holds) {
+      float* s0 = a.s0 + ch * (int64_t)KP * a.VP + col0;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s0[(int64_t)perm_row(t, 4 * g + r) * a.VP] = st[t][r];
+      for (int i = 0; i < NC; ++i)
+#pragma unroll
+        for (int t = 0; t < TW; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (col0 + 16 * i < a.VP) s0[(int64_t)perm_row(w * TW + t, 4 * g + r) * a.VP + 16 * i] = st[i][t][r];
     }
-    // K S and Q S
-    f32x4 ks[4], o[4];
+    // K S and Q S, the inner steps in two chains
+    f32x4 ks[NC], o[NC], ks2[NC], o2[NC];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) ks[t] = o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < NC; ++i) ks[i] = o[i] = ks2[i] = o2[i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      bf16x8 sp[3];
-      planes8<3>(cat8(st[2 * s], st[2 * s + 1]), sp);
-      bf16x8 so[NO];
+    for (int s = 0; s < S::KS; ++s) {
 #pragma unroll
-      for (int i = 0; i < NO; ++i) so[i] = sp[i];
+      for (int i = 0; i < NC; ++i) {
+        bf16x8 sp[3], so[NO];
+        get_operand<3>(lds + (i * Sc::bEnd + Sc::bS) * 1024, s, lane, sp);
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        bf16x8 fa[NP];
-        frag<KP, NP, S::kTile>(Kt, perm_row(t, x), s, g, fa);
-        ks[t] = mfma_planes<NP, 3, 3>(fa, sp, ks[t]);
-        frag<KP, NP, S::kTile>(Qt, perm_row(t, x), s, g, fa);
-        o[t] = mfma_planes<NP, NO, NO>(fa, so, o[t]);
+        for (int j = 0; j < NO; ++j) so[j] = sp[j];
+        f32x4& k = s & 1 ? ks2[i] : ks[i];
+        f32x4& q = s & 1 ? o2[i] : o[i];
+        k = mfma_planes<NP, 3, 3>(fk[s], sp, k);
+        q = mfma_planes<NP, NO, NO>(fq[s], so, q);
       }
     }
-    // beta (v - exp(G) K S), and u = X of it
-    bf16x8 rp[2][3];
-    int bad = (int)vec[3 * kC + 1];
+    if (more) kq += kq_step;
+    load_kq(kq);
+    // beta (v - exp(G_i) K S)
+    const int bad0 = (int)first_bad;
     float odd = 0.f;
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const int i0 = perm_row(t, 4 * g);
-      const f32x4 into = *reinterpret_cast<const f32x4*>(vec + i0), b = *reinterpret_cast<const f32x4*>(vec + 2 * kC + i0);
-      ks[t] = b * (vc[t] - into * ks[t]);
-      o[t] = (a.scale * into) * o[t];
-      odd += zero_if_finite(ks[t]);
+    for (int i = 0; i < NC; ++i) {
+      ks[i] = beta * (vc[i] - into * (ks[i] + ks2[i]));
+      o[i] = (a.scale * into) * (o[i] + o2[i]);
+      odd += zero_if_finite(ks[i]);
     }
+    int bad[NC];
+#pragma unroll
+    for (int i = 0; i < NC; ++i) bad[i] = bad0;
     if (__ballot(odd != 0.f)) {
 #pragma unroll
-      for (int t = 3; t >= 0; --t)
+      for (int i = 0; i < NC; ++i) {
 #pragma unroll
         for (int r = 3; r >= 0; --r)
-          if (ks[t][r] - ks[t][r] != 0.f) {
-            ks[t][r] = 0.f;
-            const int row = perm_row(t, 4 * g + r);
-            bad = row < bad ? row : bad;
+          if (ks[i][r] - ks[i][r] != 0.f) {
+            ks[i][r] = 0.f;
+            bad[i] = row0 + r < bad[i] ? row0 + r : bad[i];
           }
-      bad = min(bad, __shfl_xor(bad, 16));
-      bad = min(bad, __shfl_xor(bad, 32));
-    }
-#pragma unroll
-    for (int s = 0; s < 2; ++s) planes8<3>(cat8(ks[2 * s], ks[2 * s + 1]), rp[s]);
-    f32x4 u[4];
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      u[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int s = 0; s <= t / 2; ++s) {
-        bf16x8 fa[3];
-        frag_tri(Xt, t, s, g, x, fa);
-        u[t] = mfma_planes<3, 3, 3>(fa, rp[s], u[t]);
+        bad[i] = min(bad[i], __shfl_xor(bad[i], 16));
+        bad[i] = min(bad[i], __shfl_xor(bad[i], 32));
       }
     }
-    const float nan = __builtin_nanf("");
-    if (SAVE && col < a.VP) {
-      float* us = a.u + ch * (int64_t)kC * a.VP + col;
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) us[(int64_t)perm_row(t, 4 * g + r) * a.VP] = perm_row(t, 4 * g + r) >= bad ? nan : u[t][r];
+    for (int i = 0; i < NC; ++i) {
+      put_half<3>(lds + (i * Sc::bEnd + Sc::bR) * 1024, w / 2, w & 1, lane, ks[i]);
+      if (g == 0) bads[(i * 16 + x) * S::RT + w] = bad[i];
     }
+    lds_barrier();
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+#pragma unroll
+      for (int r = 0; r < S::RT; ++r) bad[i] = min(bad[i], bads[(i * 16 + x) * S::RT + r]);
+    // u = X of it
+    f32x4 u[NC];
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      f32x4 u2 = {0.f, 0.f, 0.f, 0.f};
+      u[i] = u2;
+      bf16x8 rp[3];
+      get_operand<3>(lds + (i * Sc::bEnd + Sc::bR) * 1024, 0, lane, rp);
+      u[i] = mfma_planes<3, 3, 3>(fx[0], rp, u[i]);
+      if (S::CS > 1 && w >= 2) {
+        get_operand<3>(lds + (i * Sc::bEnd + Sc::bR) * 1024, S::CS - 1, lane, rp);
+        u2 = mfma_planes<3, 3, 3>(fx[S::CS - 1], rp, u2);
+      }
+      u[i] += u2;
+      put_half<NO>(lds + (i * Sc::bEnd + Sc::bU) * 1024, w / 2, w & 1, lane, u[i]);
+      put_half<3>(lds + (i * Sc::bEnd + Sc::bL) * 1024, w / 2, w & 1, lane, left * u[i]);
+    }
+    if (more) xp += xp_step;
+    load_x(xp);
+    const float all_now = all;
+    if (more) vec += vec_step;
+    load_vec(vec);
+    load_v(more ? ci + 1 : ci);
+    lds_barrier();
     // o += P u
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
+    for (int i = 0; i < NC; ++i) {
       bf16x8 up[NO];
-      planes8<NO>(cat8(u[2 * s], u[2 * s + 1]), up);
-#pragma unroll
-      for (int t = 2 * s; t < 4; ++t) {
-        bf16x8 fa[NO];
-        frag_tri(Pt, t, s, g, x, fa);
-        o[t] = mfma_planes<NO, NO, NO>(fa, up, o[t]);
+      get_operand<NO>(lds + (i * Sc::bEnd + Sc::bU) * 1024, 0, lane, up);
+      o[i] = mfma_planes<NO, NO, NO>(fp[0], up, o[i]);
+      if (S::CS > 1 && w >= 2) {
+        get_operand<NO>(lds + (i * Sc::bEnd + Sc::bU) * 1024, S::CS - 1, lane, up);
+        o[i] = mfma_planes<NO, NO, NO>(fp[S::CS - 1], up, o[i]);
       }
     }
-    // S <- exp(G_63) S + K^T (exp(G_63 - G) u)
-    const float all = vec[3 * kC];
+    // S <- exp(G) S + K^T (exp(G - G_i) u)
+    if (holds) {
 #pragma unroll
-    for (int t = 0; t < KP / 16; ++t) st[t] *= all;
+      for (int i = 0; i < NC; ++i) {
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      bf16x8 up[3];
-      const f32x4 l0 = *reinterpret_cast<const f32x4*>(vec + kC + perm_row(2 * s, 4 * g));
-      const f32x4 l1 = *reinterpret_cast<const f32x4*>(vec + kC + perm_row(2 * s + 1, 4 * g));
-      planes8<3>(cat8(l0 * u[2 * s], l1 * u[2 * s + 1]), up);
+        for (int t = 0; t < TW; ++t) st[i][t] *= all_now;
 #pragma unroll
-      for (int t = 0; t < KP / 16; ++t) {
-        bf16x8 fa[NP];
-        frag_t<KP, NP, S::kTile>(Kt, t, s, g, x, fa);
-        st[t] = mfma_planes<NP, 3, 3>(fa, up, st[t]);
+        for (int s = 0; s < S::CS; ++s) {
+          bf16x8 up[3];
+          get_operand<3>(lds + (i * Sc::bEnd + Sc::bL) * 1024, s, lane, up);
+#pragma unroll
+          for (int t = 0; t < TW; ++t) st[i][t] = mfma_planes<NP, 3, 3>(ft[t][s], up, st[i][t]);
+        }
+        if (bad[i] < C) {
+#pragma unroll
+          for (int t = 0; t < TW; ++t) st[i][t] = f32x4{nan, nan, nan, nan};
+        }
       }
     }
+    load_pt(xp, kq);
+    put_state();
+    // out, values from the first row that is not finite on as NaN
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+    for (int i = 0; i < NC; ++i) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int64_t row = ci * kC + perm_row(t, 4 * g + r);
-        if (in && row < len) op[row * orow] = (T)(perm_row(t, 4 * g + r) >= bad ? nan : o[t][r]);
+        const bool gone = row0 + r >= bad[i];
+        if (SAVE && col0 + 16 * i < a.VP) a.u[(ch * C + row0 + r) * (int64_t)a.VP + col0 + 16 * i] = gone ? nan : u[i][r];
+        if (in[i] && row0 + r < rows) op[i][r * orow] = (T)(gone ? nan : o[i][r]);
       }
-    if (bad < kC) {
-#pragma unroll
-      for (int t = 0; t < KP / 16; ++t) st[t] = f32x4{nan, nan, nan, nan};
-    }
-    if (NB == 1 && ci + 1 < nc) {
-      __syncthreads();
-      stage_chunk<S, WAVES>(a, c0 + ci + 1, hk, h, lds, wave, lane);
+      op[i] += C * orow;
     }
   }
-  if (in) {
+  if (holds) {
 #pragma unroll
-    for (int t = 0; t < KP / 16; ++t)
+    for (int i = 0; i < NC; ++i)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int kd = perm_row(t, 4 * g + r);
-        if (kd < a.K) a.final[(head * a.K + kd) * a.V + col] = st[t][r];
-      }
+      for (int t = 0; t < TW; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int kd = perm_row(w * TW + t, 4 * g + r);
+          if (in[i] && kd < a.K) a.final[(head * a.K + kd) * a.V + col0 + 16 * i] = st[i][t][r];
+        }
   }
 }
 
@@ -411,24 +519,29 @@ __global__ void k_delta_outside(DeltaRows rows, void* p, int64_t row) {
   }
 }
 
-template <int DT, int KP, bool SAVE>
-hipError_t forward(const DeltaArgs& a, hipStream_t s) {
-  using S = DeltaShape<DT, KP, SAVE>;
-  constexpr int W = 4;
-  hipError_t e = allow_lds(k_delta_prep<DT, KP, SAVE>, prep_lds<DT, KP, SAVE>());
+template <int DT, int KP, int C, int NC, bool SAVE>
+hipError_t scan(const DeltaArgs& a, hipStream_t s) {
+  using Sc = Scan<DT, KP, C, NC, SAVE>;
+  const hipError_t e = allow_lds(k_delta_scan<DT, KP, C, NC, SAVE>, Sc::bytes);
   if (e != hipSuccess) return e;
-  constexpr int bytes = scan_bufs<DT, KP, SAVE>() * S::kStage;
-  e = allow_lds(k_delta_scan<DT, KP, W, SAVE>, bytes);
-  if (e != hipSuccess) return e;
-  if (a.chunks) k_delta_prep<DT, KP, SAVE><<<(unsigned)(a.chunks * a.Hk), 256, (unsigned)prep_lds<DT, KP, SAVE>(), s>>>(a);
-  const int64_t vg = (a.VP / 16 + W - 1) / W, heads = (a.rows.N * a.Hv + 7) / 8 * 8;
-  k_delta_scan<DT, KP, W, SAVE><<<(unsigned)(heads * vg), 64 * W, bytes, s>>>(a);
+  const int64_t groups = (a.VP / 16 + NC - 1) / NC, heads = (a.rows.N * a.Hv + 7) / 8 * 8;
+  k_delta_scan<DT, KP, C, NC, SAVE><<<(unsigned)(heads * groups), 4 * C, Sc::bytes, s>>>(a);
   return hipGetLastError();
+}
+
+template <int DT, int KP, int C, bool SAVE>
+hipError_t forward(const DeltaArgs& a, hipStream_t s) {
+  constexpr int bytes = PrepLds<DT, KP, C, SAVE>::bytes;
+  const hipError_t e = allow_lds(k_delta_prep<DT, KP, C, SAVE>, bytes);
+  if (e != hipSuccess) return e;
+  if (a.chunks) k_delta_prep<DT, KP, C, SAVE><<<(unsigned)(a.chunks * a.Hk), 4 * C, bytes, s>>>(a);
+  return a.wide_cols ? scan<DT, KP, C, 2, SAVE>(a, s) : scan<DT, KP, C, 1, SAVE>(a, s);
 }
 
 template <int DT, int KP>
 hipError_t forward(const DeltaArgs& a, bool save, hipStream_t s) {
-  return save ? forward<DT, KP, true>(a, s) : forward<DT, KP, false>(a, s);
+  if (a.rows.C == 32) return save ? forward<DT, KP, 32, true>(a, s) : forward<DT, KP, 32, false>(a, s);
+  return save ? forward<DT, KP, 64, true>(a, s) : forward<DT, KP, 64, false>(a, s);
 }
 
 template <int DT>

@@ -1,26 +1,20 @@
-// seq_delta_dev.hpp -- what the forward and backward kernels of the gated delta rule share: operand fragments, staging.
-//
-// v_mfma_f32_16x16x32_bf16: lane l = 16 g + x holds row (column) x of A (B), inner values 8 g..8 g + 7, and column x, rows
-// 4 g..4 g + 3 of the result.  Two result tiles 2 s and 2 s + 1 whose row m stands for perm_row(2 s [+ 1], m) give lane l rows
-// 32 s + 8 g..+7 of its column: an operand B of the next product as it stands.  So a chain of products needs no
-// exchange between lanes, only the A operands' rows taken in that order.
+// seq_delta_dev.hpp -- what the forward and backward kernels of the gated delta rule share.
 #pragma once
 #include "seq_delta.hpp"
 
 namespace seq {
 namespace {
 
-__device__ __forceinline__ int perm_row(int t, int m) { return 32 * (t >> 1) + 8 * (m >> 2) + 4 * (t & 1) + (m & 3); }
+// ---- 16-bit tiles in LDS (tile_at), whole fragments of them
 
-// operand A of tile t: the lane's row, values 8 (4 s + g)..+7
+// operand A (B): the lane's row (column) `row`, values 32 s + 8 g..+7
 template <int W, int NP, int TILE>
 __device__ __forceinline__ void frag(const __bf16* base, int row, int s, int g, bf16x8 (&a)[NP]) {
   const int at = tile_at<W>(row, 4 * s + g);
 #pragma unroll
   for (int i = 0; i < NP; ++i) a[i] = *reinterpret_cast<const bf16x8*>(base + i * TILE + at);
 }
-
-// operand A of tile t of the transposed tile: the lane's column perm_row(t, l % 16), rows 32 s + 8 g..+7
+// the same of the transposed tile: column perm_row(t, x), rows 32 s + 8 g..+7
 template <int W, int NP, int TILE>
 __device__ __forceinline__ void frag_t(const __bf16* base, int t, int s, int g, int x, bf16x8 (&a)[NP]) {
   const int r = 32 * s + 8 * g + (x >> 2), c = 4 * (t >> 1) + (x & 3), h = 4 * (t & 1);
@@ -31,26 +25,7 @@ __device__ __forceinline__ void frag_t(const __bf16* base, int t, int s, int g, 
     a[i] = __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7);
   }
 }
-
-// the same for the triangular tiles; frag_tri_t: columns perm_row(t, l % 16), rows 32 s + 8 g..+7
-template <int NP>
-__device__ __forceinline__ void frag_tri(const __bf16* base, int t, int s, int g, int x, bf16x8 (&a)[NP]) {
-  const int at = t < 2 ? tile_at<32>(perm_row(t, x), g) : 32 * 32 + tile_at<64>(perm_row(t, x) - 32, 4 * s + g);
-#pragma unroll
-  for (int i = 0; i < NP; ++i) a[i] = *reinterpret_cast<const bf16x8*>(base + i * kTri + at);
-}
-template <int NP>
-__device__ __forceinline__ void frag_tri_t(const __bf16* base, int t, int s, int g, int x, bf16x8 (&a)[NP]) {
-  const int r = 8 * g + (x >> 2), c = 4 * (t >> 1) + (x & 3), h = 4 * (t & 1);
-  const int lo = (s ? 32 * 32 + tile_at<64>(r, c) : tile_at<32>(r, c)) + h;
-  const int hi = (s ? 32 * 32 + tile_at<64>(r + 4, c) : tile_at<32>(r + 4, c)) + h;
-#pragma unroll
-  for (int i = 0; i < NP; ++i) {
-    const bf16x4 u = tr4(base + i * kTri + lo), v = tr4(base + i * kTri + hi);
-    a[i] = __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7);
-  }
-}
-// operand B (or A, transposed) with columns 16 t + l % 16 of a tile in rows: rows 32 s + 8 g..+7
+// column 16 t + x, rows 32 s + 8 g..+7
 template <int W, int NP, int TILE>
 __device__ __forceinline__ void frag_col(const __bf16* base, int t, int s, int g, int x, bf16x8 (&a)[NP]) {
   const int r = 32 * s + 8 * g + (x >> 2), c = 2 * t + ((x & 3) >> 1), h = 4 * (x & 1);
@@ -75,20 +50,81 @@ __device__ __forceinline__ double running_sum64(double sum, int lane, double& la
 }
 __device__ __forceinline__ double running_sum(float v, int lane, double& last) { return running_sum64(v, lane, last); }
 
-template <int DT, int KP, bool SAVE>
-constexpr int scan_bufs() { return 2 * DeltaShape<DT, KP, SAVE>::kStage <= 160 * 1024 ? 2 : 1; }
+// ---- fragments in the work memory and operands B in LDS
 
-// linear copy of a chunk's planes and vectors into LDS, 1 KB a wave at a time
-template <class S, int WAVES>
-__device__ __forceinline__ void stage_chunk(const DeltaArgs& a, int64_t c, int hk, int h, char* lds, int wave, int lane) {
-  const char* kq = a.kq + (c * a.Hk + hk) * (int64_t)S::kKQ;
-  const char* xp = a.xp + (c * a.Hv + h) * (int64_t)S::kXP;
-  const char* vec = a.vec + (c * a.Hv + h) * (int64_t)S::kVec;
-  for (int i = wave; i < S::kStage / 1024; i += WAVES) {
-    const char* src = i < S::kKQ / 1024 ? kq + i * 1024
-                      : i < (S::kKQ + S::kXP) / 1024 ? xp + (i * 1024 - S::kKQ) : vec;
-    glds16(src + lane * 16, lds + i * 1024);
+template <int NP>
+__device__ __forceinline__ void load_frag(const char* base, int plane, int lane, bf16x8 (&a)[NP]) {
+#pragma unroll
+  for (int i = 0; i < NP; ++i) a[i] = *reinterpret_cast<const bf16x8*>(base + (plane + i) * 1024 + lane * 16);
+}
+// half p (rows of tile 2 s + p) of an operand B
+template <int NP>
+__device__ __forceinline__ void put_half(char* lds, int s, int p, int lane, f32x4 v) {
+  f32x4 r = v;
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
+    const bf16x4 b = __builtin_convertvector(r, bf16x4);
+    *reinterpret_cast<bf16x4*>(lds + (s * NP + i) * 1024 + lane * 16 + 8 * p) = b;
+    if (i + 1 < NP) r -= admm::bf16_widen<f32x4>(b);
   }
+}
+template <int NP>
+__device__ __forceinline__ void put_whole(char* lds, int s, int lane, f32x8 v) {
+  bf16x8 b[NP];
+  planes8<NP>(v, b);
+#pragma unroll
+  for (int i = 0; i < NP; ++i) *reinterpret_cast<bf16x8*>(lds + (s * NP + i) * 1024 + lane * 16) = b[i];
+}
+template <int NP>
+__device__ __forceinline__ void get_operand(const char* lds, int s, int lane, bf16x8 (&b)[NP]) {
+#pragma unroll
+  for (int i = 0; i < NP; ++i) b[i] = *reinterpret_cast<const bf16x8*>(lds + (s * NP + i) * 1024 + lane * 16);
+}
+// LDS writes of all waves before, LDS reads after; loads from global memory stay in flight
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// A lane's share of a chunk's rows of a tensor: rows perm_row(t, 4 g + r) of the lane's column.  The loads are unconditional
+// (rows and columns outside are taken from the nearest inside, and become zeros on the way out), so that all of them are in
+// flight at once; a branch around each made the compiler wait for each.
+template <class T>
+struct ColumnRows {
+  T raw[4];
+  int left;   // rows of the chunk
+  // p: the chunk's first row, at the lane's column or the row's last
+  __device__ __forceinline__ void load(const T* p, int64_t stride, int rows, int row0) {
+    left = rows;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) raw[r] = p[(row0 + r < rows ? row0 + r : rows - 1) * stride];
+  }
+  __device__ __forceinline__ f32x4 get(bool in, int row0) const {
+    f32x4 v;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] = in && row0 + r < left ? (float)raw[r] : 0.f;
+    return v;
+  }
+};
+
+// a lane's share of a [K, V] state: rows perm_row(t, 4 g + r) of its column, zeros outside
+__device__ __forceinline__ f32x4 load_state(const float* p, int K, int V, int col, int t, int g) {
+  f32x4 st = {0.f, 0.f, 0.f, 0.f};
+  if (!p) return st;
+  const int c = col < V ? col : V - 1;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int kd = perm_row(t, 4 * g + r);
+    st[r] = p[(int64_t)(kd < K ? kd : K - 1) * V + c];
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r) st[r] = col < V && perm_row(t, 4 * g + r) < K ? st[r] : 0.f;
+  return st;
+}
+
+// the column tiles of this workgroup: workgroups are dealt out to the eight XCDs in turn, and those of one head (which read the
+// same fragments) go to one XCD's L2.  false: none
+__device__ __forceinline__ bool place_columns(int64_t heads, int groups, int64_t& head, int& group) {
+  head = (int64_t)(blockIdx.x / 8 / groups) * 8 + blockIdx.x % 8;
+  group = (int)(blockIdx.x / 8 % groups);
+  return head < heads;
 }
 
 template <class F>

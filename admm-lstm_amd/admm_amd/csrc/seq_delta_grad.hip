@@ -1,204 +1,268 @@
 // seq_delta_grad.hip -- gradients of the gated delta rule (seq_delta.hpp has the forward's formulas and names).
 //
-// With dS the gradient of the state behind a chunk, do that of o, R = beta (v - exp(G) K S) and u = X R:
-//     du = P^T do + exp(G_63 - G) K dS,   dR = X^T du,   dv = beta dR,
-//     dS <- exp(G_63) dS + scale Q^T (exp(G) do) - K^T (exp(G) beta dR).
+// With dS the gradient of the state behind a chunk, do that of o, R = beta (v - exp(G_i) K S) and u = X R:
+//     du = P^T do + exp(G - G_i) K dS,   dR = X^T du,   dv = beta dR,
+//     dS <- exp(G) dS + scale Q^T (exp(G_i) do) - K^T (exp(G_i) beta dR).
 // Again only these products run in order (backwards), and again each column by itself: k_delta_back, the mirror image of
 // k_delta_scan.  It leaves dS and dR of every chunk; all other gradients follow chunk by chunk (k_delta_grad), from products
 // over the value axis, with M = do u^T, N = dR u^T, and masked by i >= j (M) and i > j (N):
 //     m = scale D M,  n = -beta_i D N,
-//     dq = scale exp(G) do S^T + m K
-//     dk = exp(G_63 - G) u dS^T - exp(G) beta dR S^T + m^T Q + (n + n^T) K
+//     dq = scale exp(G_i) do S^T + m K
+//     dk = exp(G - G_i) u dS^T - exp(G_i) beta dR S^T + m^T Q + (n + n^T) K
 //     dbeta_i = dR_i . v_i - exp(G_i) k_i . (S dR_i) - sum_j D_ij N_ij (k_i . k_j)
-//     dG_i = q_i . (scale exp(G_i) S do_i) - beta_i exp(G_i) k_i . (S dR_i) - exp(G_63 - G_i) k_i . (dS u_i)
+//     dG_i = q_i . (scale exp(G_i) S do_i) - beta_i exp(G_i) k_i . (S dR_i) - exp(G - G_i) k_i . (dS u_i)
 //            + sum_j (m q.k + n k.k)_ij - sum_j (m q.k + n k.k)_ji
-//     dG_63 += exp(G_63) <S, dS> + sum_i exp(G_63 - G_i) k_i . (dS u_i),    dg_t = sum_{i >= t} dG_i.
+//     dG += exp(G) <S, dS> + sum_i exp(G - G_i) k_i . (dS u_i),    dg_t = dG + sum_{i >= t} dG_i.
 #include "seq_delta_dev.hpp"
 
 namespace seq {
 namespace {
 
-template <int DT, int KP, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void k_delta_back(DeltaGradArgs ga) {
-  using S = DeltaShape<DT, KP, true>;
+// Waves and LDS as in k_delta_scan: wave w forms rows perm_row(w, .) of du and dR and keeps TW tiles of dS.
+template <int DT, int KP, int C, int NC>
+struct Back {
+  using S = DeltaShape<DT, KP, C, true>;
+  static constexpr int TW = S::KT >= S::RT ? S::KT / S::RT : 1;
+  static constexpr int bS = 0, bO = S::KS * 3, bE = bO + S::CS * S::NP, bU = bE + S::CS * 3, bR = bU + S::CS * 3, bEnd = bR + S::CS * 3;
+  static constexpr int bytes = NC * bEnd * 1024;
+};
+
+template <int DT, int KP, int C, int NC>
+__global__ __launch_bounds__(4 * C) void k_delta_back(DeltaGradArgs ga) {
+  using S = DeltaShape<DT, KP, C, true>;
+  using B = Back<DT, KP, C, NC>;
   using T = typename Elem<DT>::T;
-  constexpr int NP = S::NP, NB = scan_bufs<DT, KP, true>(), KS = KP / 32;
+  constexpr int NP = S::NP, TW = B::TW;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const DeltaArgs& a = ga.f;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, x = lane & 15, g = lane >> 4;
-  const int vg = (a.VP / 16 + WAVES - 1) / WAVES;
-  const int64_t heads = a.rows.N * a.Hv;
-  const int64_t head = (int64_t)(blockIdx.x / 8 / vg) * 8 + blockIdx.x % 8;
-  if (head >= heads) return;
+  const int lane = threadIdx.x & 63, w = wave_id(), x = lane & 15, g = lane >> 4;
+  const int groups = (a.VP / 16 + NC - 1) / NC;
+  int64_t head;
+  int group;
+  if (!place_columns(a.rows.N * a.Hv, groups, head, group)) return;
   const int64_t n = head / a.Hv;
   const int h = (int)(head % a.Hv), hk = h / (a.Hv / a.Hk);
-  const int col = ((int)(blockIdx.x / 8 % vg) * WAVES + wave) * 16 + x;
-  const bool in = col < a.V;
+  const int col0 = group * NC * 16 + x;
   int64_t begin, len, c0;
   a.rows.range(n, begin, len, c0);
-  const int64_t nc = (len + kC - 1) / kC;
+  const int64_t nc = (len + C - 1) / C;
+  const bool holds = w * TW < S::KT;
+  const int row0 = perm_row(w, 4 * g);
 
-  f32x4 ds[KP / 16];
+  f32x4 ds[NC][TW];
 #pragma unroll
-  for (int t = 0; t < KP / 16; ++t)
+  for (int i = 0; i < NC; ++i)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int kd = perm_row(t, 4 * g + r);
-      ds[t][r] = ga.d_final && in && kd < a.K ? ga.d_final[(head * a.K + kd) * a.V + col] : 0.f;
-    }
-  const int64_t first = ((a.rows.batch(n) * a.rows.T + begin) * a.Hv + h) * (int64_t)a.V + col;
-  const int64_t orow = (int64_t)a.Hv * a.V;
-  const T* dop = static_cast<const T*>(ga.d_o) + first;
-  T* dvp = static_cast<T*>(ga.dv) + first;
-  f32x4 d[4];
-  auto load_do = [&](int64_t t0) {
+    for (int t = 0; t < TW; ++t)
+      ds[i][t] = load_state(ga.d_final && holds ? ga.d_final + head * a.K * a.V : nullptr, a.K, a.V, col0 + 16 * i, w * TW + t, g);
+
+  const int64_t last = c0 + (nc > 0 ? nc - 1 : 0);
+  const char* kq = a.kq + (last * a.Hk + hk) * (int64_t)S::kKQ;
+  const char* xp = a.xp + (last * a.Hv + h) * (int64_t)S::kXP;
+  const float* vec = reinterpret_cast<const float*>(a.vec + (last * a.Hv + h) * (int64_t)kVec);
+  const int64_t kq_step = (int64_t)a.Hk * S::kKQ, xp_step = (int64_t)a.Hv * S::kXP, vec_step = (int64_t)a.Hv * (kVec / 4);
+  const int64_t orow = (int64_t)a.Hv * a.V, first = ((a.rows.batch(n) * a.rows.T + begin) * a.Hv + h) * (int64_t)a.V;
+  const T* dop[NC];
+  T* dvp[NC];
+  bool in[NC];
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+  for (int i = 0; i < NC; ++i) {
+    const int col = col0 + 16 * i;
+    in[i] = col < a.V;
+    dop[i] = static_cast<const T*>(ga.d_o) + first + (in[i] ? col : a.V - 1);
+    dvp[i] = static_cast<T*>(ga.dv) + first + col;
+  }
+
+  bf16x8 fk[S::KS][NP], fx[S::CS][3], fp[S::CS][3], fq[TW][S::CS][NP], ft[TW][S::CS][NP];
+  f32x4 into, left, beta;
+  float all = 0.f;
+  ColumnRows<T> d[NC];
+  auto tri_t = [&](int s) { return C == 32 ? w : tri_frag_t(w, s < w / 2 ? w / 2 : s); };   // below the diagonal: loaded, not used
+  auto load_k = [&](const char* p) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int64_t row = t0 + perm_row(t, 4 * g + r);
-        d[t][r] = in && row < len ? (float)dop[row * orow] : 0.f;
+    for (int s = 0; s < S::KS; ++s) load_frag<NP>(p, (S::fK + w * S::KS + s) * NP, lane, fk[s]);
+  };
+  auto load_p = [&](const char* p) {
+#pragma unroll
+    for (int s = 0; s < S::CS; ++s) load_frag<3>(p, S::pPT + 3 * tri_t(s), lane, fp[s]);
+  };
+  auto load_x = [&](const char* p) {
+#pragma unroll
+    for (int s = 0; s < S::CS; ++s) load_frag<3>(p, S::pXT + 3 * tri_t(s), lane, fx[s]);
+  };
+  auto load_t = [&](const char* p) {
+    if (!holds) return;
+#pragma unroll
+    for (int t = 0; t < TW; ++t)
+#pragma unroll
+      for (int s = 0; s < S::CS; ++s) {
+        load_frag<NP>(p, (S::fQT + (w * TW + t) * S::CS + s) * NP, lane, fq[t][s]);
+        load_frag<NP>(p, (S::fKT + (w * TW + t) * S::CS + s) * NP, lane, ft[t][s]);
       }
   };
+  auto load_do = [&](int64_t ci) {
+    const int rows = (int)(len - ci * C < C ? len - ci * C : C);
+#pragma unroll
+    for (int i = 0; i < NC; ++i) d[i].load(dop[i] + ci * C * orow, orow, rows, row0);
+  };
+  auto load_vec = [&](const float* p) {
+    into = *reinterpret_cast<const f32x4*>(p + row0);
+    left = *reinterpret_cast<const f32x4*>(p + 64 + row0);
+    beta = *reinterpret_cast<const f32x4*>(p + 128 + row0);
+    all = p[192];
+  };
+  auto part = [&](int i, int b) { return lds + (i * B::bEnd + b) * 1024; };
+  auto put_state = [&]() {
+    if (!holds) return;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      if constexpr (TW >= 2) {
+#pragma unroll
+        for (int t = 0; t < TW; t += 2) put_whole<3>(part(i, B::bS), (w * TW + t) / 2, lane, cat8(ds[i][t], ds[i][t + 1]));
+      } else {
+        put_half<3>(part(i, B::bS), w / 2, w & 1, lane, ds[i][0]);
+      }
+    }
+  };
+  auto put_do = [&]() {
+#pragma unroll
+    for (int i = 0; i < NC; ++i) put_half<NP>(part(i, B::bO), w / 2, w & 1, lane, d[i].get(in[i], row0));
+  };
   if (nc > 0) {
-    stage_chunk<S, WAVES>(a, c0 + nc - 1, hk, h, lds, wave, lane);
-    load_do((nc - 1) * kC);
+    load_do(nc - 1);
+    load_k(kq);
+    load_vec(vec);
+    load_p(xp);
+    load_x(xp);
+    load_t(kq);
+    put_state();
+    put_do();
   }
   for (int64_t ci = nc - 1; ci >= 0; --ci) {
-    const char* buf = lds + (NB == 2 ? ((nc - 1 - ci) & 1) * S::kStage : 0);
-    vm_wait();
-    __syncthreads();
-    f32x4 dc[4];
-#pragma unroll
-    for (int t = 0; t < 4; ++t) dc[t] = d[t];
-    if (ci > 0) {
-      if (NB == 2) stage_chunk<S, WAVES>(a, c0 + ci - 1, hk, h, lds + ((nc - ci) & 1) * S::kStage, wave, lane);
-      load_do((ci - 1) * kC);
-    }
-    const __bf16* Kt = reinterpret_cast<const __bf16*>(buf);
-    const __bf16* Qt = Kt + NP * S::kTile;
-    const __bf16* Xt = reinterpret_cast<const __bf16*>(buf + S::kKQ);
-    const __bf16* Pt = Xt + 3 * kTri;
-    const float* vec = reinterpret_cast<const float*>(buf + S::kKQ + S::kXP);
+    const bool more = ci > 0;
     const int64_t ch = (c0 + ci) * a.Hv + h;
-    if (col < a.VP) {
-      float* p = ga.ds + ch * (int64_t)KP * a.VP + col;
+    const int rows = (int)(len - ci * C < C ? len - ci * C : C);
+    f32x4 dc[NC];
 #pragma unroll
-      for (int t = 0; t < KP / 16; ++t)
+    for (int i = 0; i < NC; ++i) dc[i] = d[i].get(in[i], row0);
+    lds_barrier();   // dS and do are in LDS
+    if (holds) {
+      float* p = ga.ds + ch * (int64_t)KP * a.VP + col0;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) p[(int64_t)perm_row(t, 4 * g + r) * a.VP] = ds[t][r];
+      for (int i = 0; i < NC; ++i)
+#pragma unroll
+        for (int t = 0; t < TW; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (col0 + 16 * i < a.VP) p[(int64_t)perm_row(w * TW + t, 4 * g + r) * a.VP + 16 * i] = ds[i][t][r];
     }
-    // du = exp(G_63 - G) K dS + P^T do
-    f32x4 du[4];
+    // du = exp(G - G_i) K dS + P^T do
+    f32x4 du[NC], du2[NC];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) du[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < NC; ++i) du[i] = du2[i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      bf16x8 sp[3];
-      planes8<3>(cat8(ds[2 * s], ds[2 * s + 1]), sp);
+    for (int s = 0; s < S::KS; ++s)
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        bf16x8 fa[NP];
-        frag<KP, NP, S::kTile>(Kt, perm_row(t, x), s, g, fa);
-        du[t] = mfma_planes<NP, 3, 3>(fa, sp, du[t]);
+      for (int i = 0; i < NC; ++i) {
+        bf16x8 sp[3];
+        get_operand<3>(part(i, B::bS), s, lane, sp);
+        f32x4& u = s & 1 ? du2[i] : du[i];
+        u = mfma_planes<NP, 3, 3>(fk[s], sp, u);
       }
-    }
 #pragma unroll
-    for (int t = 0; t < 4; ++t) du[t] *= *reinterpret_cast<const f32x4*>(vec + kC + perm_row(t, 4 * g));
+    for (int i = 0; i < NC; ++i) {
+      f32x4 p = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      bf16x8 dp[NP];
-      planes8<NP>(cat8(dc[2 * s], dc[2 * s + 1]), dp);
-#pragma unroll
-      for (int t = 0; t < 2 + 2 * s; ++t) {
-        bf16x8 fa[3];
-        frag_tri_t(Pt, t, s, g, x, fa);
-        du[t] = mfma_planes<3, NP, 3>(fa, dp, du[t]);
+      for (int s = 0; s < S::CS; ++s) {
+        if (s < w / 2) continue;
+        bf16x8 dp[NP];
+        get_operand<NP>(part(i, B::bO), s, lane, dp);
+        p = mfma_planes<3, NP, 3>(fp[s], dp, p);
       }
+      du[i] = left * (du[i] + du2[i]) + p;
+      put_half<3>(part(i, B::bU), w / 2, w & 1, lane, du[i]);
+      put_half<3>(part(i, B::bE), w / 2, w & 1, lane, (a.scale * into) * dc[i]);
     }
+    if (more) kq -= kq_step, xp -= xp_step;
+    load_k(kq);
+    load_p(xp);
+    load_do(more ? ci - 1 : ci);
+    lds_barrier();
     // dR = X^T du
-    f32x4 dr[4];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) dr[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < NC; ++i) {
+      f32x4 dr = {0.f, 0.f, 0.f, 0.f}, dr2 = dr;
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      bf16x8 dp[3];
-      planes8<3>(cat8(du[2 * s], du[2 * s + 1]), dp);
-#pragma unroll
-      for (int t = 0; t < 2 + 2 * s; ++t) {
-        bf16x8 fa[3];
-        frag_tri_t(Xt, t, s, g, x, fa);
-        dr[t] = mfma_planes<3, 3, 3>(fa, dp, dr[t]);
+      for (int s = 0; s < S::CS; ++s) {
+        if (s < w / 2) continue;
+        bf16x8 dp[3];
+        get_operand<3>(part(i, B::bU), s, lane, dp);
+        f32x4& r = s & 1 ? dr2 : dr;
+        r = mfma_planes<3, 3, 3>(fx[s], dp, r);
       }
-    }
-    if (col < a.VP) {
-      float* p = ga.dr + ch * (int64_t)kC * a.VP + col;
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) p[(int64_t)perm_row(t, 4 * g + r) * a.VP] = dr[t][r];
-    }
-    const float all = vec[3 * kC];
-#pragma unroll
-    for (int t = 0; t < KP / 16; ++t) ds[t] *= all;
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const int i0 = perm_row(t, 4 * g);
-      const f32x4 into = *reinterpret_cast<const f32x4*>(vec + i0), b = *reinterpret_cast<const f32x4*>(vec + 2 * kC + i0);
-      const f32x4 dv = b * dr[t];
+      dr += dr2;
+      const f32x4 dv = beta * dr;
+      put_half<3>(part(i, B::bR), w / 2, w & 1, lane, -into * dv);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int64_t row = ci * kC + i0 + r;
-        if (in && row < len) dvp[row * orow] = (T)dv[r];
-      }
-      dc[t] *= a.scale * into;
-      dr[t] = -into * dv;
-    }
-    // dS <- exp(G_63) dS + scale Q^T (exp(G) do) - K^T (exp(G) beta dR)
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      bf16x8 dp[3], rp[3];
-      planes8<3>(cat8(dc[2 * s], dc[2 * s + 1]), dp);
-      planes8<3>(cat8(dr[2 * s], dr[2 * s + 1]), rp);
-#pragma unroll
-      for (int t = 0; t < KP / 16; ++t) {
-        bf16x8 fa[NP];
-        frag_t<KP, NP, S::kTile>(Qt, t, s, g, x, fa);
-        ds[t] = mfma_planes<NP, 3, 3>(fa, dp, ds[t]);
-        frag_t<KP, NP, S::kTile>(Kt, t, s, g, x, fa);
-        ds[t] = mfma_planes<NP, 3, 3>(fa, rp, ds[t]);
+        if (col0 + 16 * i < a.VP) ga.dr[(ch * C + row0 + r) * (int64_t)a.VP + col0 + 16 * i] = dr[r];
+        if (in[i] && row0 + r < rows) dvp[i][(ci * C + row0 + r) * orow] = (T)dv[r];
       }
     }
-    if (NB == 1 && ci > 0) {
-      __syncthreads();
-      stage_chunk<S, WAVES>(a, c0 + ci - 1, hk, h, lds, wave, lane);
+    load_x(xp);
+    const float all_now = all;
+    if (more) vec -= vec_step;
+    load_vec(vec);
+    lds_barrier();
+    // dS <- exp(G) dS + scale Q^T (exp(G_i) do) - K^T (exp(G_i) beta dR)
+    if (holds) {
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+#pragma unroll
+        for (int t = 0; t < TW; ++t) ds[i][t] *= all_now;
+#pragma unroll
+        for (int s = 0; s < S::CS; ++s) {
+          bf16x8 dp[3], rp[3];
+          get_operand<3>(part(i, B::bE), s, lane, dp);
+          get_operand<3>(part(i, B::bR), s, lane, rp);
+#pragma unroll
+          for (int t = 0; t < TW; ++t) {
+            ds[i][t] = mfma_planes<NP, 3, 3>(fq[t][s], dp, ds[i][t]);
+            ds[i][t] = mfma_planes<NP, 3, 3>(ft[t][s], rp, ds[i][t]);
+          }
+        }
+      }
     }
+    load_t(kq);
+    put_state();
+    put_do();
   }
-  if (ga.d_initial && in) {
+  if (ga.d_initial && holds) {
 #pragma unroll
-    for (int t = 0; t < KP / 16; ++t)
+    for (int i = 0; i < NC; ++i)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int kd = perm_row(t, 4 * g + r);
-        if (kd < a.K) ga.d_initial[(head * a.K + kd) * a.V + col] = ds[t][r];
-      }
+      for (int t = 0; t < TW; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int kd = perm_row(w * TW + t, 4 * g + r);
+          if (in[i] && kd < a.K) ga.d_initial[(head * a.K + kd) * a.V + col0 + 16 * i] = ds[i][t][r];
+        }
   }
 }
 
 // ----------------------------------------------------------------------------------- the rest, chunk by chunk
 
 constexpr int kSlice = 32;              // values of v taken at a time
-constexpr int kST = kC * kSlice;        // values of a staged plane
-constexpr int kMT = kC * kC;            // values of a plane of m or n
 
-template <int DT, int KP>
+template <int DT, int KP, int C>
 struct GradLds {
-  using S = DeltaShape<DT, KP, true>;
+  using S = DeltaShape<DT, KP, C, true>;
+  static constexpr int kST = C * kSlice, kMT = C * C;   // values of a staged plane, of a plane of m or n
   static constexpr int stage = (S::NP + 6) * kST * 2, mats = 2 * S::NO * kMT * 2;
-  static constexpr int kq = 0, work = S::kKQ, vec = work + (stage > mats ? stage : mats);
+  static constexpr int kq = 0, work = 2 * S::NP * C * KP * 2, vec = work + (stage > mats ? stage : mats);
   // G hi, G lo, beta, exp(G), exp(G_63 - G), dR . v, column sums; row sums of m q.k + n k.k, of -D N k.k, of q X, k Y, k Z
   // by wave; <S, dS> by wave
-  static constexpr int bytes = vec + (7 + 5 * 4) * kC * 4 + 4 * 4 + 16;
+  static constexpr int bytes = vec + (7 + 5 * S::RT) * C * 4 + 32;
 };
 
 __device__ __forceinline__ float sum16(float v) {
@@ -215,69 +279,79 @@ __device__ __forceinline__ float whole(const __bf16* p) {
   return v;
 }
 
-template <int DT, int KP>
-__global__ __launch_bounds__(256) void k_delta_grad(DeltaGradArgs ga, bool wide_v, bool wide_o) {
-  using S = DeltaShape<DT, KP, true>;
-  using L = GradLds<DT, KP>;
+template <int DT, int KP, int C>
+__global__ __launch_bounds__(4 * C) void k_delta_grad(DeltaGradArgs ga, bool wide_v, bool wide_o) {
+  using S = DeltaShape<DT, KP, C, true>;
+  using L = GradLds<DT, KP, C>;
   using T = typename Elem<DT>::T;
-  constexpr int NP = S::NP, NO = S::NO, NT = KP >= 64 ? KP / 64 : 1;   // 16-column tiles of K a wave owns
+  constexpr int NP = S::NP, NO = S::NO, RT = S::RT, kST = L::kST, kMT = L::kMT, kTile = C * KP;
+  constexpr int NT = S::KT >= RT ? S::KT / RT : 1;   // 16-column tiles of K a wave owns
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const DeltaArgs& a = ga.f;
   __bf16* const Kt = reinterpret_cast<__bf16*>(lds);
-  __bf16* const Qt = Kt + NP * S::kTile;
+  __bf16* const Qt = Kt + NP * kTile;
   __bf16* const dO = reinterpret_cast<__bf16*>(lds + L::work);
   __bf16* const dR = dO + NP * kST;
   __bf16* const uu = dR + 3 * kST;
   __bf16* const mt_ = reinterpret_cast<__bf16*>(lds + L::work);   // m, n: after the value axis is done
   __bf16* const nt_ = mt_ + NO * kMT;
   float* const ghi = reinterpret_cast<float*>(lds + L::vec);
-  float *const glo = ghi + kC, *const bet = ghi + 2 * kC, *const into = ghi + 3 * kC, *const left = ghi + 4 * kC;
-  float *const rv = ghi + 5 * kC, *const cols = ghi + 6 * kC, *const rsum = ghi + 7 * kC, *const rnb = rsum + 4 * kC;
-  float *const qx = rnb + 4 * kC, *const ky = qx + 4 * kC, *const kz = ky + 4 * kC, *const sds = kz + 4 * kC;
+  float *const glo = ghi + C, *const bet = ghi + 2 * C, *const into = ghi + 3 * C, *const left = ghi + 4 * C;
+  float *const rv = ghi + 5 * C, *const cols = ghi + 6 * C, *const rsum = ghi + 7 * C, *const rnb = rsum + RT * C;
+  float *const qx = rnb + RT * C, *const ky = qx + RT * C, *const kz = ky + RT * C, *const sds = kz + RT * C;
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, x = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, wave = wave_id(), x = lane & 15, g = lane >> 4;
   const int64_t c = blockIdx.x / a.Hv;
   const int h = (int)(blockIdx.x % a.Hv), hk = h / (a.Hv / a.Hk);
   const int64_t n = a.rows.find(c);
   int64_t begin, len, chunk0;
   a.rows.range(n, begin, len, chunk0);
-  const int64_t t0 = (c - chunk0) * kC;
+  const int64_t t0 = (c - chunk0) * C;
   if (t0 < 0 || t0 >= len) return;
-  const int rows = (int)(len - t0 < kC ? len - t0 : kC);
+  const int rows = (int)(len - t0 < C ? len - t0 : C);
   const int64_t bt = a.rows.batch(n), r0 = begin + t0, ch = c * a.Hv + h;
 
-  const char* kq = a.kq + (c * a.Hk + hk) * (int64_t)S::kKQ;
-  for (int i = wave; i < S::kKQ / 1024; i += 4) glds16(kq + i * 1024 + lane * 16, lds + i * 1024);
+  {   // K and Q rows from their fragments
+    const char* kq = a.kq + (c * a.Hk + hk) * (int64_t)S::kKQ + lane * 16;
+#pragma unroll 4
+    for (int f = wave; f < 2 * RT * S::KS * NP; f += RT) {
+      const int e = f / NP, t = e / S::KS % RT, s = e % S::KS, w = e / (RT * S::KS);
+      *reinterpret_cast<bf16x8*>(Kt + (w * NP + f % NP) * kTile + tile_at<KP>(perm_row(t, x), 4 * s + g)) =
+          *reinterpret_cast<const bf16x8*>(kq + f * 1024);
+    }
+  }
   float graw = 0.f;
   if (wave == 0) {
     graw = lane < rows ? a.g[bt * a.gs[0] + (r0 + lane) * a.gs[1] + h * a.gs[2]] : 0.f;
     double last;
     const double sum = running_sum(graw < kMinG ? kMinG : graw, lane, last);
     const float hi = (float)sum;
-    const float* vec = reinterpret_cast<const float*>(a.vec + ch * (int64_t)S::kVec);
-    ghi[lane] = hi;
-    glo[lane] = (float)(sum - (double)hi);
-    into[lane] = vec[lane];
-    left[lane] = vec[kC + lane];
-    bet[lane] = vec[2 * kC + lane];
+    const float* vec = reinterpret_cast<const float*>(a.vec + ch * (int64_t)kVec);
+    if (lane < C) {
+      ghi[lane] = hi;
+      glo[lane] = (float)(sum - (double)hi);
+      into[lane] = vec[lane];
+      left[lane] = vec[64 + lane];
+      bet[lane] = vec[128 + lane];
+    }
   }
 
   const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-  f32x4 X1[4][NT], Y[4][NT], Z[4][NT], M[4], N[4];
+  f32x4 X1[RT][NT], Y[RT][NT], Z[RT][NT], M[RT], N[RT];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < RT; ++i) {
     M[i] = N[i] = zero;
 #pragma unroll
     for (int j = 0; j < NT; ++j) X1[i][j] = Y[i][j] = Z[i][j] = zero;
   }
   const float* s0 = a.s0 + ch * (int64_t)KP * a.VP;
   const float* dse = ga.ds + ch * (int64_t)KP * a.VP;
-  const bool active = wave * NT * 16 < KP;
+  const bool active = wave * NT < S::KT;
   float dot = 0.f, rdot = 0.f;
   {
     const int row = tid >> 2, p = tid & 3;
-    const float* rp = ga.dr + (ch * kC + row) * (int64_t)a.VP + 8 * p;
-    const float* up = a.u + (ch * kC + row) * (int64_t)a.VP + 8 * p;
+    const float* rp = ga.dr + (ch * C + row) * (int64_t)a.VP + 8 * p;
+    const float* up = a.u + (ch * C + row) * (int64_t)a.VP + 8 * p;
     const T* op = static_cast<const T*>(ga.d_o) + ((bt * a.rows.T + r0 + row) * a.Hv + h) * (int64_t)a.V + 8 * p;
     const T* vp = static_cast<const T*>(a.v) + bt * a.vs[0] + (r0 + row) * a.vs[1] + h * a.vs[2] + 8 * p;
     const int at = tile_at<kSlice>(row, p);
@@ -325,7 +399,7 @@ __global__ __launch_bounds__(256) void k_delta_grad(DeltaGradArgs ga, bool wide_
         }
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < RT; ++i) {
         bf16x8 fo[NP], fr[3], fi[3];
         frag<kSlice, NP, kST>(dO, 16 * i + x, 0, g, fo);
         frag<kSlice, 3, kST>(dR, 16 * i + x, 0, g, fr);
@@ -351,31 +425,30 @@ __global__ __launch_bounds__(256) void k_delta_grad(DeltaGradArgs ga, bool wide_
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) dot += __shfl_xor(dot, d);
   if (lane == 0) sds[wave] = dot;
-  vm_wait();
   __syncthreads();   // K and Q are in; the staged values are done with
 
   // m and n: the lane's column j = 16 wave + x, rows 16 i + 4 g..+3
   {
     const int j = 16 * wave + x;
-    f32x4 qk[4], kk[4];
+    f32x4 qk[RT], kk[RT];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) qk[i] = kk[i] = zero;
+    for (int i = 0; i < RT; ++i) qk[i] = kk[i] = zero;
 #pragma unroll
     for (int s = 0; s < KP / 32; ++s) {
       bf16x8 kb[NP], fa[NP];
-      frag<KP, NP, S::kTile>(Kt, j, s, g, kb);
+      frag<KP, NP, kTile>(Kt, j, s, g, kb);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < RT; ++i) {
         if (i < wave) continue;
-        frag<KP, NP, S::kTile>(Qt, 16 * i + x, s, g, fa);
+        frag<KP, NP, kTile>(Qt, 16 * i + x, s, g, fa);
         qk[i] = mfma_planes<NP, NP, 3>(fa, kb, qk[i]);
-        frag<KP, NP, S::kTile>(Kt, 16 * i + x, s, g, fa);
+        frag<KP, NP, kTile>(Kt, 16 * i + x, s, g, fa);
         kk[i] = mfma_planes<NP, NP, 3>(fa, kb, kk[i]);
       }
     }
     float csum = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < RT; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int row = 16 * i + 4 * g + r;
@@ -387,10 +460,10 @@ __global__ __launch_bounds__(256) void k_delta_grad(DeltaGradArgs ga, bool wide_
         csum += e;
         const float rs = sum16(e), rb = sum16(row > j ? nb * kk[i][r] : 0.f);
         if (x == 0) {
-          rsum[wave * kC + row] = rs;
-          rnb[wave * kC + row] = rb;
+          rsum[wave * C + row] = rs;
+          rnb[wave * C + row] = rb;
         }
-        const int at = tile_at<kC>(row, j >> 3) + (j & 7);
+        const int at = tile_at<C>(row, j >> 3) + (j & 7);
         float rm = m, rn = nn;
 #pragma unroll
         for (int p = 0; p < NO; ++p) {
@@ -409,7 +482,7 @@ __global__ __launch_bounds__(256) void k_delta_grad(DeltaGradArgs ga, bool wide_
 
   // dq and dk: the lane's column 16 (wave NT + j) + x, rows 16 i + 4 g..+3
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < RT; ++i)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int row = 16 * i + 4 * g + r;
@@ -419,7 +492,7 @@ __global__ __launch_bounds__(256) void k_delta_grad(DeltaGradArgs ga, bool wide_
         for (int j = 0; j < NT; ++j) {
           const int kd = 16 * (wave * NT + j) + x;
           const int at = tile_at<KP>(row, kd >> 3) + (kd & 7);
-          const float kv = whole<NP, S::kTile>(Kt + at), qv = whole<NP, S::kTile>(Qt + at);
+          const float kv = whole<NP, kTile>(Kt + at), qv = whole<NP, kTile>(Qt + at);
           const float xs = a.scale * into[row] * X1[i][j][r], ys = into[row] * Y[i][j][r], zs = left[row] * Z[i][j][r];
           sq = fmaf(qv, xs, sq);
           sy = fmaf(kv, ys, sy);
@@ -430,32 +503,32 @@ __global__ __launch_bounds__(256) void k_delta_grad(DeltaGradArgs ga, bool wide_
       }
       sq = sum16(sq), sy = sum16(sy), sz = sum16(sz);
       if (x == 0) {
-        qx[wave * kC + row] = sq;
-        ky[wave * kC + row] = sy;
-        kz[wave * kC + row] = sz;
+        qx[wave * C + row] = sq;
+        ky[wave * C + row] = sy;
+        kz[wave * C + row] = sz;
       }
     }
   if (active) {
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
+    for (int s = 0; s < S::CS; ++s) {
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
         bf16x8 kb[NP], qb[NP];
-        frag_col<KP, NP, S::kTile>(Kt, wave * NT + j, s, g, x, kb);
-        frag_col<KP, NP, S::kTile>(Qt, wave * NT + j, s, g, x, qb);
+        frag_col<KP, NP, kTile>(Kt, wave * NT + j, s, g, x, kb);
+        frag_col<KP, NP, kTile>(Qt, wave * NT + j, s, g, x, qb);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < RT; ++i) {
           bf16x8 fa[NO];
           if (s <= i / 2) {   // rows i of m and n have columns up to the diagonal
-            frag<kC, NO, kMT>(mt_, 16 * i + x, s, g, fa);
+            frag<C, NO, kMT>(mt_, 16 * i + x, s, g, fa);
             X1[i][j] = mfma_planes<NO, NP, NO>(fa, kb, X1[i][j]);
-            frag<kC, NO, kMT>(nt_, 16 * i + x, s, g, fa);
+            frag<C, NO, kMT>(nt_, 16 * i + x, s, g, fa);
             Y[i][j] = mfma_planes<NO, NP, NO>(fa, kb, Y[i][j]);
           }
           if (s >= i / 2) {
-            frag_col<kC, NO, kMT>(mt_, i, s, g, x, fa);
+            frag_col<C, NO, kMT>(mt_, i, s, g, x, fa);
             Y[i][j] = mfma_planes<NO, NP, NO>(fa, qb, Y[i][j]);
-            frag_col<kC, NO, kMT>(nt_, i, s, g, x, fa);
+            frag_col<C, NO, kMT>(nt_, i, s, g, x, fa);
             Y[i][j] = mfma_planes<NO, NP, NO>(fa, kb, Y[i][j]);
           }
         }
@@ -463,7 +536,7 @@ __global__ __launch_bounds__(256) void k_delta_grad(DeltaGradArgs ga, bool wide_
     }
     const int64_t first = bt * a.rows.T + r0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < RT; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int row = 16 * i + 4 * g + r;
@@ -485,19 +558,28 @@ __global__ __launch_bounds__(256) void k_delta_grad(DeltaGradArgs ga, bool wide_
   }
   __syncthreads();
   if (wave == 0) {
-    auto waves = [&](const float* p) { return (p[lane] + p[kC + lane]) + (p[2 * kC + lane] + p[3 * kC + lane]); };
+    const int at = lane < C ? lane : 0;
+    auto waves = [&](const float* p) {
+      float v = 0.f;
+#pragma unroll
+      for (int i = 0; i < RT; ++i) v += p[i * C + at];
+      return lane < C ? v : 0.f;
+    };
     const float y = waves(ky), z = waves(kz);
     // columns right of the diagonal tile hold zeros in rsum and rnb: every wave writes every row
-    const double own = (double)waves(rsum) - cols[lane] + waves(qx) - bet[lane] * y - z;
+    const double own = lane < C ? (double)waves(rsum) - cols[at] + waves(qx) - bet[at] * y - z : 0.0;
     double tail, zall;
     const double upto = running_sum64(own, lane, tail);
     running_sum64(z, lane, zall);
-    const float all = reinterpret_cast<const float*>(a.vec + ch * (int64_t)S::kVec)[3 * kC];
-    const double end = zall + (double)all * ((sds[0] + sds[1]) + (sds[2] + sds[3]));
+    const float all = reinterpret_cast<const float*>(a.vec + ch * (int64_t)kVec)[192];
+    float dots = 0.f;
+#pragma unroll
+    for (int i = 0; i < RT; ++i) dots += sds[i];
+    const double end = zall + (double)all * dots;
     if (lane < rows) {
-      const int64_t at = (bt * a.rows.T + r0 + lane) * a.Hv + h;
-      ga.dg[at] = graw < kMinG ? 0.f : (float)(end + tail - upto + own);
-      ga.dbeta[at] = rv[lane] - y + waves(rnb);
+      const int64_t to = (bt * a.rows.T + r0 + lane) * a.Hv + h;
+      ga.dg[to] = graw < kMinG ? 0.f : (float)(end + tail - upto + own);
+      ga.dbeta[to] = rv[lane] - y + waves(rnb);
     }
   }
 }
@@ -517,19 +599,27 @@ __global__ void k_delta_heads(const float* dq32, const float* dk32, T* dq, T* dk
   }
 }
 
-template <int DT, int KP>
-hipError_t backward(const DeltaGradArgs& ga, bool wide_v, bool wide_o, hipStream_t s) {
-  using S = DeltaShape<DT, KP, true>;
-  using T = typename Elem<DT>::T;
-  constexpr int W = 4, bytes = scan_bufs<DT, KP, true>() * S::kStage, glds = GradLds<DT, KP>::bytes;
+template <int DT, int KP, int C, int NC>
+hipError_t back(const DeltaGradArgs& ga, hipStream_t s) {
+  constexpr int bytes = Back<DT, KP, C, NC>::bytes;
   const DeltaArgs& a = ga.f;
-  hipError_t e = allow_lds(k_delta_back<DT, KP, W>, bytes);
+  const hipError_t e = allow_lds(k_delta_back<DT, KP, C, NC>, bytes);
   if (e != hipSuccess) return e;
-  e = allow_lds(k_delta_grad<DT, KP>, glds);
+  const int64_t groups = (a.VP / 16 + NC - 1) / NC, heads = (a.rows.N * a.Hv + 7) / 8 * 8;
+  k_delta_back<DT, KP, C, NC><<<(unsigned)(heads * groups), 4 * C, bytes, s>>>(ga);
+  return hipGetLastError();
+}
+
+template <int DT, int KP, int C>
+hipError_t backward(const DeltaGradArgs& ga, bool wide_v, bool wide_o, hipStream_t s) {
+  using T = typename Elem<DT>::T;
+  constexpr int bytes = GradLds<DT, KP, C>::bytes;
+  const DeltaArgs& a = ga.f;
+  hipError_t e = a.wide_cols ? back<DT, KP, C, 2>(ga, s) : back<DT, KP, C, 1>(ga, s);
   if (e != hipSuccess) return e;
-  const int64_t vg = (a.VP / 16 + W - 1) / W, heads = (a.rows.N * a.Hv + 7) / 8 * 8;
-  k_delta_back<DT, KP, W><<<(unsigned)(heads * vg), 64 * W, bytes, s>>>(ga);
-  if (a.chunks) k_delta_grad<DT, KP><<<(unsigned)(a.chunks * a.Hv), 256, glds, s>>>(ga, wide_v, wide_o);
+  e = allow_lds(k_delta_grad<DT, KP, C>, bytes);
+  if (e != hipSuccess) return e;
+  if (a.chunks) k_delta_grad<DT, KP, C><<<(unsigned)(a.chunks * a.Hv), 4 * C, bytes, s>>>(ga, wide_v, wide_o);
   if (ga.dq32) {
     const int64_t rows = a.rows.off ? a.rows.T : a.rows.N * a.rows.T, n = rows * a.Hk * a.K;
     const int64_t want = (n + 255) / 256;
@@ -537,6 +627,11 @@ hipError_t backward(const DeltaGradArgs& ga, bool wide_v, bool wide_o, hipStream
                ga.dq32, ga.dk32, static_cast<T*>(ga.dq), static_cast<T*>(ga.dk), n, a.Hv / a.Hk, a.K);
   }
   return hipGetLastError();
+}
+
+template <int DT, int KP>
+hipError_t backward(const DeltaGradArgs& ga, bool wide_v, bool wide_o, hipStream_t s) {
+  return ga.f.rows.C == 32 ? backward<DT, KP, 32>(ga, wide_v, wide_o, s) : backward<DT, KP, 64>(ga, wide_v, wide_o, s);
 }
 
 template <int DT>

@@ -76,11 +76,15 @@ __device__ __forceinline__ f32x4 mfma_planes(const bf16x8 (&a)[NA], const bf16x8
 }
 
 // 16 bytes a lane from global memory straight into LDS: `lds` is the wave's base, lane l's bytes land at lds + 16 l.
-// The caller waits for them (vm_wait) before the barrier that hands them to other waves.
+// The caller waits for them (vm_wait) before the barrier that hands them to other waves, and keeps other buffers' readers out by
+// barriers too.  In assembly (m0: the LDS base; there is no result register) because the compiler, which cannot tell the
+// buffers apart, waits for all such loads before the next transposing read of any of them.
 __device__ __forceinline__ void glds16(const void* g, void* lds) {
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)g,
-                                   (__attribute__((address_space(3))) uint32_t*)lds, 16, 0, 0);
+  const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds);
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(g) : "memory");
 }
+// the wave's index, as a scalar
+__device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 __device__ __forceinline__ void vm_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // Four rows by sixteen columns of 16-bit values, transposed on the way out of LDS: lane i of each 16 gives the address

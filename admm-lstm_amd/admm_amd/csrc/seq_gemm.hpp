@@ -96,7 +96,7 @@ struct Gemm {
 
   // b_of: which matrix B (not DUAL, not SPLIT).  acc[i][j]: rows 16 (wm MT + i) + x, columns 16 j' + 4 g..+3 of C
   __device__ static void run(const GemmArgs& g, int tm, int tn, int b_of, char* lds, f32x4 (&acc)[MT][NT]) {
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), x = lane & 15, q = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = wave_id(), x = lane & 15, q = lane >> 4;
     const int wm = wave / WN, wn = wave % WN;
     const int kt = (g.K + kBK - 1) / kBK, terms = g.planes == 1 ? 1 : 6, total = kt * terms * (SPLIT ? 2 : 1);
 #pragma unroll

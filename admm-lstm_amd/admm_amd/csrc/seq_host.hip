@@ -72,7 +72,8 @@ int check_heads(int Hk, int Hv, int K, int V, int dtype) {
 }
 
 struct DeltaSizes {
-  int KP, NP, NO;
+  int KP, C;
+  bool wide_cols;
   int64_t per, chunks, VP, kq, xp, vec, s0, u, heads, need;
 };
 
@@ -86,19 +87,21 @@ int delta_sizes(const SeqDelta* d, bool saved, DeltaSizes& z) {
   if (d->offsets ? d->batch != 1 : d->sequences != d->batch)
     return fail(SEQ_EINVAL, d->offsets ? "packed sequences need batch 1 (got %lld)" : "sequences must equal batch (%lld)", (long long)d->batch);
   z.KP = d->K <= 32 ? 32 : d->K <= 64 ? 64 : 128;
-  z.NP = d->dtype + 1;
-  z.NO = d->dtype == SEQ_FP32 ? 3 : 2;
-  z.per = (d->T + kC - 1) / kC;
+  // sequences of at most 32 rows (or packed ones of at most 32 on average) would leave half of a 64-row chunk empty
+  z.C = d->T <= 32 || (d->offsets && d->T <= 32 * d->sequences) ? 32 : 64;
+  const int NP = d->dtype + 1, NO = d->dtype == SEQ_FP32 ? 3 : 2, tri = z.C == 64 ? 6 : 2;
+  z.per = (d->T + z.C - 1) / z.C;
   z.VP = (d->V + 15) / 16 * 16;
-  z.chunks = d->offsets ? (d->sequences && d->T ? d->T / kC + d->sequences + 1 : 0) : z.per * d->batch;
-  const int64_t blocks = (z.VP / 16 + 3) / 4;
-  if (z.chunks > kMaxBlocks / d->Hv || (d->sequences + 8) > kMaxBlocks / (d->Hv * blocks))
+  z.wide_cols = d->sequences * d->Hv * (z.VP / 16) > 512;
+  z.chunks = d->offsets ? (d->sequences && d->T ? d->T / z.C + d->sequences + 1 : 0) : z.per * d->batch;
+  if (z.chunks > kMaxBlocks / d->Hv || (d->sequences + 8) > kMaxBlocks / (d->Hv * (z.VP / 16)))
     return fail(SEQ_EINVAL, "too many sequences, rows or heads for one launch");
-  z.kq = up256(z.chunks * d->Hk * (4LL * z.NP * kC * z.KP));
-  z.xp = up256(z.chunks * d->Hv * (2LL * (3 + (saved ? 3 : z.NO)) * kTri));
-  z.vec = up256(z.chunks * d->Hv * (4LL * kC * 4));
+  // sizes of DeltaShape: K, Q, K^T (saved: Q^T), each z.C x KP planes; X, P (saved: their transposes) as fragments
+  z.kq = up256(z.chunks * d->Hk * ((saved ? 4LL : 3LL) * NP * z.C * z.KP * 2));
+  z.xp = up256(z.chunks * d->Hv * ((saved ? 12LL : 3LL + NO) * tri * 1024));
+  z.vec = up256(z.chunks * d->Hv * (int64_t)kVec);
   z.s0 = up256(z.chunks * d->Hv * 4 * z.KP * z.VP);
-  z.u = up256(z.chunks * d->Hv * 4 * kC * z.VP);
+  z.u = up256(z.chunks * d->Hv * 4 * z.C * z.VP);
   const int64_t rows = d->batch * d->T;
   z.heads = d->Hv > d->Hk ? up256(rows * d->Hv * d->K * 4) : 0;
   z.need = z.kq + z.xp + z.vec + (saved ? z.s0 + z.u : 0);
@@ -120,6 +123,7 @@ bool wide_rows(const SeqDelta* d, int len, const void* p, const S& stride) {
 
 void delta_args(const SeqDelta* d, const DeltaSizes& z, void* work, DeltaArgs& a) {
   memset(&a, 0, sizeof a);
+  a.rows.C = z.C;
   a.rows.T = d->T;
   a.rows.N = d->sequences;
   a.rows.per = z.per;
@@ -135,6 +139,7 @@ void delta_args(const SeqDelta* d, const DeltaSizes& z, void* work, DeltaArgs& a
   memcpy(a.bs, d->beta_stride, sizeof a.bs);
   a.wide_q = wide_rows(d, d->K, d->q, d->q_stride);
   a.wide_k = wide_rows(d, d->K, d->k, d->k_stride);
+  a.wide_cols = z.wide_cols;
   a.initial = d->initial;
   a.chunks = z.chunks;
   char* w = static_cast<char*>(work);

@@ -91,7 +91,7 @@ template <int DT, int WM, int WN, int MT, int NT, bool KEEP>
 __global__ __launch_bounds__(64 * WM * WN) void k_unit(GemmArgs g, int kind, typename Elem<DT>::T* y, float* pre, bool wide) {
   using G = Gemm<DT, WM, WN, MT, NT, true, false, true, false>;
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, x = lane & 15, q = lane >> 4, wm = wave / WN, wn = wave % WN;
+  const int lane = threadIdx.x & 63, wave = wave_id(), x = lane & 15, q = lane >> 4, wm = wave / WN, wn = wave % WN;
   int tm, tn;
   G::place(g, tm, tn);
   f32x4 acc[MT][NT];
@@ -123,7 +123,7 @@ template <int DT, int WM, int WN, int MT, int NT, bool AI, bool BI, bool SPLIT>
 __global__ __launch_bounds__(64 * WM * WN) void k_unit_gemm(GemmArgs g, typename Elem<DT>::T* c0, typename Elem<DT>::T* c1, bool wide) {
   using G = Gemm<DT, WM, WN, MT, NT, AI, BI, false, SPLIT>;
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, x = lane & 15, q = lane >> 4, wm = wave / WN, wn = wave % WN;
+  const int lane = threadIdx.x & 63, wave = wave_id(), x = lane & 15, q = lane >> 4, wm = wave / WN, wn = wave % WN;
   int tm, tn;
   G::place(g, tm, tn);
   f32x4 acc[MT][NT];
