@@ -1,21 +1,22 @@
-"""ctypes binding of libseqops.so (the C ABI declared in include/seq_ops.h): the sequence-layer operators.
+"""Binding of libseqops.so (the C ABI declared in include/seq_ops.h): the sequence-layer operators.
 
 Like libadmmlstm.so (``_native``) it is built in-tree by ``csrc/Makefile`` and is the only compute path of its operators:
-loading fails loudly when it is missing, and host tensors are refused.
+loading fails loudly when it is missing, and host tensors are refused.  ``load()`` gives the C ABI through ctypes,
+``entry_points()`` the extension ``_seq_torch`` that ``blocks/`` calls.
 """
 from __future__ import annotations
 
 import ctypes
+import importlib
 import os
 from ctypes import POINTER, Structure, c_char_p, c_float, c_int, c_int32, c_int64, c_uint64, c_void_p
 
 import torch  # noqa: F401  (must precede the CDLL load: one HIP runtime per process)
 
-from ._native import AdmmError, NativeUnavailable
+from ._native import NativeUnavailable
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), 'libseqops.so')
 ABI_VERSION = 1
-DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
 class SeqDelta(Structure):
@@ -85,43 +86,14 @@ def load() -> ctypes.CDLL:
     return lib
 
 
-def check(rc: int, what: str) -> None:
-    if rc != 0:
-        raise AdmmError(f'{what} failed (code {rc}): {_lib.seq_last_error().decode(errors="replace")}', rc)
-
-
-def stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
-
-
-def require(cond: bool, msg: str) -> None:
-    if not cond:
-        raise ValueError(msg)
-
-
-def require_tensors(**tensors) -> None:
-    """All of them tensors (None is skipped)."""
-    for name, t in tensors.items():
-        if t is not None and not isinstance(t, torch.Tensor):
-            raise TypeError(f'{name} must be a tensor (got {type(t).__name__})')
-
-
-def require_device(**tensors) -> torch.device:
-    """All of them HIP tensors on one device (None is skipped); returns it."""
-    dev = None
-    for name, t in tensors.items():
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise RuntimeError(f'{name} must be a HIP device tensor (got {t.device}); '
-                               'admm-lstm_amd has no CPU execution path')
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise ValueError(f'{name} is on {t.device}, the other tensors on {dev}')
-    return dev
-
-
-def rows_last(t: torch.Tensor) -> torch.Tensor:
-    """The tensor itself where its last axis is contiguous, else a contiguous copy."""
-    return t if t.stride(-1) == 1 or t.size(-1) == 1 else t.contiguous()
+def entry_points():
+    """The extension module with the operators' entry points (csrc/seq_torch.cpp)."""
+    load()
+    try:
+        mod = importlib.import_module('admm_amd._seq_torch')
+    except ImportError as e:
+        raise NativeUnavailable(f'admm_amd/_seq_torch.so cannot be imported ({e}): build it with '
+                                f'`make -C admm-lstm_amd/admm_amd/csrc`. There is no CPU fallback.') from e
+    if mod.abi_version() != ABI_VERSION:
+        raise NativeUnavailable(f'_seq_torch: ABI {mod.abi_version()} != expected {ABI_VERSION}')
+    return mod
