@@ -236,11 +236,13 @@ __global__ __launch_bounds__(4 * C) void k_delta_prep(DeltaArgs a) {
 
 // --------------------------------------------------------------------------------------------- chunk after chunk
 
-// A workgroup owns NC tiles of 16 columns, from the first chunk to the last; its C / 16 waves share the rows.  Wave w forms rows
-// perm_row(w, .) of K S, Q S, u and o, and keeps TW tiles of the state in registers; what a product needs of the other waves'
-// results (S, beta (v - exp(G_i) K S), u) goes through LDS as planes in operand order, three barriers a chunk.  The fragments of
-// the next chunk are loaded as soon as those of this one are used.  Bound by the chain of products and exchanges of a chunk
-// (with few heads) or by issue and LDS (with many): one wave for all rows took four times as long for a chunk.
+// A workgroup owns NC tiles of 16 columns, from the first chunk to the last.  C / 16 waves carry the state: wave w forms rows
+// perm_row(w, .) of K S and u, and keeps TW tiles of S in registers; as many more waves form o (Q S and P u) beside them.  What
+// a product needs of the other waves' results (S, beta (v - exp(G_i) K S), u) goes through LDS as planes in operand order,
+// three barriers a chunk.  The fragments of the next chunk are loaded as soon as those of this one are used.
+//
+// Bound by a chunk's chain of products and exchanges (few heads) or by loads and issue (many).  T 8192 of 128 x 128, bf16: one
+// wave for all rows and products took 6.3 us a chunk, four waves 2.5 us.
 template <int DT, int KP, int C, int NC, bool SAVE>
 struct Scan {
   using S = DeltaShape<DT, KP, C, SAVE>;
@@ -250,13 +252,13 @@ struct Scan {
 };
 
 template <int DT, int KP, int C, int NC, bool SAVE>
-__global__ __launch_bounds__(4 * C) void k_delta_scan(DeltaArgs a) {
+__global__ __launch_bounds__(8 * C, 2) void k_delta_scan(DeltaArgs a) {
   using S = DeltaShape<DT, KP, C, SAVE>;
   using Sc = Scan<DT, KP, C, NC, SAVE>;
   using T = typename Elem<DT>::T;
   constexpr int NP = S::NP, NO = S::NO, TW = Sc::TW;
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  const int lane = threadIdx.x & 63, w = wave_id(), x = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = wave_id(), w = wave % S::RT, x = lane & 15, g = lane >> 4;
   const int groups = (a.VP / 16 + NC - 1) / NC;
   int64_t head;
   int group;
@@ -266,244 +268,306 @@ __global__ __launch_bounds__(4 * C) void k_delta_scan(DeltaArgs a) {
   const int col0 = group * NC * 16 + x;   // the lane's column in the first tile
   int64_t begin, len, c0;
   a.rows.range(n, begin, len, c0);
-  const int64_t nc = (len + C - 1) / C;
-  const bool holds = w * TW < S::KT;      // whether this wave has tiles of the state
+  begin = uniform(begin), len = uniform(len), c0 = uniform(c0);
+  const int nc = (int)((len + C - 1) / C);
   const int row0 = perm_row(w, 4 * g);    // its rows of a chunk: row0..row0 + 3
   const float nan = __builtin_nanf("");
-
-  f32x4 st[NC][TW];
-#pragma unroll
-  for (int i = 0; i < NC; ++i)
-#pragma unroll
-    for (int t = 0; t < TW; ++t)
-      st[i][t] = load_state(a.initial && holds ? a.initial + head * a.K * a.V : nullptr, a.K, a.V, col0 + 16 * i, w * TW + t, g);
+  const uint32_t at16 = lane * 16;
 
   const char* kq = a.kq + (c0 * a.Hk + hk) * (int64_t)S::kKQ;
   const char* xp = a.xp + (c0 * a.Hv + h) * (int64_t)S::kXP;
-  const float* vec = reinterpret_cast<const float*>(a.vec + (c0 * a.Hv + h) * (int64_t)kVec);
-  const int64_t kq_step = (int64_t)a.Hk * S::kKQ, xp_step = (int64_t)a.Hv * S::kXP, vec_step = (int64_t)a.Hv * (kVec / 4);
-  const T* vp[NC];
-  T* op[NC];
+  const char* vec = a.vec + (c0 * a.Hv + h) * (int64_t)kVec;
+  const int64_t kq_step = (int64_t)a.Hk * S::kKQ, xp_step = (int64_t)a.Hv * S::kXP, vec_step = (int64_t)a.Hv * kVec;
   bool in[NC];
-  const int64_t orow = (int64_t)a.Hv * a.V;
 #pragma unroll
-  for (int i = 0; i < NC; ++i) {
-    const int col = col0 + 16 * i;
-    in[i] = col < a.V;
-    vp[i] = static_cast<const T*>(a.v) + a.rows.batch(n) * a.vs[0] + begin * a.vs[1] + h * a.vs[2] + (in[i] ? col : a.V - 1);
-    op[i] = static_cast<T*>(a.o) + ((a.rows.batch(n) * a.rows.T + begin) * a.Hv + h) * (int64_t)a.V + col + row0 * orow;
-  }
+  for (int i = 0; i < NC; ++i) in[i] = col0 + 16 * i < a.V;
+  int* const bads = reinterpret_cast<int*>(lds + Sc::bad);
+  auto part = [&](int i, int b) { return lds + (i * Sc::bEnd + b) * 1024; };
+  // the first row of a lane's column that is not finite
+  auto first_bad = [&](int i) {
+    int b = C;
+#pragma unroll
+    for (int r = 0; r < S::RT; ++r) b = min(b, bads[(i * 16 + x) * S::RT + r]);
+    return b;
+  };
 
-  bf16x8 fk[S::KS][NP], fq[S::KS][NP], fx[S::CS][3], fp[S::CS][NO], ft[TW][S::CS][NP];
-  f32x4 into, left, beta;
-  float all = 0.f, first_bad = 0.f;
-  ColumnRows<T> v[NC];
-  auto load_kq = [&](const char* p) {
+  if (wave < S::RT) {   // ---- the state
+    const bool holds = w * TW < S::KT;      // whether this wave has tiles of it
+    f32x4 st[NC][TW];
 #pragma unroll
-    for (int s = 0; s < S::KS; ++s) {
-      load_frag<NP>(p, (S::fK + w * S::KS + s) * NP, lane, fk[s]);
-      load_frag<NP>(p, (S::fQ + w * S::KS + s) * NP, lane, fq[s]);
-    }
-  };
-  auto load_x = [&](const char* p) {   // (rows of the upper half have no second inner step: theirs is loaded, not used)
+    for (int i = 0; i < NC; ++i)
 #pragma unroll
-    for (int s = 0; s < S::CS; ++s) load_frag<3>(p, S::pX + 3 * tri_frag(w, s <= w / 2 ? s : 0), lane, fx[s]);
-  };
-  auto load_pt = [&](const char* p, const char* k) {
+      for (int t = 0; t < TW; ++t)
+        st[i][t] = load_state(a.initial && holds ? a.initial + head * a.K * a.V : nullptr, a.K, a.V, col0 + 16 * i, w * TW + t, g);
+    const T* vp[NC];
 #pragma unroll
-    for (int s = 0; s < S::CS; ++s) load_frag<NO>(p, S::pP + S::NPP * tri_frag(w, s <= w / 2 ? s : 0), lane, fp[s]);
-    if (holds) {
+    for (int i = 0; i < NC; ++i)
+      vp[i] = static_cast<const T*>(a.v) + a.rows.batch(n) * a.vs[0] + begin * a.vs[1] + h * a.vs[2] + (in[i] ? col0 + 16 * i : a.V - 1);
+    int64_t vrow[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) vrow[r] = (row0 + r) * a.vs[1];
+
+    bf16x8 fk[S::KS][NP], fx[S::CS][3], ft[TW][S::CS][NP];
+    f32x4 into, left, beta;
+    float all = 0.f, bad0 = 0.f;
+    ColumnRows<T, C> v[NC];
+    auto load_k = [&]() {
+#pragma unroll
+      for (int s = 0; s < S::KS; ++s) load_frag<NP>(kq, (S::fK + w * S::KS + s) * NP, at16, fk[s]);
+    };
+    auto load_x = [&]() {   // (rows of the upper half have no second inner step: theirs is loaded, not used)
+#pragma unroll
+      for (int s = 0; s < S::CS; ++s) load_frag<3>(xp, S::pX + 3 * tri_frag(w, s <= w / 2 ? s : 0), at16, fx[s]);
+    };
+    auto load_t = [&]() {
+      if (!holds) return;
 #pragma unroll
       for (int t = 0; t < TW; ++t)
 #pragma unroll
-        for (int s = 0; s < S::CS; ++s) load_frag<NP>(k, (S::fKT + (w * TW + t) * S::CS + s) * NP, lane, ft[t][s]);
+        for (int s = 0; s < S::CS; ++s) load_frag<NP>(kq, (S::fKT + (w * TW + t) * S::CS + s) * NP, at16, ft[t][s]);
+    };
+    auto load_v = [&](int ci) {
+      const int64_t left_rows = len - (int64_t)ci * C;
+#pragma unroll
+      for (int i = 0; i < NC; ++i) v[i].load(vp[i] + (int64_t)ci * C * a.vs[1], vrow, a.vs[1], (int)(left_rows < C ? left_rows : C), row0);
+    };
+    auto load_vec = [&]() {
+      const float* p = reinterpret_cast<const float*>(vec);
+      into = *reinterpret_cast<const f32x4*>(p + row0);
+      left = *reinterpret_cast<const f32x4*>(p + 64 + row0);
+      beta = *reinterpret_cast<const f32x4*>(p + 128 + row0);
+      all = p[192];
+      bad0 = p[193];
+    };
+    auto put_state = [&]() {
+      if (!holds) return;
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        if constexpr (TW >= 2) {
+#pragma unroll
+          for (int t = 0; t < TW; t += 2) put_whole<3>(part(i, Sc::bS), (w * TW + t) / 2, lane, cat8(st[i][t], st[i][t + 1]));
+        } else {
+          put_half<3>(part(i, Sc::bS), w / 2, w & 1, lane, st[i][0]);
+        }
+      }
+    };
+    if (nc > 0) {
+      load_k();
+      load_v(0);
+      load_vec();
+      load_x();
+      load_t();
+      put_state();
     }
-  };
-  auto load_v = [&](int64_t ci) {
-    const int rows = (int)(len - ci * C < C ? len - ci * C : C);
+    for (int ci = 0; ci < nc; ++ci) {
+      const bool more = ci + 1 < nc;   // behind the last chunk its own values are loaded again, and not used
+      const int64_t ch = (c0 + ci) * a.Hv + h;
+      lds_barrier();   // S is in LDS
+      // K S, the inner steps in two chains
+      f32x4 ks[NC], ks2[NC];
 #pragma unroll
-    for (int i = 0; i < NC; ++i) v[i].load(vp[i] + ci * C * a.vs[1], a.vs[1], rows, row0);
-  };
-  auto load_vec = [&](const float* p) {
-    into = *reinterpret_cast<const f32x4*>(p + row0);
-    left = *reinterpret_cast<const f32x4*>(p + 64 + row0);
-    beta = *reinterpret_cast<const f32x4*>(p + 128 + row0);
-    all = p[192];
-    first_bad = p[193];
-  };
-  auto put_state = [&]() {
-    if (!holds) return;
+      for (int i = 0; i < NC; ++i) ks[i] = ks2[i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < NC; ++i) {
-      char* b = lds + (i * Sc::bEnd + Sc::bS) * 1024;
-      if constexpr (TW >= 2) {
+      for (int s = 0; s < S::KS; ++s)
 #pragma unroll
-        for (int t = 0; t < TW; t += 2) put_whole<3>(b, (w * TW + t) / 2, lane, cat8(st[i][t], st[i][t + 1]));
-      } else {
-        put_half<3>(b, w / 2, w & 1, lane, st[i][0]);
+        for (int i = 0; i < NC; ++i) {
+          bf16x8 sp[3];
+          get_operand<3>(part(i, Sc::bS), s, lane, sp);
+          f32x4& k = s & 1 ? ks2[i] : ks[i];
+          k = mfma_planes<NP, 3, 3>(fk[s], sp, k);
+        }
+      if (more) kq += kq_step;
+      load_k();
+      // beta (v - exp(G_i) K S)
+      int bad[NC];
+      float odd = 0.f;
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        ks[i] = beta * (v[i].get(in[i], row0) - into * (ks[i] + ks2[i]));
+        odd += zero_if_finite(ks[i]);
+        bad[i] = (int)bad0;
+      }
+      if (__ballot(odd != 0.f)) {
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+#pragma unroll
+          for (int r = 3; r >= 0; --r)
+            if (ks[i][r] - ks[i][r] != 0.f) {
+              ks[i][r] = 0.f;
+              bad[i] = row0 + r < bad[i] ? row0 + r : bad[i];
+            }
+          bad[i] = min(bad[i], __shfl_xor(bad[i], 16));
+          bad[i] = min(bad[i], __shfl_xor(bad[i], 32));
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        put_half<3>(part(i, Sc::bR), w / 2, w & 1, lane, ks[i]);
+        if (g == 0) bads[(i * 16 + x) * S::RT + w] = bad[i];
+      }
+      load_v(more ? ci + 1 : ci);
+      if (SAVE && holds) {
+        float* s0 = a.s0 + ch * (int64_t)KP * a.VP + col0;
+#pragma unroll
+        for (int i = 0; i < NC; ++i)
+#pragma unroll
+          for (int t = 0; t < TW; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (col0 + 16 * i < a.VP) s0[perm_row(w * TW + t, 4 * g + r) * a.VP + 16 * i] = st[i][t][r];
+      }
+      lds_barrier();
+      // u = X of it
+      f32x4 u[NC];
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        f32x4 u2 = {0.f, 0.f, 0.f, 0.f};
+        u[i] = u2;
+        bf16x8 rp[3];
+        get_operand<3>(part(i, Sc::bR), 0, lane, rp);
+        u[i] = mfma_planes<3, 3, 3>(fx[0], rp, u[i]);
+        if (S::CS > 1 && w >= 2) {
+          get_operand<3>(part(i, Sc::bR), S::CS - 1, lane, rp);
+          u2 = mfma_planes<3, 3, 3>(fx[S::CS - 1], rp, u2);
+        }
+        u[i] += u2;
+        put_half<3>(part(i, Sc::bL), w / 2, w & 1, lane, left * u[i]);
+        put_half<NO>(part(i, Sc::bU), w / 2, w & 1, lane, u[i]);
+        bad[i] = first_bad(i);
+      }
+      if (more) xp += xp_step;
+      load_x();
+      const float all_now = all;
+      if (more) vec += vec_step;
+      load_vec();
+      lds_barrier();
+      // S <- exp(G) S + K^T (exp(G - G_i) u)
+      bool any_bad = false;
+#pragma unroll
+      for (int i = 0; i < NC; ++i) any_bad |= bad[i] < C;
+      if (holds) {
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+#pragma unroll
+          for (int t = 0; t < TW; ++t) st[i][t] *= all_now;
+#pragma unroll
+          for (int s = 0; s < S::CS; ++s) {
+            bf16x8 up[3];
+            get_operand<3>(part(i, Sc::bL), s, lane, up);
+#pragma unroll
+            for (int t = 0; t < TW; ++t) st[i][t] = mfma_planes<NP, 3, 3>(ft[t][s], up, st[i][t]);
+          }
+        }
+      }
+      if (__ballot(any_bad)) {   // what is not finite: NaN from its row on
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+#pragma unroll
+          for (int t = 0; t < TW; ++t)
+            if (bad[i] < C) st[i][t] = f32x4{nan, nan, nan, nan};
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (row0 + r >= bad[i]) u[i][r] = nan;
+        }
+      }
+      put_state();
+      load_t();
+      if (SAVE) {
+        float* us = a.u + (ch * C + row0) * (int64_t)a.VP + col0;
+#pragma unroll
+        for (int i = 0; i < NC; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (col0 + 16 * i < a.VP) us[r * a.VP + 16 * i] = u[i][r];
       }
     }
-  };
-  if (nc > 0) {
-    load_kq(kq);
-    load_v(0);
-    load_vec(vec);
-    load_x(xp);
-    load_pt(xp, kq);
-    put_state();
-  }
-  int* const bads = reinterpret_cast<int*>(lds + Sc::bad);
-  for (int64_t ci = 0; ci < nc; ++ci) {
-    const bool more = ci + 1 < nc;   // behind the last chunk its own values are loaded again, and not used
-    const int64_t ch = (c0 + ci) * a.Hv + h;
-    const int rows = (int)(len - ci * C < C ? len - ci * C : C);
-    f32x4 vc[NC];
-#pragma unroll
-    for (int i = 0; i < NC; ++i) vc[i] = v[i].get(in[i], row0);
-    lds_barrier();   // the state is in LDS
-    if (SAVE && holds) {
-      float* s0 = a.s0 + ch * (int64_t)KP * a.VP + col0;
+    if (holds) {
 #pragma unroll
       for (int i = 0; i < NC; ++i)
 #pragma unroll
         for (int t = 0; t < TW; ++t)
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (col0 + 16 * i < a.VP) s0[(int64_t)perm_row(w * TW + t, 4 * g + r) * a.VP + 16 * i] = st[i][t][r];
-    }
-    // K S and Q S, the inner steps in two chains
-    f32x4 ks[NC], o[NC], ks2[NC], o2[NC];
-#pragma unroll
-    for (int i = 0; i < NC; ++i) ks[i] = o[i] = ks2[i] = o2[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int s = 0; s < S::KS; ++s) {
-#pragma unroll
-      for (int i = 0; i < NC; ++i) {
-        bf16x8 sp[3], so[NO];
-        get_operand<3>(lds + (i * Sc::bEnd + Sc::bS) * 1024, s, lane, sp);
-#pragma unroll
-        for (int j = 0; j < NO; ++j) so[j] = sp[j];
-        f32x4& k = s & 1 ? ks2[i] : ks[i];
-        f32x4& q = s & 1 ? o2[i] : o[i];
-        k = mfma_planes<NP, 3, 3>(fk[s], sp, k);
-        q = mfma_planes<NP, NO, NO>(fq[s], so, q);
-      }
-    }
-    if (more) kq += kq_step;
-    load_kq(kq);
-    // beta (v - exp(G_i) K S)
-    const int bad0 = (int)first_bad;
-    float odd = 0.f;
-#pragma unroll
-    for (int i = 0; i < NC; ++i) {
-      ks[i] = beta * (vc[i] - into * (ks[i] + ks2[i]));
-      o[i] = (a.scale * into) * (o[i] + o2[i]);
-      odd += zero_if_finite(ks[i]);
-    }
-    int bad[NC];
-#pragma unroll
-    for (int i = 0; i < NC; ++i) bad[i] = bad0;
-    if (__ballot(odd != 0.f)) {
-#pragma unroll
-      for (int i = 0; i < NC; ++i) {
-#pragma unroll
-        for (int r = 3; r >= 0; --r)
-          if (ks[i][r] - ks[i][r] != 0.f) {
-            ks[i][r] = 0.f;
-            bad[i] = row0 + r < bad[i] ? row0 + r : bad[i];
+          for (int r = 0; r < 4; ++r) {
+            const int kd = perm_row(w * TW + t, 4 * g + r);
+            if (in[i] && kd < a.K) a.final[(head * a.K + kd) * a.V + col0 + 16 * i] = st[i][t][r];
           }
-        bad[i] = min(bad[i], __shfl_xor(bad[i], 16));
-        bad[i] = min(bad[i], __shfl_xor(bad[i], 32));
-      }
     }
-#pragma unroll
-    for (int i = 0; i < NC; ++i) {
-      put_half<3>(lds + (i * Sc::bEnd + Sc::bR) * 1024, w / 2, w & 1, lane, ks[i]);
-      if (g == 0) bads[(i * 16 + x) * S::RT + w] = bad[i];
-    }
-    lds_barrier();
+  } else {   // ---- o
+    T* op[NC];
+    const int64_t orow = (int64_t)a.Hv * a.V;
 #pragma unroll
     for (int i = 0; i < NC; ++i)
+      op[i] = static_cast<T*>(a.o) + ((a.rows.batch(n) * a.rows.T + begin) * a.Hv + h) * (int64_t)a.V + col0 + 16 * i + row0 * orow;
+    bf16x8 fq[S::KS][NP], fp[S::CS][NO];
+    f32x4 into;
+    auto load_q = [&]() {
 #pragma unroll
-      for (int r = 0; r < S::RT; ++r) bad[i] = min(bad[i], bads[(i * 16 + x) * S::RT + r]);
-    // u = X of it
-    f32x4 u[NC];
+      for (int s = 0; s < S::KS; ++s) load_frag<NP>(kq, (S::fQ + w * S::KS + s) * NP, at16, fq[s]);
+      into = *reinterpret_cast<const f32x4*>(vec + row0 * 4);
+    };
+    auto load_p = [&]() {
 #pragma unroll
-    for (int i = 0; i < NC; ++i) {
-      f32x4 u2 = {0.f, 0.f, 0.f, 0.f};
-      u[i] = u2;
-      bf16x8 rp[3];
-      get_operand<3>(lds + (i * Sc::bEnd + Sc::bR) * 1024, 0, lane, rp);
-      u[i] = mfma_planes<3, 3, 3>(fx[0], rp, u[i]);
-      if (S::CS > 1 && w >= 2) {
-        get_operand<3>(lds + (i * Sc::bEnd + Sc::bR) * 1024, S::CS - 1, lane, rp);
-        u2 = mfma_planes<3, 3, 3>(fx[S::CS - 1], rp, u2);
-      }
-      u[i] += u2;
-      put_half<NO>(lds + (i * Sc::bEnd + Sc::bU) * 1024, w / 2, w & 1, lane, u[i]);
-      put_half<3>(lds + (i * Sc::bEnd + Sc::bL) * 1024, w / 2, w & 1, lane, left * u[i]);
+      for (int s = 0; s < S::CS; ++s) load_frag<NO>(xp, S::pP + S::NPP * tri_frag(w, s <= w / 2 ? s : 0), at16, fp[s]);
+    };
+    if (nc > 0) {
+      load_q();
+      load_p();
     }
-    if (more) xp += xp_step;
-    load_x(xp);
-    const float all_now = all;
-    if (more) vec += vec_step;
-    load_vec(vec);
-    load_v(more ? ci + 1 : ci);
-    lds_barrier();
-    // o += P u
+    for (int ci = 0; ci < nc; ++ci) {
+      const bool more = ci + 1 < nc;
+      const int rows = (int)(len - (int64_t)ci * C < C ? len - (int64_t)ci * C : C);
+      lds_barrier();
+      f32x4 o[NC], o2[NC];
 #pragma unroll
-    for (int i = 0; i < NC; ++i) {
-      bf16x8 up[NO];
-      get_operand<NO>(lds + (i * Sc::bEnd + Sc::bU) * 1024, 0, lane, up);
-      o[i] = mfma_planes<NO, NO, NO>(fp[0], up, o[i]);
-      if (S::CS > 1 && w >= 2) {
-        get_operand<NO>(lds + (i * Sc::bEnd + Sc::bU) * 1024, S::CS - 1, lane, up);
-        o[i] = mfma_planes<NO, NO, NO>(fp[S::CS - 1], up, o[i]);
-      }
-    }
-    // S <- exp(G) S + K^T (exp(G - G_i) u)
-    if (holds) {
+      for (int i = 0; i < NC; ++i) o[i] = o2[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < S::KS; ++s)
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+          bf16x8 so[NO];
+          get_operand<3, NO>(part(i, Sc::bS), s, lane, so);
+          f32x4& q = s & 1 ? o2[i] : o[i];
+          q = mfma_planes<NP, NO, NO>(fq[s], so, q);
+        }
+#pragma unroll
+      for (int i = 0; i < NC; ++i) o[i] = (a.scale * into) * (o[i] + o2[i]);
+      if (more) kq += kq_step, vec += vec_step;
+      load_q();
+      lds_barrier();
+      lds_barrier();
+      int bad[NC];
 #pragma unroll
       for (int i = 0; i < NC; ++i) {
-#pragma unroll
-        for (int t = 0; t < TW; ++t) st[i][t] *= all_now;
-#pragma unroll
-        for (int s = 0; s < S::CS; ++s) {
-          bf16x8 up[3];
-          get_operand<3>(lds + (i * Sc::bEnd + Sc::bL) * 1024, s, lane, up);
-#pragma unroll
-          for (int t = 0; t < TW; ++t) st[i][t] = mfma_planes<NP, 3, 3>(ft[t][s], up, st[i][t]);
+        bf16x8 up[NO];
+        get_operand<NO>(part(i, Sc::bU), 0, lane, up);
+        o[i] = mfma_planes<NO, NO, NO>(fp[0], up, o[i]);
+        if (S::CS > 1 && w >= 2) {
+          get_operand<NO>(part(i, Sc::bU), S::CS - 1, lane, up);
+          o[i] = mfma_planes<NO, NO, NO>(fp[S::CS - 1], up, o[i]);
         }
-        if (bad[i] < C) {
+        bad[i] = first_bad(i);
+      }
+      if (more) xp += xp_step;
+      load_p();
 #pragma unroll
-          for (int t = 0; t < TW; ++t) st[i][t] = f32x4{nan, nan, nan, nan};
+      for (int i = 0; i < NC; ++i) {
+        if (__ballot(bad[i] < C)) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (row0 + r >= bad[i]) o[i][r] = nan;
         }
+        if (rows == C) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (in[i]) op[i][r * orow] = (T)o[i][r];
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (in[i] && row0 + r < rows) op[i][r * orow] = (T)o[i][r];
+        }
+        op[i] += C * orow;
       }
     }
-    load_pt(xp, kq);
-    put_state();
-    // out, values from the first row that is not finite on as NaN
-#pragma unroll
-    for (int i = 0; i < NC; ++i) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const bool gone = row0 + r >= bad[i];
-        if (SAVE && col0 + 16 * i < a.VP) a.u[(ch * C + row0 + r) * (int64_t)a.VP + col0 + 16 * i] = gone ? nan : u[i][r];
-        if (in[i] && row0 + r < rows) op[i][r * orow] = (T)(gone ? nan : o[i][r]);
-      }
-      op[i] += C * orow;
-    }
-  }
-  if (holds) {
-#pragma unroll
-    for (int i = 0; i < NC; ++i)
-#pragma unroll
-      for (int t = 0; t < TW; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int kd = perm_row(w * TW + t, 4 * g + r);
-          if (in[i] && kd < a.K) a.final[(head * a.K + kd) * a.V + col0 + 16 * i] = st[i][t][r];
-        }
   }
 }
 
@@ -525,7 +589,7 @@ hipError_t scan(const DeltaArgs& a, hipStream_t s) {
   const hipError_t e = allow_lds(k_delta_scan<DT, KP, C, NC, SAVE>, Sc::bytes);
   if (e != hipSuccess) return e;
   const int64_t groups = (a.VP / 16 + NC - 1) / NC, heads = (a.rows.N * a.Hv + 7) / 8 * 8;
-  k_delta_scan<DT, KP, C, NC, SAVE><<<(unsigned)(heads * groups), 4 * C, Sc::bytes, s>>>(a);
+  k_delta_scan<DT, KP, C, NC, SAVE><<<(unsigned)(heads * groups), 8 * C, Sc::bytes, s>>>(a);
   return hipGetLastError();
 }
 

@@ -52,10 +52,17 @@ __device__ __forceinline__ double running_sum(float v, int lane, double& last) {
 
 // ---- fragments in the work memory and operands B in LDS
 
+// a value that is the same in all lanes, as a scalar (addresses made of it need no vector arithmetic)
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+  return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v) |
+                   (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32);
+}
+
+// base: scalar; at16: 16 * lane
 template <int NP>
-__device__ __forceinline__ void load_frag(const char* base, int plane, int lane, bf16x8 (&a)[NP]) {
+__device__ __forceinline__ void load_frag(const char* base, int plane, uint32_t at16, bf16x8 (&a)[NP]) {
 #pragma unroll
-  for (int i = 0; i < NP; ++i) a[i] = *reinterpret_cast<const bf16x8*>(base + (plane + i) * 1024 + lane * 16);
+  for (int i = 0; i < NP; ++i) a[i] = *reinterpret_cast<const bf16x8*>(base + (plane + i) * 1024 + at16);
 }
 // half p (rows of tile 2 s + p) of an operand B
 template <int NP>
@@ -75,10 +82,11 @@ __device__ __forceinline__ void put_whole(char* lds, int s, int lane, f32x8 v) {
 #pragma unroll
   for (int i = 0; i < NP; ++i) *reinterpret_cast<bf16x8*>(lds + (s * NP + i) * 1024 + lane * 16) = b[i];
 }
-template <int NP>
-__device__ __forceinline__ void get_operand(const char* lds, int s, int lane, bf16x8 (&b)[NP]) {
+// the first NB of an operand's NP planes
+template <int NP, int NB = NP>
+__device__ __forceinline__ void get_operand(const char* lds, int s, int lane, bf16x8 (&b)[NB]) {
 #pragma unroll
-  for (int i = 0; i < NP; ++i) b[i] = *reinterpret_cast<const bf16x8*>(lds + (s * NP + i) * 1024 + lane * 16);
+  for (int i = 0; i < NB; ++i) b[i] = *reinterpret_cast<const bf16x8*>(lds + (s * NP + i) * 1024 + lane * 16);
 }
 // LDS writes of all waves before, LDS reads after; loads from global memory stay in flight
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
@@ -86,15 +94,21 @@ __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(
 // A lane's share of a chunk's rows of a tensor: rows perm_row(t, 4 g + r) of the lane's column.  The loads are unconditional
 // (rows and columns outside are taken from the nearest inside, and become zeros on the way out), so that all of them are in
 // flight at once; a branch around each made the compiler wait for each.
-template <class T>
+template <class T, int C>
 struct ColumnRows {
   T raw[4];
   int left;   // rows of the chunk
-  // p: the chunk's first row, at the lane's column or the row's last
-  __device__ __forceinline__ void load(const T* p, int64_t stride, int rows, int row0) {
+  // p: the chunk's first row, at the lane's column or the row's last; at[r]: r rows behind the lane's first (in elements)
+  __device__ __forceinline__ void load(const T* p, const int64_t (&at)[4], int64_t stride, int rows, int row0) {
     left = rows;
+    if (rows == C) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) raw[r] = p[(row0 + r < rows ? row0 + r : rows - 1) * stride];
+      for (int r = 0; r < 4; ++r) raw[r] = p[at[r]];
+    } else {
+      asm volatile("");   // a branch: the products below are not worth forming for every chunk
+#pragma unroll
+      for (int r = 0; r < 4; ++r) raw[r] = p[(row0 + r < rows ? row0 + r : rows - 1) * stride];
+    }
   }
   __device__ __forceinline__ f32x4 get(bool in, int row0) const {
     f32x4 v;

@@ -76,19 +76,22 @@ __global__ __launch_bounds__(4 * C) void k_delta_back(DeltaGradArgs ga) {
   bf16x8 fk[S::KS][NP], fx[S::CS][3], fp[S::CS][3], fq[TW][S::CS][NP], ft[TW][S::CS][NP];
   f32x4 into, left, beta;
   float all = 0.f;
-  ColumnRows<T> d[NC];
+  ColumnRows<T, C> d[NC];
+  int64_t drow[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) drow[r] = (row0 + r) * orow;
   auto tri_t = [&](int s) { return C == 32 ? w : tri_frag_t(w, s < w / 2 ? w / 2 : s); };   // below the diagonal: loaded, not used
   auto load_k = [&](const char* p) {
 #pragma unroll
-    for (int s = 0; s < S::KS; ++s) load_frag<NP>(p, (S::fK + w * S::KS + s) * NP, lane, fk[s]);
+    for (int s = 0; s < S::KS; ++s) load_frag<NP>(p, (S::fK + w * S::KS + s) * NP, lane * 16, fk[s]);
   };
   auto load_p = [&](const char* p) {
 #pragma unroll
-    for (int s = 0; s < S::CS; ++s) load_frag<3>(p, S::pPT + 3 * tri_t(s), lane, fp[s]);
+    for (int s = 0; s < S::CS; ++s) load_frag<3>(p, S::pPT + 3 * tri_t(s), lane * 16, fp[s]);
   };
   auto load_x = [&](const char* p) {
 #pragma unroll
-    for (int s = 0; s < S::CS; ++s) load_frag<3>(p, S::pXT + 3 * tri_t(s), lane, fx[s]);
+    for (int s = 0; s < S::CS; ++s) load_frag<3>(p, S::pXT + 3 * tri_t(s), lane * 16, fx[s]);
   };
   auto load_t = [&](const char* p) {
     if (!holds) return;
@@ -96,14 +99,14 @@ __global__ __launch_bounds__(4 * C) void k_delta_back(DeltaGradArgs ga) {
     for (int t = 0; t < TW; ++t)
 #pragma unroll
       for (int s = 0; s < S::CS; ++s) {
-        load_frag<NP>(p, (S::fQT + (w * TW + t) * S::CS + s) * NP, lane, fq[t][s]);
-        load_frag<NP>(p, (S::fKT + (w * TW + t) * S::CS + s) * NP, lane, ft[t][s]);
+        load_frag<NP>(p, (S::fQT + (w * TW + t) * S::CS + s) * NP, lane * 16, fq[t][s]);
+        load_frag<NP>(p, (S::fKT + (w * TW + t) * S::CS + s) * NP, lane * 16, ft[t][s]);
       }
   };
   auto load_do = [&](int64_t ci) {
     const int rows = (int)(len - ci * C < C ? len - ci * C : C);
 #pragma unroll
-    for (int i = 0; i < NC; ++i) d[i].load(dop[i] + ci * C * orow, orow, rows, row0);
+    for (int i = 0; i < NC; ++i) d[i].load(dop[i] + ci * C * orow, drow, orow, rows, row0);
   };
   auto load_vec = [&](const float* p) {
     into = *reinterpret_cast<const f32x4*>(p + row0);
@@ -206,7 +209,7 @@ __global__ __launch_bounds__(4 * C) void k_delta_back(DeltaGradArgs ga) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         if (col0 + 16 * i < a.VP) ga.dr[(ch * C + row0 + r) * (int64_t)a.VP + col0 + 16 * i] = dr[r];
-        if (in[i] && row0 + r < rows) dvp[i][(ci * C + row0 + r) * orow] = (T)dv[r];
+        if (in[i] && row0 + r < rows) dvp[i][ci * C * orow + drow[r]] = (T)dv[r];
       }
     }
     load_x(xp);
