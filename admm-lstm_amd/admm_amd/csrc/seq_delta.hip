@@ -236,18 +236,20 @@ __global__ __launch_bounds__(4 * C) void k_delta_prep(DeltaArgs a) {
 
 // --------------------------------------------------------------------------------------------- chunk after chunk
 
-// A workgroup owns NC tiles of 16 columns, from the first chunk to the last.  C / 16 waves carry the state: wave w forms rows
-// perm_row(w, .) of K S and u, and keeps TW tiles of S in registers; as many more waves form o (Q S and P u) beside them.  What
-// a product needs of the other waves' results (S, beta (v - exp(G_i) K S), u) goes through LDS as planes in operand order,
-// three barriers a chunk.  The fragments of the next chunk are loaded as soon as those of this one are used.
+// A workgroup owns NC tiles of 16 columns, from the first chunk to the last.  C / 16 waves carry the state: each keeps TW tiles
+// of S in registers and forms their share of K S for all rows; the shares are added up in LDS, where wave w takes rows
+// perm_row(w, .) of R = beta (v - exp(G_i) K S) and of u.  R and u are handed on as planes in operand order: three barriers a
+// chunk.  As many more waves form o (Q S and P u) beside them, a step behind.  The fragments of the next chunk are loaded as
+// soon as those of this one are used.
 //
 // Bound by a chunk's chain of products and exchanges (few heads) or by loads and issue (many).  T 8192 of 128 x 128, bf16: one
-// wave for all rows and products took 6.3 us a chunk, four waves 2.5 us.
+// wave for all rows and products took 6.3 us a chunk, four waves 2.5 us, eight with all of S handed through LDS 2.0 us.
 template <int DT, int KP, int C, int NC, bool SAVE>
 struct Scan {
   using S = DeltaShape<DT, KP, C, SAVE>;
-  static constexpr int TW = S::KT >= S::RT ? S::KT / S::RT : 1;
-  static constexpr int bS = 0, bR = S::KS * 3, bU = bR + S::CS * 3, bL = bU + S::CS * S::NO, bEnd = bL + S::CS * 3;   // KB
+  static constexpr int TW = S::KT >= 2 * S::RT ? S::KT / S::RT : 2, HW = S::KT / TW;   // HW waves have tiles of the state
+  static constexpr int bS = 0, bK = S::KS * S::NO, bR = bK + HW * S::RT, bU = bR + S::CS * 3, bL = bU + S::CS * S::NO,
+                       bEnd = bL + S::CS * 3;   // KB
   static constexpr int bad = NC * bEnd * 1024, bytes = bad + NC * 16 * S::RT * 4;
 };
 
@@ -256,15 +258,14 @@ __global__ __launch_bounds__(8 * C, 2) void k_delta_scan(DeltaArgs a) {
   using S = DeltaShape<DT, KP, C, SAVE>;
   using Sc = Scan<DT, KP, C, NC, SAVE>;
   using T = typename Elem<DT>::T;
-  constexpr int NP = S::NP, NO = S::NO, TW = Sc::TW;
+  constexpr int NP = S::NP, NO = S::NO, TW = Sc::TW, HW = Sc::HW;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lane = threadIdx.x & 63, wave = wave_id(), w = wave % S::RT, x = lane & 15, g = lane >> 4;
   const int groups = (a.VP / 16 + NC - 1) / NC;
-  int64_t head;
-  int group;
-  if (!place_columns(a.rows.N * a.Hv, groups, head, group)) return;
-  const int64_t n = head / a.Hv;
-  const int h = (int)(head % a.Hv), hk = h / (a.Hv / a.Hk);
+  int64_t n;
+  int h, hk, group;
+  if (!place_columns(a, groups, n, h, hk, group)) return;
+  const int64_t head = n * a.Hv + h;
   const int col0 = group * NC * 16 + x;   // the lane's column in the first tile
   int64_t begin, len, c0;
   a.rows.range(n, begin, len, c0);
@@ -292,7 +293,7 @@ __global__ __launch_bounds__(8 * C, 2) void k_delta_scan(DeltaArgs a) {
   };
 
   if (wave < S::RT) {   // ---- the state
-    const bool holds = w * TW < S::KT;      // whether this wave has tiles of it
+    const bool holds = w < HW;              // whether this wave has tiles of it
     f32x4 st[NC][TW];
 #pragma unroll
     for (int i = 0; i < NC; ++i)
@@ -307,18 +308,25 @@ __global__ __launch_bounds__(8 * C, 2) void k_delta_scan(DeltaArgs a) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) vrow[r] = (row0 + r) * a.vs[1];
 
-    bf16x8 fk[S::KS][NP], fx[S::CS][3], ft[TW][S::CS][NP];
-    f32x4 into, left, beta;
-    float all = 0.f, bad0 = 0.f;
+    bf16x8 fk[S::RT][TW / 2][NP], fx[S::CS][3], ft[TW][S::CS][NP];
+    struct { f32x4 into, left, beta; float all, bad; } f, fnext;   // of the wave's rows
     ColumnRows<T, C> v[NC];
     auto load_k = [&]() {
+      if (!holds) return;
 #pragma unroll
-      for (int s = 0; s < S::KS; ++s) load_frag<NP>(kq, (S::fK + w * S::KS + s) * NP, at16, fk[s]);
-    };
-    auto load_x = [&]() {   // (rows of the upper half have no second inner step: theirs is loaded, not used)
+      for (int t = 0; t < S::RT; ++t)
 #pragma unroll
-      for (int s = 0; s < S::CS; ++s) load_frag<3>(xp, S::pX + 3 * tri_frag(w, s <= w / 2 ? s : 0), at16, fx[s]);
+        for (int s = 0; s < TW / 2; ++s) load_frag<NP>(kq, (S::fK + t * S::KS + w * (TW / 2) + s) * NP, at16, fk[t][s]);
     };
+    auto load_x = [&]() {   // (rows of the upper half have no second inner step: theirs stays zero)
+#pragma unroll
+      for (int s = 0; s < S::CS; ++s)
+        if (s <= w / 2) load_frag<3>(xp, S::pX + 3 * tri_frag(w, s), at16, fx[s]);
+    };
+#pragma unroll
+    for (int s = 0; s < S::CS; ++s)
+#pragma unroll
+      for (int i = 0; i < 3; ++i) fx[s][i] = bf16x8{};
     auto load_t = [&]() {
       if (!holds) return;
 #pragma unroll
@@ -333,22 +341,31 @@ __global__ __launch_bounds__(8 * C, 2) void k_delta_scan(DeltaArgs a) {
     };
     auto load_vec = [&]() {
       const float* p = reinterpret_cast<const float*>(vec);
-      into = *reinterpret_cast<const f32x4*>(p + row0);
-      left = *reinterpret_cast<const f32x4*>(p + 64 + row0);
-      beta = *reinterpret_cast<const f32x4*>(p + 128 + row0);
-      all = p[192];
-      bad0 = p[193];
+      fnext.into = *reinterpret_cast<const f32x4*>(p + row0);
+      fnext.left = *reinterpret_cast<const f32x4*>(p + 64 + row0);
+      fnext.beta = *reinterpret_cast<const f32x4*>(p + 128 + row0);
+      fnext.all = p[192];
+      fnext.bad = p[193];
     };
+    // S as planes for Q S, and this wave's share of K S
     auto put_state = [&]() {
       if (!holds) return;
 #pragma unroll
       for (int i = 0; i < NC; ++i) {
-        if constexpr (TW >= 2) {
+        f32x4 ks[S::RT];
 #pragma unroll
-          for (int t = 0; t < TW; t += 2) put_whole<3>(part(i, Sc::bS), (w * TW + t) / 2, lane, cat8(st[i][t], st[i][t + 1]));
-        } else {
-          put_half<3>(part(i, Sc::bS), w / 2, w & 1, lane, st[i][0]);
+        for (int t = 0; t < S::RT; ++t) ks[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < TW / 2; ++s) {
+          bf16x8 sp[3];
+          planes8<3>(cat8(st[i][2 * s], st[i][2 * s + 1]), sp);
+          mfma_rows<NP, 3, 3, S::RT>([&](int t) -> const bf16x8(&)[NP] { return fk[t][s]; }, sp, ks);
+#pragma unroll
+          for (int j = 0; j < NO; ++j)
+            *reinterpret_cast<bf16x8*>(part(i, Sc::bS) + ((w * (TW / 2) + s) * NO + j) * 1024 + at16) = sp[j];
         }
+#pragma unroll
+        for (int t = 0; t < S::RT; ++t) *reinterpret_cast<f32x4*>(part(i, Sc::bK) + (t * HW + w) * 1024 + at16) = ks[t];
       }
     };
     if (nc > 0) {
@@ -362,32 +379,28 @@ __global__ __launch_bounds__(8 * C, 2) void k_delta_scan(DeltaArgs a) {
     for (int ci = 0; ci < nc; ++ci) {
       const bool more = ci + 1 < nc;   // behind the last chunk its own values are loaded again, and not used
       const int64_t ch = (c0 + ci) * a.Hv + h;
-      lds_barrier();   // S is in LDS
-      // K S, the inner steps in two chains
-      f32x4 ks[NC], ks2[NC];
+      lds_barrier();
+      f32x4 ks[NC];
 #pragma unroll
-      for (int i = 0; i < NC; ++i) ks[i] = ks2[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int i = 0; i < NC; ++i) {
+        ks[i] = *reinterpret_cast<const f32x4*>(part(i, Sc::bK) + w * HW * 1024 + at16);
 #pragma unroll
-      for (int s = 0; s < S::KS; ++s)
-#pragma unroll
-        for (int i = 0; i < NC; ++i) {
-          bf16x8 sp[3];
-          get_operand<3>(part(i, Sc::bS), s, lane, sp);
-          f32x4& k = s & 1 ? ks2[i] : ks[i];
-          k = mfma_planes<NP, 3, 3>(fk[s], sp, k);
-        }
-      if (more) kq += kq_step;
-      load_k();
+        for (int j = 1; j < HW; ++j) ks[i] += *reinterpret_cast<const f32x4*>(part(i, Sc::bK) + (w * HW + j) * 1024 + at16);
+      }
+      f = fnext;
+      if (more) vec += vec_step;
+      load_vec();
       // beta (v - exp(G_i) K S)
       int bad[NC];
       float odd = 0.f;
 #pragma unroll
       for (int i = 0; i < NC; ++i) {
-        ks[i] = beta * (v[i].get(in[i], row0) - into * (ks[i] + ks2[i]));
+        ks[i] = f.beta * (v[i].get(in[i], row0) - f.into * ks[i]);
         odd += zero_if_finite(ks[i]);
-        bad[i] = (int)bad0;
+        bad[i] = (int)f.bad;
       }
       if (__ballot(odd != 0.f)) {
+        rare_path();
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
 #pragma unroll
@@ -405,6 +418,8 @@ __global__ __launch_bounds__(8 * C, 2) void k_delta_scan(DeltaArgs a) {
         put_half<3>(part(i, Sc::bR), w / 2, w & 1, lane, ks[i]);
         if (g == 0) bads[(i * 16 + x) * S::RT + w] = bad[i];
       }
+      if (more) kq += kq_step;
+      load_k();
       load_v(more ? ci + 1 : ci);
       if (SAVE && holds) {
         float* s0 = a.s0 + ch * (int64_t)KP * a.VP + col0;
@@ -421,35 +436,20 @@ __global__ __launch_bounds__(8 * C, 2) void k_delta_scan(DeltaArgs a) {
       f32x4 u[NC];
 #pragma unroll
       for (int i = 0; i < NC; ++i) {
-        f32x4 u2 = {0.f, 0.f, 0.f, 0.f};
-        u[i] = u2;
-        bf16x8 rp[3];
-        get_operand<3>(part(i, Sc::bR), 0, lane, rp);
-        u[i] = mfma_planes<3, 3, 3>(fx[0], rp, u[i]);
-        if (S::CS > 1 && w >= 2) {
-          get_operand<3>(part(i, Sc::bR), S::CS - 1, lane, rp);
-          u2 = mfma_planes<3, 3, 3>(fx[S::CS - 1], rp, u2);
-        }
-        u[i] += u2;
-        put_half<3>(part(i, Sc::bL), w / 2, w & 1, lane, left * u[i]);
+        u[i] = product<3, 3, 3, S::CS>(fx, [&](int s, bf16x8(&b)[3]) { get_operand<3>(part(i, Sc::bR), s, lane, b); });
+        put_half<3>(part(i, Sc::bL), w / 2, w & 1, lane, f.left * u[i]);
         put_half<NO>(part(i, Sc::bU), w / 2, w & 1, lane, u[i]);
         bad[i] = first_bad(i);
       }
       if (more) xp += xp_step;
       load_x();
-      const float all_now = all;
-      if (more) vec += vec_step;
-      load_vec();
       lds_barrier();
       // S <- exp(G) S + K^T (exp(G - G_i) u)
-      bool any_bad = false;
-#pragma unroll
-      for (int i = 0; i < NC; ++i) any_bad |= bad[i] < C;
       if (holds) {
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
 #pragma unroll
-          for (int t = 0; t < TW; ++t) st[i][t] *= all_now;
+          for (int t = 0; t < TW; ++t) st[i][t] *= bad[i] < C ? nan : f.all;   // a column that is no longer finite
 #pragma unroll
           for (int s = 0; s < S::CS; ++s) {
             bf16x8 up[3];
@@ -457,17 +457,6 @@ __global__ __launch_bounds__(8 * C, 2) void k_delta_scan(DeltaArgs a) {
 #pragma unroll
             for (int t = 0; t < TW; ++t) st[i][t] = mfma_planes<NP, 3, 3>(ft[t][s], up, st[i][t]);
           }
-        }
-      }
-      if (__ballot(any_bad)) {   // what is not finite: NaN from its row on
-#pragma unroll
-        for (int i = 0; i < NC; ++i) {
-#pragma unroll
-          for (int t = 0; t < TW; ++t)
-            if (bad[i] < C) st[i][t] = f32x4{nan, nan, nan, nan};
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (row0 + r >= bad[i]) u[i][r] = nan;
         }
       }
       put_state();
@@ -478,7 +467,7 @@ __global__ __launch_bounds__(8 * C, 2) void k_delta_scan(DeltaArgs a) {
         for (int i = 0; i < NC; ++i)
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            if (col0 + 16 * i < a.VP) us[r * a.VP + 16 * i] = u[i][r];
+            if (col0 + 16 * i < a.VP) us[r * a.VP + 16 * i] = row0 + r >= bad[i] ? nan : u[i][r];
       }
     }
     if (holds) {
@@ -507,55 +496,23 @@ __global__ __launch_bounds__(8 * C, 2) void k_delta_scan(DeltaArgs a) {
     };
     auto load_p = [&]() {
 #pragma unroll
-      for (int s = 0; s < S::CS; ++s) load_frag<NO>(xp, S::pP + S::NPP * tri_frag(w, s <= w / 2 ? s : 0), at16, fp[s]);
+      for (int s = 0; s < S::CS; ++s)
+        if (s <= w / 2) load_frag<NO>(xp, S::pP + S::NPP * tri_frag(w, s), at16, fp[s]);
     };
-    if (nc > 0) {
-      load_q();
-      load_p();
-    }
-    for (int ci = 0; ci < nc; ++ci) {
-      const bool more = ci + 1 < nc;
+#pragma unroll
+    for (int s = 0; s < S::CS; ++s)
+#pragma unroll
+      for (int i = 0; i < NO; ++i) fp[s][i] = bf16x8{};
+    f32x4 o[NC];
+    int bad[NC];
+    // o of chunk ci, of which only P u is missing
+    auto finish = [&](int ci) {
       const int rows = (int)(len - (int64_t)ci * C < C ? len - (int64_t)ci * C : C);
-      lds_barrier();
-      f32x4 o[NC], o2[NC];
-#pragma unroll
-      for (int i = 0; i < NC; ++i) o[i] = o2[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int s = 0; s < S::KS; ++s)
-#pragma unroll
-        for (int i = 0; i < NC; ++i) {
-          bf16x8 so[NO];
-          get_operand<3, NO>(part(i, Sc::bS), s, lane, so);
-          f32x4& q = s & 1 ? o2[i] : o[i];
-          q = mfma_planes<NP, NO, NO>(fq[s], so, q);
-        }
-#pragma unroll
-      for (int i = 0; i < NC; ++i) o[i] = (a.scale * into) * (o[i] + o2[i]);
-      if (more) kq += kq_step, vec += vec_step;
-      load_q();
-      lds_barrier();
-      lds_barrier();
-      int bad[NC];
 #pragma unroll
       for (int i = 0; i < NC; ++i) {
-        bf16x8 up[NO];
-        get_operand<NO>(part(i, Sc::bU), 0, lane, up);
-        o[i] = mfma_planes<NO, NO, NO>(fp[0], up, o[i]);
-        if (S::CS > 1 && w >= 2) {
-          get_operand<NO>(part(i, Sc::bU), S::CS - 1, lane, up);
-          o[i] = mfma_planes<NO, NO, NO>(fp[S::CS - 1], up, o[i]);
-        }
-        bad[i] = first_bad(i);
-      }
-      if (more) xp += xp_step;
-      load_p();
+        o[i] += product<NO, NO, NO, S::CS>(fp, [&](int s, bf16x8(&b)[NO]) { get_operand<NO>(part(i, Sc::bU), s, lane, b); });
 #pragma unroll
-      for (int i = 0; i < NC; ++i) {
-        if (__ballot(bad[i] < C)) {
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (row0 + r >= bad[i]) o[i][r] = nan;
-        }
+        for (int r = 0; r < 4; ++r) o[i][r] = row0 + r >= bad[i] ? nan : o[i][r];
         if (rows == C) {
 #pragma unroll
           for (int r = 0; r < 4; ++r)
@@ -567,7 +524,25 @@ __global__ __launch_bounds__(8 * C, 2) void k_delta_scan(DeltaArgs a) {
         }
         op[i] += C * orow;
       }
+    };
+    if (nc > 0) load_q();
+    for (int ci = 0; ci < nc; ++ci) {
+      lds_barrier();
+      if (ci > 0) finish(ci - 1);
+      load_p();
+      lds_barrier();
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+        o[i] = product<NP, NO, NO, S::KS>(fq, [&](int s, bf16x8(&b)[NO]) { get_operand<NO>(part(i, Sc::bS), s, lane, b); });
+#pragma unroll
+      for (int i = 0; i < NC; ++i) o[i] *= a.scale * into;
+      if (ci + 1 < nc) kq += kq_step, vec += vec_step, xp += xp_step;
+      load_q();
+      lds_barrier();
+#pragma unroll
+      for (int i = 0; i < NC; ++i) bad[i] = first_bad(i);
     }
+    if (nc > 0) finish(nc - 1);
   }
 }
 
@@ -588,8 +563,8 @@ hipError_t scan(const DeltaArgs& a, hipStream_t s) {
   using Sc = Scan<DT, KP, C, NC, SAVE>;
   const hipError_t e = allow_lds(k_delta_scan<DT, KP, C, NC, SAVE>, Sc::bytes);
   if (e != hipSuccess) return e;
-  const int64_t groups = (a.VP / 16 + NC - 1) / NC, heads = (a.rows.N * a.Hv + 7) / 8 * 8;
-  k_delta_scan<DT, KP, C, NC, SAVE><<<(unsigned)(heads * groups), 8 * C, Sc::bytes, s>>>(a);
+  const int groups = (a.VP / 16 + NC - 1) / NC;
+  k_delta_scan<DT, KP, C, NC, SAVE><<<column_blocks(a, groups), 8 * C, Sc::bytes, s>>>(a);
   return hipGetLastError();
 }
 

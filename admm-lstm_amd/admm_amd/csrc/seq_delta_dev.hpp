@@ -52,6 +52,38 @@ __device__ __forceinline__ double running_sum(float v, int lane, double& last) {
 
 // ---- fragments in the work memory and operands B in LDS
 
+// keeps a branch around what hardly ever runs (the compiler would rather run both sides and select)
+__device__ __forceinline__ void rare_path() { asm volatile(""); }
+
+// sum over S inner steps of a[s] b(s), a step's plane pairs and the steps in several chains: a matrix instruction that takes the
+// result of the last one waits for all of it
+template <int NA, int NB, int L, int S, class B>
+__device__ __forceinline__ f32x4 product(const bf16x8 (&a)[S][NA], const B& load) {
+  constexpr int kChains = S >= 4 ? 4 : S == 2 ? 4 : 2;
+  f32x4 acc[kChains];
+#pragma unroll
+  for (int c = 0; c < kChains; ++c) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+  bf16x8 b[S][NB];
+#pragma unroll
+  for (int s = 0; s < S; ++s) load(s, b[s]);
+  int n[S] = {};
+#pragma unroll
+  for (int q = L - 1; q >= 0; --q)
+#pragma unroll
+    for (int i = 0; i < NA; ++i)
+      if (q - i >= 0 && q - i < NB) {
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+          const int c = S >= 4 ? s % 4 : S == 2 ? 2 * s + (n[s] & 1) : n[s] & 1;
+          acc[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[s][i], b[s][q - i], acc[c], 0, 0, 0);
+          ++n[s];
+        }
+      }
+  f32x4 sum = acc[0] + acc[1];
+  if (kChains == 4) sum += acc[2 % kChains] + acc[3 % kChains];
+  return sum;
+}
+
 // a value that is the same in all lanes, as a scalar (addresses made of it need no vector arithmetic)
 __device__ __forceinline__ int64_t uniform(int64_t v) {
   return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v) |
@@ -105,7 +137,7 @@ struct ColumnRows {
 #pragma unroll
       for (int r = 0; r < 4; ++r) raw[r] = p[at[r]];
     } else {
-      asm volatile("");   // a branch: the products below are not worth forming for every chunk
+      rare_path();
 #pragma unroll
       for (int r = 0; r < 4; ++r) raw[r] = p[(row0 + r < rows ? row0 + r : rows - 1) * stride];
     }
@@ -133,12 +165,22 @@ __device__ __forceinline__ f32x4 load_state(const float* p, int K, int V, int co
   return st;
 }
 
-// the column tiles of this workgroup: workgroups are dealt out to the eight XCDs in turn, and those of one head (which read the
-// same fragments) go to one XCD's L2.  false: none
-__device__ __forceinline__ bool place_columns(int64_t heads, int groups, int64_t& head, int& group) {
-  head = (int64_t)(blockIdx.x / 8 / groups) * 8 + blockIdx.x % 8;
-  group = (int)(blockIdx.x / 8 % groups);
-  return head < heads;
+// The value head and column tiles of this workgroup.  Workgroups are dealt out to the eight XCDs in turn: those of one sequence
+// and query/key head, which read the same fragments, go to one XCD's L2.  false: none
+__device__ __forceinline__ bool place_columns(const DeltaArgs& a, int groups, int64_t& n, int& h, int& hk, int& group) {
+  const int share = a.Hv / a.Hk, per = share * groups;   // workgroups of a query/key head
+  const int64_t unit = (int64_t)(blockIdx.x / 8 / per) * 8 + blockIdx.x % 8;
+  if (unit >= a.rows.N * a.Hk) return false;
+  const int at = (int)(blockIdx.x / 8 % per);
+  n = unit / a.Hk;
+  hk = (int)(unit % a.Hk);
+  h = hk * share + at % share;
+  group = at / share;
+  return true;
+}
+// workgroups for that
+inline unsigned column_blocks(const DeltaArgs& a, int groups) {
+  return (unsigned)((a.rows.N * a.Hk + 7) / 8 * 8 * (a.Hv / a.Hk) * groups);
 }
 
 template <class F>

@@ -37,11 +37,10 @@ __global__ __launch_bounds__(4 * C) void k_delta_back(DeltaGradArgs ga) {
   const DeltaArgs& a = ga.f;
   const int lane = threadIdx.x & 63, w = wave_id(), x = lane & 15, g = lane >> 4;
   const int groups = (a.VP / 16 + NC - 1) / NC;
-  int64_t head;
-  int group;
-  if (!place_columns(a.rows.N * a.Hv, groups, head, group)) return;
-  const int64_t n = head / a.Hv;
-  const int h = (int)(head % a.Hv), hk = h / (a.Hv / a.Hk);
+  int64_t n;
+  int h, hk, group;
+  if (!place_columns(a, groups, n, h, hk, group)) return;
+  const int64_t head = n * a.Hv + h;
   const int col0 = group * NC * 16 + x;
   int64_t begin, len, c0;
   a.rows.range(n, begin, len, c0);
@@ -608,8 +607,8 @@ hipError_t back(const DeltaGradArgs& ga, hipStream_t s) {
   const DeltaArgs& a = ga.f;
   const hipError_t e = allow_lds(k_delta_back<DT, KP, C, NC>, bytes);
   if (e != hipSuccess) return e;
-  const int64_t groups = (a.VP / 16 + NC - 1) / NC, heads = (a.rows.N * a.Hv + 7) / 8 * 8;
-  k_delta_back<DT, KP, C, NC><<<(unsigned)(heads * groups), 4 * C, bytes, s>>>(ga);
+  const int groups = (a.VP / 16 + NC - 1) / NC;
+  k_delta_back<DT, KP, C, NC><<<column_blocks(a, groups), 4 * C, bytes, s>>>(ga);
   return hipGetLastError();
 }
 

@@ -75,6 +75,27 @@ __device__ __forceinline__ f32x4 mfma_planes(const bf16x8 (&a)[NA], const bf16x8
   return acc;
 }
 
+// acc[t] += a(t) b for R row tiles: plane pairs outside, rows inside, so that neighbouring instructions do not wait for each other
+template <int NA, int NB, int L, int R, class A>
+__device__ __forceinline__ void mfma_rows(const A& a, const bf16x8 (&b)[NB], f32x4 (&acc)[R]) {
+#pragma unroll
+  for (int s = L - 1; s >= 0; --s)
+#pragma unroll
+    for (int i = 0; i < NA; ++i)
+      if (s - i >= 0 && s - i < NB) {
+#pragma unroll
+        for (int t = 0; t < R; ++t) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a(t)[i], b[s - i], acc[t], 0, 0, 0);
+      }
+}
+
+// Between matrix instructions and control flow behind which their results are read first.  The wait states that such a read needs
+// are the compiler's to insert, and where two ways of different length lead to it, it has left them out on the shorter one.
+__device__ __forceinline__ void mfma_settle() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_nop 15\n\ts_nop 3");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
 // 16 bytes a lane from global memory straight into LDS: `lds` is the wave's base, lane l's bytes land at lds + 16 l.
 // The caller waits for them (vm_wait) before the barrier that hands them to other waves, and keeps other buffers' readers out by
 // barriers too.  In assembly (m0: the LDS base; there is no result register) because the compiler, which cannot tell the

@@ -136,6 +136,7 @@ struct Gemm {
         }
       }
     }
+    mfma_settle();   // the callers store behind bounds checks
   }
 };
 

@@ -94,7 +94,7 @@ int delta_sizes(const SeqDelta* d, bool saved, DeltaSizes& z) {
   z.VP = (d->V + 15) / 16 * 16;
   z.wide_cols = d->sequences * d->Hv * (z.VP / 16) > 512;
   z.chunks = d->offsets ? (d->sequences && d->T ? d->T / z.C + d->sequences + 1 : 0) : z.per * d->batch;
-  if (z.chunks > kMaxBlocks / d->Hv || (d->sequences + 8) > kMaxBlocks / (d->Hv * (z.VP / 16)))
+  if (z.chunks > kMaxBlocks / d->Hv || (d->sequences + 8) > kMaxBlocks / ((int64_t)d->Hv * (z.VP / 16) * 8))
     return fail(SEQ_EINVAL, "too many sequences, rows or heads for one launch");
   // sizes of DeltaShape: K, Q, K^T (saved: Q^T), each z.C x KP planes; X, P (saved: their transposes) as fragments
   z.kq = up256(z.chunks * d->Hk * ((saved ? 4LL : 3LL) * NP * z.C * z.KP * 2));
