@@ -18,24 +18,28 @@
 namespace seq {
 namespace {
 
-// Waves and LDS as in k_delta_scan: wave w forms rows perm_row(w, .) of du and dR and keeps TW tiles of dS.
+// As in k_delta_scan, HW of C / 16 waves keep TW tiles of dS each and form their share of K dS, and wave w takes rows
+// perm_row(w, .) of du and dR.  As many more waves form what does not depend on dS, P^T do and scale Q^T (exp(G_i) do), one
+// chunk ahead.
 template <int DT, int KP, int C, int NC>
 struct Back {
   using S = DeltaShape<DT, KP, C, true>;
-  static constexpr int TW = S::KT >= S::RT ? S::KT / S::RT : 1;
-  static constexpr int bS = 0, bO = S::KS * 3, bE = bO + S::CS * S::NP, bU = bE + S::CS * 3, bR = bU + S::CS * 3, bEnd = bR + S::CS * 3;
+  static constexpr int TW = S::KT >= 2 * S::RT ? S::KT / S::RT : 2, HW = S::KT / TW;
+  // shares of K dS; do, and scale exp(G_i) do, as operands; du; exp(G_i) beta dR; P^T do; scale Q^T (exp(G_i) do), twice   (KB)
+  static constexpr int bK = 0, bO = HW * S::RT, bE = bO + S::CS * S::NP, bU = bE + S::CS * 3, bR = bU + S::CS * 3,
+                       bP = bR + S::CS * 3, bQ = bP + S::RT, bEnd = bQ + 2 * S::KT;
   static constexpr int bytes = NC * bEnd * 1024;
 };
 
 template <int DT, int KP, int C, int NC>
-__global__ __launch_bounds__(4 * C) void k_delta_back(DeltaGradArgs ga) {
+__global__ __launch_bounds__(8 * C, 2) void k_delta_back(DeltaGradArgs ga) {
   using S = DeltaShape<DT, KP, C, true>;
   using B = Back<DT, KP, C, NC>;
   using T = typename Elem<DT>::T;
-  constexpr int NP = S::NP, TW = B::TW;
+  constexpr int NP = S::NP, TW = B::TW, HW = B::HW;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const DeltaArgs& a = ga.f;
-  const int lane = threadIdx.x & 63, w = wave_id(), x = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = wave_id(), w = wave % S::RT, x = lane & 15, g = lane >> 4;
   const int groups = (a.VP / 16 + NC - 1) / NC;
   int64_t n;
   int h, hk, group;
@@ -44,211 +48,235 @@ __global__ __launch_bounds__(4 * C) void k_delta_back(DeltaGradArgs ga) {
   const int col0 = group * NC * 16 + x;
   int64_t begin, len, c0;
   a.rows.range(n, begin, len, c0);
-  const int64_t nc = (len + C - 1) / C;
-  const bool holds = w * TW < S::KT;
+  begin = uniform(begin), len = uniform(len), c0 = uniform(c0);
+  const int nc = (int)((len + C - 1) / C);
   const int row0 = perm_row(w, 4 * g);
-
-  f32x4 ds[NC][TW];
-#pragma unroll
-  for (int i = 0; i < NC; ++i)
-#pragma unroll
-    for (int t = 0; t < TW; ++t)
-      ds[i][t] = load_state(ga.d_final && holds ? ga.d_final + head * a.K * a.V : nullptr, a.K, a.V, col0 + 16 * i, w * TW + t, g);
+  const uint32_t at16 = lane * 16;
 
   const int64_t last = c0 + (nc > 0 ? nc - 1 : 0);
   const char* kq = a.kq + (last * a.Hk + hk) * (int64_t)S::kKQ;
   const char* xp = a.xp + (last * a.Hv + h) * (int64_t)S::kXP;
-  const float* vec = reinterpret_cast<const float*>(a.vec + (last * a.Hv + h) * (int64_t)kVec);
-  const int64_t kq_step = (int64_t)a.Hk * S::kKQ, xp_step = (int64_t)a.Hv * S::kXP, vec_step = (int64_t)a.Hv * (kVec / 4);
+  const char* vec = a.vec + (last * a.Hv + h) * (int64_t)kVec;
+  const int64_t kq_step = (int64_t)a.Hk * S::kKQ, xp_step = (int64_t)a.Hv * S::kXP, vec_step = (int64_t)a.Hv * kVec;
   const int64_t orow = (int64_t)a.Hv * a.V, first = ((a.rows.batch(n) * a.rows.T + begin) * a.Hv + h) * (int64_t)a.V;
-  const T* dop[NC];
-  T* dvp[NC];
   bool in[NC];
 #pragma unroll
-  for (int i = 0; i < NC; ++i) {
-    const int col = col0 + 16 * i;
-    in[i] = col < a.V;
-    dop[i] = static_cast<const T*>(ga.d_o) + first + (in[i] ? col : a.V - 1);
-    dvp[i] = static_cast<T*>(ga.dv) + first + col;
-  }
-
-  bf16x8 fk[S::KS][NP], fx[S::CS][3], fp[S::CS][3], fq[TW][S::CS][NP], ft[TW][S::CS][NP];
-  f32x4 into, left, beta;
-  float all = 0.f;
-  ColumnRows<T, C> d[NC];
-  int64_t drow[4];
+  for (int i = 0; i < NC; ++i) in[i] = col0 + 16 * i < a.V;
+  auto part = [&](int i, int b) { return lds + (i * B::bEnd + b) * 1024; };
+  // fragment of the transposed triangular matrices; below the diagonal there is none
+  auto tri_t = [&](int s) { return C == 32 ? w : tri_frag_t(w, s); };
+  bf16x8 ft[TW][S::CS][NP], fx[S::CS][3];   // K^T and X^T, or Q^T and P^T
 #pragma unroll
-  for (int r = 0; r < 4; ++r) drow[r] = (row0 + r) * orow;
-  auto tri_t = [&](int s) { return C == 32 ? w : tri_frag_t(w, s < w / 2 ? w / 2 : s); };   // below the diagonal: loaded, not used
-  auto load_k = [&](const char* p) {
+  for (int s = 0; s < S::CS; ++s)
 #pragma unroll
-    for (int s = 0; s < S::KS; ++s) load_frag<NP>(p, (S::fK + w * S::KS + s) * NP, lane * 16, fk[s]);
-  };
-  auto load_p = [&](const char* p) {
-#pragma unroll
-    for (int s = 0; s < S::CS; ++s) load_frag<3>(p, S::pPT + 3 * tri_t(s), lane * 16, fp[s]);
-  };
-  auto load_x = [&](const char* p) {
-#pragma unroll
-    for (int s = 0; s < S::CS; ++s) load_frag<3>(p, S::pXT + 3 * tri_t(s), lane * 16, fx[s]);
-  };
-  auto load_t = [&](const char* p) {
-    if (!holds) return;
+    for (int i = 0; i < 3; ++i) fx[s][i] = bf16x8{};
+  auto load_t = [&](int f) {
 #pragma unroll
     for (int t = 0; t < TW; ++t)
 #pragma unroll
-      for (int s = 0; s < S::CS; ++s) {
-        load_frag<NP>(p, (S::fQT + (w * TW + t) * S::CS + s) * NP, lane * 16, fq[t][s]);
-        load_frag<NP>(p, (S::fKT + (w * TW + t) * S::CS + s) * NP, lane * 16, ft[t][s]);
+      for (int s = 0; s < S::CS; ++s) load_frag<NP>(kq, (f + (w * TW + t) * S::CS + s) * NP, at16, ft[t][s]);
+  };
+  auto load_x = [&](int p) {
+#pragma unroll
+    for (int s = 0; s < S::CS; ++s)
+      if (s >= w / 2) load_frag<3>(xp, p + 3 * tri_t(s), at16, fx[s]);
+  };
+
+  const bool holds = w < HW;
+  if (wave < S::RT) {   // ---- dS
+    f32x4 ds[NC][TW];
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+#pragma unroll
+      for (int t = 0; t < TW; ++t)
+        ds[i][t] = load_state(ga.d_final && holds ? ga.d_final + head * a.K * a.V : nullptr, a.K, a.V, col0 + 16 * i, w * TW + t, g);
+    T* dvp[NC];
+#pragma unroll
+    for (int i = 0; i < NC; ++i) dvp[i] = static_cast<T*>(ga.dv) + first + col0 + 16 * i + row0 * orow;
+    bf16x8 fk[S::RT][TW / 2][NP];
+    struct { f32x4 into, left, beta; float all; } f, fnext;
+    auto load_k = [&]() {
+      if (!holds) return;
+#pragma unroll
+      for (int t = 0; t < S::RT; ++t)
+#pragma unroll
+        for (int s = 0; s < TW / 2; ++s) load_frag<NP>(kq, (S::fK + t * S::KS + w * (TW / 2) + s) * NP, at16, fk[t][s]);
+    };
+    auto load_vec = [&]() {
+      const float* p = reinterpret_cast<const float*>(vec);
+      fnext.into = *reinterpret_cast<const f32x4*>(p + row0);
+      fnext.left = *reinterpret_cast<const f32x4*>(p + 64 + row0);
+      fnext.beta = *reinterpret_cast<const f32x4*>(p + 128 + row0);
+      fnext.all = p[192];
+    };
+    auto put_share = [&]() {
+      if (!holds) return;
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        f32x4 ks[S::RT];
+#pragma unroll
+        for (int t = 0; t < S::RT; ++t) ks[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < TW / 2; ++s) {
+          bf16x8 sp[3];
+          planes8<3>(cat8(ds[i][2 * s], ds[i][2 * s + 1]), sp);
+          mfma_rows<NP, 3, 3, S::RT>([&](int t) -> const bf16x8(&)[NP] { return fk[t][s]; }, sp, ks);
+        }
+#pragma unroll
+        for (int t = 0; t < S::RT; ++t) *reinterpret_cast<f32x4*>(part(i, B::bK) + (t * HW + w) * 1024 + at16) = ks[t];
       }
-  };
-  auto load_do = [&](int64_t ci) {
-    const int rows = (int)(len - ci * C < C ? len - ci * C : C);
+    };
+    if (nc > 0) {
+      load_k();
+      load_vec();
+      load_x(S::pXT);
+      if (holds) load_t(S::fKT);
+      put_share();
+      lds_barrier();   // (the other waves exchange the last chunk's do)
+      lds_barrier();
+    }
+    for (int ci = nc - 1; ci >= 0; --ci) {
+      const bool more = ci > 0;
+      const int64_t ch = (c0 + ci) * a.Hv + h;
+      const int rows = (int)(len - (int64_t)ci * C < C ? len - (int64_t)ci * C : C);
+      lds_barrier();
+      // du = exp(G - G_i) K dS + P^T do
+      f = fnext;
+      if (more) vec -= vec_step;
+      load_vec();
 #pragma unroll
-    for (int i = 0; i < NC; ++i) d[i].load(dop[i] + ci * C * orow, drow, orow, rows, row0);
-  };
-  auto load_vec = [&](const float* p) {
-    into = *reinterpret_cast<const f32x4*>(p + row0);
-    left = *reinterpret_cast<const f32x4*>(p + 64 + row0);
-    beta = *reinterpret_cast<const f32x4*>(p + 128 + row0);
-    all = p[192];
-  };
-  auto part = [&](int i, int b) { return lds + (i * B::bEnd + b) * 1024; };
-  auto put_state = [&]() {
-    if (!holds) return;
+      for (int i = 0; i < NC; ++i) {
+        f32x4 k = *reinterpret_cast<const f32x4*>(part(i, B::bK) + w * HW * 1024 + at16);
 #pragma unroll
-    for (int i = 0; i < NC; ++i) {
-      if constexpr (TW >= 2) {
+        for (int j = 1; j < HW; ++j) k += *reinterpret_cast<const f32x4*>(part(i, B::bK) + (w * HW + j) * 1024 + at16);
+        put_half<3>(part(i, B::bU), w / 2, w & 1, lane, f.left * k + *reinterpret_cast<const f32x4*>(part(i, B::bP) + w * 1024 + at16));
+      }
+      if (more) kq -= kq_step;
+      load_k();
+      if (holds) {
+        float* p = ga.ds + ch * (int64_t)KP * a.VP + col0;
 #pragma unroll
-        for (int t = 0; t < TW; t += 2) put_whole<3>(part(i, B::bS), (w * TW + t) / 2, lane, cat8(ds[i][t], ds[i][t + 1]));
-      } else {
-        put_half<3>(part(i, B::bS), w / 2, w & 1, lane, ds[i][0]);
+        for (int i = 0; i < NC; ++i)
+#pragma unroll
+          for (int t = 0; t < TW; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (col0 + 16 * i < a.VP) p[perm_row(w * TW + t, 4 * g + r) * a.VP + 16 * i] = ds[i][t][r];
+      }
+      lds_barrier();
+      // dR = X^T du
+      f32x4 dr[NC];
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        dr[i] = product<3, 3, 3, S::CS>(fx, [&](int s, bf16x8(&b)[3]) { get_operand<3>(part(i, B::bU), s, lane, b); });
+        put_half<3>(part(i, B::bR), w / 2, w & 1, lane, -f.into * (f.beta * dr[i]));
+      }
+      if (more) xp -= xp_step;
+      load_x(S::pXT);
+      lds_barrier();
+      // dS <- exp(G) dS + scale Q^T (exp(G_i) do) - K^T (exp(G_i) beta dR)
+      if (holds) {
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+          const char* q = part(i, B::bQ) + (ci & 1) * S::KT * 1024;
+#pragma unroll
+          for (int t = 0; t < TW; ++t) ds[i][t] = f.all * ds[i][t] + *reinterpret_cast<const f32x4*>(q + (w * TW + t) * 1024 + at16);
+#pragma unroll
+          for (int s = 0; s < S::CS; ++s) {
+            bf16x8 rp[3];
+            get_operand<3>(part(i, B::bR), s, lane, rp);
+            mfma_rows<NP, 3, 3, TW>([&](int t) -> const bf16x8(&)[NP] { return ft[t][s]; }, rp, ds[i]);
+          }
+        }
+      }
+      put_share();
+      if (holds) load_t(S::fKT);
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        float* p = ga.dr + (ch * C + row0) * (int64_t)a.VP + col0 + 16 * i;
+        T* dv = dvp[i] + (int64_t)ci * C * orow;
+        const f32x4 bd = f.beta * dr[i];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          if (col0 + 16 * i < a.VP) p[r * a.VP] = dr[i][r];
+          if (in[i] && row0 + r < rows) dv[r * orow] = (T)bd[r];
+        }
       }
     }
-  };
-  auto put_do = [&]() {
-#pragma unroll
-    for (int i = 0; i < NC; ++i) put_half<NP>(part(i, B::bO), w / 2, w & 1, lane, d[i].get(in[i], row0));
-  };
-  if (nc > 0) {
-    load_do(nc - 1);
-    load_k(kq);
-    load_vec(vec);
-    load_p(xp);
-    load_x(xp);
-    load_t(kq);
-    put_state();
-    put_do();
-  }
-  for (int64_t ci = nc - 1; ci >= 0; --ci) {
-    const bool more = ci > 0;
-    const int64_t ch = (c0 + ci) * a.Hv + h;
-    const int rows = (int)(len - ci * C < C ? len - ci * C : C);
-    f32x4 dc[NC];
-#pragma unroll
-    for (int i = 0; i < NC; ++i) dc[i] = d[i].get(in[i], row0);
-    lds_barrier();   // dS and do are in LDS
-    if (holds) {
-      float* p = ga.ds + ch * (int64_t)KP * a.VP + col0;
+    if (ga.d_initial && holds) {
 #pragma unroll
       for (int i = 0; i < NC; ++i)
 #pragma unroll
         for (int t = 0; t < TW; ++t)
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (col0 + 16 * i < a.VP) p[(int64_t)perm_row(w * TW + t, 4 * g + r) * a.VP + 16 * i] = ds[i][t][r];
-    }
-    // du = exp(G - G_i) K dS + P^T do
-    f32x4 du[NC], du2[NC];
-#pragma unroll
-    for (int i = 0; i < NC; ++i) du[i] = du2[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int s = 0; s < S::KS; ++s)
-#pragma unroll
-      for (int i = 0; i < NC; ++i) {
-        bf16x8 sp[3];
-        get_operand<3>(part(i, B::bS), s, lane, sp);
-        f32x4& u = s & 1 ? du2[i] : du[i];
-        u = mfma_planes<NP, 3, 3>(fk[s], sp, u);
-      }
-#pragma unroll
-    for (int i = 0; i < NC; ++i) {
-      f32x4 p = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int s = 0; s < S::CS; ++s) {
-        if (s < w / 2) continue;
-        bf16x8 dp[NP];
-        get_operand<NP>(part(i, B::bO), s, lane, dp);
-        p = mfma_planes<3, NP, 3>(fp[s], dp, p);
-      }
-      du[i] = left * (du[i] + du2[i]) + p;
-      put_half<3>(part(i, B::bU), w / 2, w & 1, lane, du[i]);
-      put_half<3>(part(i, B::bE), w / 2, w & 1, lane, (a.scale * into) * dc[i]);
-    }
-    if (more) kq -= kq_step, xp -= xp_step;
-    load_k(kq);
-    load_p(xp);
-    load_do(more ? ci - 1 : ci);
-    lds_barrier();
-    // dR = X^T du
-#pragma unroll
-    for (int i = 0; i < NC; ++i) {
-      f32x4 dr = {0.f, 0.f, 0.f, 0.f}, dr2 = dr;
-#pragma unroll
-      for (int s = 0; s < S::CS; ++s) {
-        if (s < w / 2) continue;
-        bf16x8 dp[3];
-        get_operand<3>(part(i, B::bU), s, lane, dp);
-        f32x4& r = s & 1 ? dr2 : dr;
-        r = mfma_planes<3, 3, 3>(fx[s], dp, r);
-      }
-      dr += dr2;
-      const f32x4 dv = beta * dr;
-      put_half<3>(part(i, B::bR), w / 2, w & 1, lane, -into * dv);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        if (col0 + 16 * i < a.VP) ga.dr[(ch * C + row0 + r) * (int64_t)a.VP + col0 + 16 * i] = dr[r];
-        if (in[i] && row0 + r < rows) dvp[i][ci * C * orow + drow[r]] = (T)dv[r];
-      }
-    }
-    load_x(xp);
-    const float all_now = all;
-    if (more) vec -= vec_step;
-    load_vec(vec);
-    lds_barrier();
-    // dS <- exp(G) dS + scale Q^T (exp(G_i) do) - K^T (exp(G_i) beta dR)
-    if (holds) {
-#pragma unroll
-      for (int i = 0; i < NC; ++i) {
-#pragma unroll
-        for (int t = 0; t < TW; ++t) ds[i][t] *= all_now;
-#pragma unroll
-        for (int s = 0; s < S::CS; ++s) {
-          bf16x8 dp[3], rp[3];
-          get_operand<3>(part(i, B::bE), s, lane, dp);
-          get_operand<3>(part(i, B::bR), s, lane, rp);
-#pragma unroll
-          for (int t = 0; t < TW; ++t) {
-            ds[i][t] = mfma_planes<NP, 3, 3>(fq[t][s], dp, ds[i][t]);
-            ds[i][t] = mfma_planes<NP, 3, 3>(ft[t][s], rp, ds[i][t]);
+          for (int r = 0; r < 4; ++r) {
+            const int kd = perm_row(w * TW + t, 4 * g + r);
+            if (in[i] && kd < a.K) ga.d_initial[(head * a.K + kd) * a.V + col0 + 16 * i] = ds[i][t][r];
           }
+    }
+  } else {   // ---- what depends on do alone, of chunk ci while the others are at ci + 1
+    const T* dop[NC];
+#pragma unroll
+    for (int i = 0; i < NC; ++i) dop[i] = static_cast<const T*>(ga.d_o) + first + (in[i] ? col0 + 16 * i : a.V - 1);
+    int64_t drow[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) drow[r] = (row0 + r) * orow;
+    ColumnRows<T, C> d[NC];
+    f32x4 into;
+    auto load_do = [&](int ci) {
+      const int64_t left_rows = len - (int64_t)ci * C;
+#pragma unroll
+      for (int i = 0; i < NC; ++i) d[i].load(dop[i] + (int64_t)ci * C * orow, drow, orow, (int)(left_rows < C ? left_rows : C), row0);
+      into = *reinterpret_cast<const f32x4*>(vec + row0 * 4);
+    };
+    if (nc > 0) {
+      load_do(nc - 1);
+      load_x(S::pPT);
+      if (holds) load_t(S::fQT);
+    }
+    // three barriers a chunk, as the others; before the first chunk and without the first one
+    for (int ci = nc - 1; ci >= 0; --ci) {
+      const bool more = ci > 0;
+      if (ci < nc - 1) lds_barrier();
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        const f32x4 v = d[i].get(in[i], row0);
+        put_half<NP>(part(i, B::bO), w / 2, w & 1, lane, v);
+        put_half<3>(part(i, B::bE), w / 2, w & 1, lane, (a.scale * into) * v);
+      }
+      if (more) kq -= kq_step, xp -= xp_step, vec -= vec_step;
+      load_do(more ? ci - 1 : ci);
+      lds_barrier();
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+        *reinterpret_cast<f32x4*>(part(i, B::bP) + w * 1024 + at16) =
+            product<3, NP, 3, S::CS>(fx, [&](int s, bf16x8(&b)[NP]) { get_operand<NP>(part(i, B::bO), s, lane, b); });
+      load_x(S::pPT);
+      lds_barrier();
+      if (holds) {
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+          f32x4 q[TW];
+#pragma unroll
+          for (int t = 0; t < TW; ++t) q[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int s = 0; s < S::CS; ++s) {
+            bf16x8 ep[3];
+            get_operand<3>(part(i, B::bE), s, lane, ep);
+            mfma_rows<NP, 3, 3, TW>([&](int t) -> const bf16x8(&)[NP] { return ft[t][s]; }, ep, q);
+          }
+#pragma unroll
+          for (int t = 0; t < TW; ++t)
+            *reinterpret_cast<f32x4*>(part(i, B::bQ) + ((ci & 1) * S::KT + w * TW + t) * 1024 + at16) = q[t];
         }
+        load_t(S::fQT);
       }
     }
-    load_t(kq);
-    put_state();
-    put_do();
-  }
-  if (ga.d_initial && holds) {
-#pragma unroll
-    for (int i = 0; i < NC; ++i)
-#pragma unroll
-      for (int t = 0; t < TW; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int kd = perm_row(w * TW + t, 4 * g + r);
-          if (in[i] && kd < a.K) ga.d_initial[(head * a.K + kd) * a.V + col0 + 16 * i] = ds[i][t][r];
-        }
+    if (nc > 0) {   // the others' last chunk
+      lds_barrier();
+      lds_barrier();
+      lds_barrier();
+    }
   }
 }
 
@@ -608,7 +636,7 @@ hipError_t back(const DeltaGradArgs& ga, hipStream_t s) {
   const hipError_t e = allow_lds(k_delta_back<DT, KP, C, NC>, bytes);
   if (e != hipSuccess) return e;
   const int groups = (a.VP / 16 + NC - 1) / NC;
-  k_delta_back<DT, KP, C, NC><<<column_blocks(a, groups), 4 * C, bytes, s>>>(ga);
+  k_delta_back<DT, KP, C, NC><<<column_blocks(a, groups), 8 * C, bytes, s>>>(ga);
   return hipGetLastError();
 }
 
