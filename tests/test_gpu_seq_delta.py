@@ -296,7 +296,9 @@ def test_captured_training_step(rule):
 
 # ------------------------------------------------------------------------------------------------ single tokens
 
-STEPS = [(1, 1, 1, 1, 1), (3, 2, 4, 32, 32), (2, 1, 3, 33, 30), (5, 2, 2, 64, 65), (4, 1, 2, 100, 36), (7, 2, 2, 128, 128)]
+# the last two: enough heads for whole rows of columns in a workgroup
+STEPS = [(1, 1, 1, 1, 1), (3, 2, 4, 32, 32), (2, 1, 3, 33, 30), (5, 2, 2, 64, 65), (4, 1, 2, 100, 36), (7, 2, 2, 128, 128),
+         (260, 2, 4, 9, 131), (130, 8, 8, 40, 100)]
 
 
 @pytest.mark.parametrize('dtype', [BF16, FP16, FP32])
@@ -309,6 +311,20 @@ def test_steps_follow_the_sequence(rule, shape, dtype):
     wo, wf = R.delta_rule(*(x.cpu() for x in (q, k, v, g, beta)), initial=s0.cpu())
     R.assert_close('state', state, wf, R.f32_atol(K + 128))
     R.assert_close('o', torch.stack(os, 1), wo, R.f32_atol(K + 128))
+
+
+@pytest.mark.parametrize('K', [30, 64, 128])
+def test_steps_of_many_states(rule, K):
+    """More states than the caches hold, which are passed by; the first and last streams are compared."""
+    B, H, V = 64 * 128 // K, 16, 260
+    q, k, v, g, beta, s0 = R.delta_inputs(B, 1, H, H, K, V, BF16, seed=31)
+    assert B * H * K * V > 32 << 20
+    state = s0.clone()
+    o = rule.gated_delta_step(q[:, 0], k[:, 0], v[:, 0], g[:, 0], beta[:, 0], state)
+    at = [0, 1, B // 2, B - 1]
+    wo, wf = R.delta_rule(*(x[at].cpu() for x in (q, k, v, g, beta)), initial=s0[at].cpu())
+    R.assert_close('state', state[at], wf, R.f32_atol(K + 128))
+    R.assert_close('o', o[at], wo[:, 0], R.f32_atol(K + 128))
 
 
 @pytest.mark.parametrize('wide', [torch.int32, torch.int64])
