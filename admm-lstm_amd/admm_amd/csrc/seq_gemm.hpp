@@ -39,35 +39,62 @@ __device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
 // INNER (inner axis contiguous): R rows of 8 pieces, piece c of row r at place c ^ (r & 7).
 // else: kBK rows of R / 8 pieces, piece c of row k at place c ^ spread(k): the four rows that a transposing read takes
 // together, and the next lanes' four, lie in different banks.
-template <int R, bool INNER>
+template <int R, bool INNER, int WAVES>
 struct TileOf {
   static constexpr int kBytes = R * kBK * 2;
-  static constexpr int kP = INNER ? kBK / 8 : R / 8;   // pieces of a row
+  static constexpr int kP = INNER ? kBK / 8 : R / 8;         // pieces of a row
+  static constexpr int kLoads = kBytes / 1024 / WAVES;       // of 1 KB, for each wave
   __device__ static int spread(int row) {
     if (INNER) return row & 7;
     return (((row & 3) << 1) | ((row >> 3 & 3) << 3)) & (kP - 1);
   }
-  // element offset of the fragment with outer rows 16 t + x, inner values 32 s + 8 g..+7
-  __device__ static bf16x8 frag(const __bf16* p, int t, int s, int g, int x) {
-    if (INNER) {
-      const int r = 16 * t + x;
-      return *reinterpret_cast<const bf16x8*>(p + r * kBK + 8 * ((4 * s + g) ^ spread(r)));
-    }
-    const int k = 32 * s + 8 * g + (x >> 2), c = 2 * t + ((x & 3) >> 1), h = 4 * (x & 1);
-    const bf16x4 u = tr4(p + k * R + 8 * (c ^ spread(k)) + h), v = tr4(p + (k + 4) * R + 8 * (c ^ spread(k + 4)) + h);
-    return __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7);
-  }
-  // Loads the tile whose first outer row is o0 and first inner value k0 of a matrix with `outer` and `inner` values: WAVES
-  // waves, 1 KB at a time.  Pieces outside come from g_zeros.
-  template <int WAVES>
-  __device__ static void load(const char* base, int64_t ld, int o0, int k0, int outer, int inner, char* lds, int wave, int lane) {
+  // Offsets of the lane's pieces from the tile's first value.  Outer values outside the matrix are taken from the last ones
+  // inside (what they make is not stored), so that only the last tile along the inner axis needs a look at its pieces.
+  uint32_t off[kLoads];
+  __device__ void place(int64_t ld, int o0, int outer, int wave, int lane) {
 #pragma unroll
-    for (int i = 0; i < kBytes / 1024 / WAVES; ++i) {
+    for (int i = 0; i < kLoads; ++i) {
       const int at = (i * WAVES + wave) * 64 + lane, row = at / kP, piece = (at % kP) ^ spread(row);
-      const int o = INNER ? o0 + row : o0 + 8 * piece, k = INNER ? k0 + 8 * piece : k0 + row;
-      const char* src = base + ((INNER ? o : k) * ld + (INNER ? k : o)) * 2;
-      glds16(o < outer && k < inner ? src : reinterpret_cast<const char*>(&g_zeros), lds + (i * WAVES + wave) * 1024);
+      const int last = INNER ? outer - 1 - o0 : (outer + 7) / 8 * 8 - 8 - o0;
+      const int o = INNER ? row : 8 * piece, k = INNER ? 8 * piece : row, oc = o < last ? o : last;
+      off[i] = (uint32_t)(((INNER ? oc : k) * ld + (INNER ? k : oc)) * 2);
     }
+  }
+  // base: the matrix at outer value o0, inner value k0 (a scalar); inner: values left from k0 on
+  __device__ void load(const char* base, int inner, char* lds, int wave, int lane) const {
+    if (inner >= kBK) {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) glds16(base + off[i], lds + (i * WAVES + wave) * 1024);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int at = (i * WAVES + wave) * 64 + lane, row = at / kP, k = INNER ? 8 * ((at % kP) ^ spread(row)) : row;
+        glds16(k < inner ? base + off[i] : reinterpret_cast<const char*>(&g_zeros), lds + (i * WAVES + wave) * 1024);
+      }
+    }
+  }
+};
+
+// Where a lane finds the fragments (outer rows 16 t + x, inner values 32 s + 8 g..+7) of T tiles from t0 on
+template <int R, bool INNER, int T>
+struct FragsOf {
+  int at[INNER ? 2 : T];
+  __device__ FragsOf(int t0, int g, int x) {
+    if (INNER) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) at[s] = ((16 * t0 + x) * kBK + 8 * ((4 * s + g) ^ (x & 7))) * 2;
+    } else {
+      const int k = 8 * g + (x >> 2);   // spread() is the same for rows k, k + 4 and k + 32
+#pragma unroll
+      for (int t = 0; t < T; ++t)
+        at[t] = (k * R + 8 * ((2 * (t0 + t) + ((x & 3) >> 1)) ^ TileOf<R, false, 1>::spread(k)) + 4 * (x & 1)) * 2;
+    }
+  }
+  __device__ bf16x8 get(const char* lds, int t, int s) const {
+    if (INNER) return *reinterpret_cast<const bf16x8*>(lds + at[s] + t * 16 * kBK * 2);
+    const __bf16* p = reinterpret_cast<const __bf16*>(lds + at[t] + s * 32 * R * 2);
+    const bf16x4 u = tr4(p), v = tr4(p + 4 * R);
+    return __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7);
   }
 };
 
@@ -77,8 +104,8 @@ template <int DT, int WM, int WN, int MT, int NT, bool AI, bool BI, bool DUAL, b
 struct Gemm {
   static constexpr int kWaves = WM * WN, kThreads = 64 * kWaves;
   static constexpr int BM = WM * MT * 16, BN = WN * NT * 16, BH = DUAL ? BN / 2 : BN;   // BH: columns of C in a tile
-  using TA = TileOf<BM, AI>;
-  using TB = TileOf<BH, BI>;
+  using TA = TileOf<BM, AI, kWaves>;
+  using TB = TileOf<BH, BI, kWaves>;
   static constexpr int kBuf = TA::kBytes + (DUAL ? 2 : 1) * TB::kBytes;
   static constexpr int kLds = 2 * kBuf;
   static_assert(TA::kBytes % (1024 * kWaves) == 0 && TB::kBytes % (1024 * kWaves) == 0, "whole loads for each wave");
@@ -103,36 +130,50 @@ struct Gemm {
     for (int i = 0; i < MT; ++i)
 #pragma unroll
       for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    auto issue = [&](int it, char* buf) {
-      const int seg = it / kt, k0 = (it - seg * kt) * kBK, mat = SPLIT ? seg / terms : 0, term = SPLIT ? seg % terms : seg;
-      // plane pairs, smallest first: (2,0) (0,2) (1,1) (1,0) (0,1) (0,0)
-      const int pa = terms == 1 ? 0 : term == 0 ? 2 : term == 2 || term == 3 ? 1 : 0;
-      const int pb = terms == 1 ? 0 : term == 1 ? 2 : term == 2 || term == 4 ? 1 : 0;
-      TA::template load<kWaves>(g.a[mat][pa], g.lda, tm * BM, k0, g.M, g.K, buf, wave, lane);
-      TB::template load<kWaves>(g.b[SPLIT ? mat : b_of][pb], g.ldb, tn * BH, k0, g.N, g.K, buf + TA::kBytes, wave, lane);
-      if (DUAL)
-        TB::template load<kWaves>(g.b[1][pb], g.ldb, tn * BH, k0, g.N, g.K, buf + TA::kBytes + TB::kBytes, wave, lane);
+    TA la;
+    TB lb;
+    la.place(g.lda, tm * BM, g.M, wave, lane);
+    lb.place(g.ldb, tn * BH, g.N, wave, lane);
+    const int64_t a0 = (AI ? (int64_t)tm * BM * g.lda : (int64_t)tm * BM) * 2, b0 = (BI ? (int64_t)tn * BH * g.ldb : (int64_t)tn * BH) * 2;
+    const int64_t a_step = (AI ? kBK : kBK * g.lda) * 2, b_step = (BI ? kBK : kBK * g.ldb) * 2;
+    int seg = 0, left = 0;   // segment, inner values left in it
+    const char *pa = nullptr, *pb = nullptr, *pb1 = nullptr;
+    auto issue = [&](char* buf) {
+      if (left <= 0) {
+        const int mat = SPLIT ? seg / terms : 0, term = SPLIT ? seg % terms : seg;
+        // plane pairs, smallest first: (2,0) (0,2) (1,1) (1,0) (0,1) (0,0)
+        const int ia = terms == 1 ? 0 : term == 0 ? 2 : term == 2 || term == 3 ? 1 : 0;
+        const int ib = terms == 1 ? 0 : term == 1 ? 2 : term == 2 || term == 4 ? 1 : 0;
+        pa = g.a[mat][ia] + a0;
+        pb = g.b[SPLIT ? mat : b_of][ib] + b0;
+        pb1 = g.b[1][ib] + b0;
+        left = g.K;
+        ++seg;
+      }
+      la.load(pa, left, buf, wave, lane);
+      lb.load(pb, left, buf + TA::kBytes, wave, lane);
+      if (DUAL) lb.load(pb1, left, buf + TA::kBytes + TB::kBytes, wave, lane);
+      pa += a_step, pb += b_step, pb1 += b_step, left -= kBK;
     };
-    if (total) issue(0, lds);
+    const FragsOf<BM, AI, MT> fa(wm * MT, q, x);
+    constexpr int TN = DUAL ? NT / 2 : NT;
+    const FragsOf<BH, BI, TN> fb(wn * TN, q, x);
+    if (total) issue(lds);
     for (int it = 0; it < total; ++it) {
       const char* buf = lds + (it & 1) * kBuf;
       vm_wait();
       __syncthreads();
-      if (it + 1 < total) issue(it + 1, lds + ((it + 1) & 1) * kBuf);
-      const __bf16* At = reinterpret_cast<const __bf16*>(buf);
+      if (it + 1 < total) issue(lds + ((it + 1) & 1) * kBuf);
 #pragma unroll
       for (int s = 0; s < kBK / 32; ++s) {
-        bf16x8 fb[NT];
+        bf16x8 b[NT];
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          const int half = DUAL ? j / (NT / 2) : 0, t = DUAL ? wn * (NT / 2) + j % (NT / 2) : wn * NT + j;
-          fb[j] = TB::frag(reinterpret_cast<const __bf16*>(buf + TA::kBytes + half * TB::kBytes), t, s, q, x);
-        }
+        for (int j = 0; j < NT; ++j) b[j] = fb.get(buf + TA::kBytes + (DUAL ? j / TN * TB::kBytes : 0), DUAL ? j % TN : j, s);
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
-          const bf16x8 fa = TA::frag(At, wm * MT + i, s, q, x);
+          const bf16x8 a = fa.get(buf, i, s);
 #pragma unroll
-          for (int j = 0; j < NT; ++j) acc[i][j] = mfma16<DT>(fb[j], fa, acc[i][j]);
+          for (int j = 0; j < NT; ++j) acc[i][j] = mfma16<DT>(b[j], a, acc[i][j]);
         }
       }
     }
