@@ -18,6 +18,8 @@ hipError_t dropout(int dtype, const void* x, const void* res, void* y, int64_t n
                    const int64_t* seed_dev, hipStream_t s);
 hipError_t unit_forward(const UnitArgs& u, hipStream_t s);
 hipError_t unit_backward(const UnitArgs& u, hipStream_t s);
+int unit_few_splits(int D, int F, int dtype);
+hipError_t unit_few(const UnitArgs& u, int splits, float* sums, hipStream_t s);
 }  // namespace seq
 
 using namespace seq;
@@ -156,6 +158,7 @@ bool delta_inputs(const SeqDelta* d) { return d->batch * d->T == 0 || (d->q && d
 
 struct UnitSizes {
   bool copy_x, copy_w;
+  int few;   // the forward of a few rows: workgroups along the inner axis; 0: tiles
   int64_t D8, F8, x, w, da, need;
 };
 
@@ -171,12 +174,16 @@ int unit_sizes(const SeqUnit* u, bool backward, UnitSizes& z) {
   const int np = u->dtype == SEQ_FP32 ? 3 : 1;
   z.D8 = (u->D + 7) / 8 * 8;
   z.F8 = (u->F + 7) / 8 * 8;
-  z.copy_x = np == 3 || !aligned16(u->x) || u->x_ld % 8 || u->D % 8;
-  z.copy_w = np == 3 || !aligned16(u->wg) || !aligned16(u->wu) || u->wg_ld % 8 || u->wu_ld != u->wg_ld || u->F % 8;
+  // rows that loads of 16 bytes at 32-bit offsets do not fit
+  z.copy_x = np == 3 || !aligned16(u->x) || u->x_ld % 8 || u->D % 8 || u->x_ld > 1 << 22;
+  z.copy_w = np == 3 || !aligned16(u->wg) || !aligned16(u->wu) || u->wg_ld % 8 || u->wu_ld != u->wg_ld || u->F % 8 || u->wg_ld > 1 << 22;
   z.x = z.copy_x ? up256(u->M * z.D8 * 2 * np) : 0;
   z.w = z.copy_w ? up256(u->D * z.F8 * 2 * np) : 0;
   z.da = backward ? up256(u->M * z.F8 * 2 * np) : 0;
   z.need = z.x + 2 * z.w + 2 * z.da;
+  // up to 32 rows: two tiles of 16 beside each weight fragment are still bound by the weights
+  z.few = !backward && u->M <= 32 ? unit_few_splits(u->D, u->F, u->dtype) : 0;
+  if (z.few) z.need = z.few > 1 ? up256(2LL * z.few * u->M * u->F * 4) : 0;
   return SEQ_OK;
 }
 
@@ -321,6 +328,7 @@ int seq_unit_forward(const SeqUnit* u, void* work, int64_t work_bytes, void* y, 
   UnitArgs a;
   unit_args(u, z, work, a);
   a.y = y, a.pre = pre;
+  if (z.few) return hip_result(unit_few(a, z.few, static_cast<float*>(work), static_cast<hipStream_t>(stream)), "gated_unit");
   return hip_result(unit_forward(a, static_cast<hipStream_t>(stream)), "gated_unit");
 }
 

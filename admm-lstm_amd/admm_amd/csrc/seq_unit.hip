@@ -12,35 +12,11 @@
 // rows are not 16-byte aligned are copied to padded rows.
 #include "seq_gemm.hpp"
 #include "seq_unit.hpp"
+#include "seq_unit_act.hpp"
 
 namespace seq {
 
 namespace {
-
-__device__ __forceinline__ float sigmoid(float z) { return admm::sigm(z); }
-
-// act(z), and its derivative
-__device__ __forceinline__ float act(int kind, float z) {
-  if (kind == SEQ_SILU) return z * sigmoid(z);
-  if (kind == SEQ_GELU) return 0.5f * z * erfcf(-0.70710678118654752f * z);
-  return sigmoid(z);
-}
-__device__ __forceinline__ void act_grad(int kind, float z, float& f, float& df) {
-  if (kind == SEQ_GELU) {
-    const float phi = 0.5f * erfcf(-0.70710678118654752f * z);
-    f = z * phi;
-    df = fmaf(z, 0.39894228040143268f * expf(-0.5f * z * z), phi);
-  } else {
-    const admm::SigPair s = admm::sig_pair(z);
-    if (kind == SEQ_SILU) {
-      f = z * s.s;
-      df = s.s * fmaf(z, s.sc, 1.f);
-    } else {
-      f = s.s;
-      df = s.s * s.sc;
-    }
-  }
-}
 
 // rows of n values with the stride ld, as rows of n8 >= n values, the rest zero: 16-bit values as they are, f32 as three planes
 // (`plane` elements apart)
@@ -49,9 +25,10 @@ __global__ __launch_bounds__(256) void k_unit_copy(const void* src, int64_t ld, 
   using T = typename Elem<DT>::T;
   const T* s = static_cast<const T*>(src);
   const int64_t pieces = n8 / 8, all = rows * pieces;
+  const bool small = all < (int64_t)1 << 32;
   const bool wide = reinterpret_cast<uintptr_t>(src) % 16 == 0 && ld * (int)sizeof(T) % 16 == 0;
   for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / pieces, p = i % pieces;
+    const int64_t r = small ? (uint32_t)i / (uint32_t)pieces : i / pieces, p = i - r * pieces;
     const int left = n - (int)(8 * p);
     __bf16* d = dst + r * n8 + 8 * p;
     if constexpr (DT == SEQ_FP32) {
@@ -147,9 +124,10 @@ __global__ __launch_bounds__(256) void k_unit_back(UnitArgs u) {
   using T = typename Elem<DT>::T;
   const int64_t pieces = u.F8 / 8, all = u.M * pieces, plane = u.M * u.F8, MF = (int64_t)u.M * u.F;
   const T* dy = static_cast<const T*>(u.dy);
+  const bool small = all < (int64_t)1 << 32;   // 64-bit division takes longer than the rest
   const bool wide = u.F % 8 == 0, wide_dy = reinterpret_cast<uintptr_t>(dy) % 16 == 0 && u.dy_ld * (int)sizeof(T) % 16 == 0;
   for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / pieces, p = i % pieces;
+    const int64_t r = small ? (uint32_t)i / (uint32_t)pieces : i / pieces, p = i - r * pieces;
     const int left = u.F - (int)(8 * p);
     const f32x8 a = load8(u.pre + r * u.F + 8 * p, left, wide), b = load8(u.pre + MF + r * u.F + 8 * p, left, wide);
     const f32x8 d = load8(dy + r * u.dy_ld + 8 * p, left, wide_dy);
@@ -230,8 +208,16 @@ hipError_t launch_gemm(GemmArgs g, void* c0, void* c1, hipStream_t s) {
   return hipSuccess;
 }
 
-// tiles of 256 x 256 where they make work for most of the 256 compute units, else 64 x 64
-bool big(int64_t m, int64_t n) { return ((m + 255) / 256) * ((n + 255) / 256) >= 128; }
+// Tile sizes of an m x n result (n: both projections' columns): 0: 256 x 256 (8 waves, one workgroup a compute unit), 1: 128 x
+// 128 (4 waves, two), 2: 64 x 64 (4 waves, four).  The one whose rounds over the 256 units take the least: a round is the work of a
+// unit's workgroups over the share of the matrix cores' rate that the tile reaches (measured at M 4096, D 2048: 1, 0.7, 0.35 of
+// that of the first; smaller tiles read more of LDS for a product).
+int tile_for(int64_t m, int64_t n) {
+  auto rounds = [](int64_t tiles, int slots) { return (double)((tiles + slots - 1) / slots); };
+  auto count = [&](int t) { return ((m + t - 1) / t) * ((n + t - 1) / t); };
+  const double cost[3] = {rounds(count(256), 256), rounds(count(128), 512) * 2 / 4 / 0.7, rounds(count(64), 1024) * 4 / 16 / 0.35};
+  return cost[0] <= cost[1] && cost[0] <= cost[2] ? 0 : cost[1] <= cost[2] ? 1 : 2;
+}
 
 template <int DT>
 hipError_t forward(const UnitArgs& u, hipStream_t s) {
@@ -248,7 +234,9 @@ hipError_t forward(const UnitArgs& u, hipStream_t s) {
   planes(g.a[0], u.copy_x, u.x, u.xp, u.M * u.D8);
   planes(g.b[0], u.copy_w, u.wg, u.wgp, u.D * u.F8);
   planes(g.b[1], u.copy_w, u.wu, u.wup, u.D * u.F8);
-  const hipError_t e = big(u.M, 2 * (int64_t)u.F) ? launch_unit<DT, 2, 4, 8, 4>(g, u, s) : launch_unit<DT, 2, 2, 2, 4>(g, u, s);
+  const int tile = tile_for(u.M, 2 * (int64_t)u.F);
+  const hipError_t e = tile == 0 ? launch_unit<DT, 2, 4, 8, 4>(g, u, s)
+                       : tile == 1 ? launch_unit<DT, 2, 2, 4, 4>(g, u, s) : launch_unit<DT, 2, 2, 2, 2>(g, u, s);
   return e != hipSuccess ? e : hipGetLastError();
 }
 
@@ -272,8 +260,10 @@ hipError_t backward(const UnitArgs& u, hipStream_t s) {
     planes(g.a[1], true, nullptr, u.dbp, u.M * u.F8);
     planes(g.b[0], u.copy_w, u.wg, u.wgp, u.D * u.F8);
     planes(g.b[1], u.copy_w, u.wu, u.wup, u.D * u.F8);
-    e = big(u.M, u.D) ? launch_gemm<DT, 2, 4, 8, 4, true, true, true>(g, u.dx, nullptr, s)
-                      : launch_gemm<DT, 2, 2, 2, 2, true, true, true>(g, u.dx, nullptr, s);
+    const int tile = tile_for(u.M, u.D);
+    e = tile == 0 ? launch_gemm<DT, 2, 4, 8, 4, true, true, true>(g, u.dx, nullptr, s)
+        : tile == 1 ? launch_gemm<DT, 2, 2, 4, 4, true, true, true>(g, u.dx, nullptr, s)
+                    : launch_gemm<DT, 2, 2, 2, 2, true, true, true>(g, u.dx, nullptr, s);
     if (e != hipSuccess) return e;
   }
   if (u.dwg) {
@@ -285,8 +275,10 @@ hipError_t backward(const UnitArgs& u, hipStream_t s) {
     planes(g.a[0], u.copy_x, u.x, u.xp, u.M * u.D8);
     planes(g.b[0], true, nullptr, u.dap, u.M * u.F8);
     planes(g.b[1], true, nullptr, u.dbp, u.M * u.F8);
-    e = big(u.D, 2 * (int64_t)u.F) ? launch_gemm<DT, 2, 4, 8, 4, false, false, false>(g, u.dwg, u.dwu, s)
-                                   : launch_gemm<DT, 2, 2, 2, 2, false, false, false>(g, u.dwg, u.dwu, s);
+    const int tile = tile_for(u.D, 2 * (int64_t)u.F);
+    e = tile == 0 ? launch_gemm<DT, 2, 4, 8, 4, false, false, false>(g, u.dwg, u.dwu, s)
+        : tile == 1 ? launch_gemm<DT, 2, 2, 4, 4, false, false, false>(g, u.dwg, u.dwu, s)
+                    : launch_gemm<DT, 2, 2, 2, 2, false, false, false>(g, u.dwg, u.dwu, s);
     if (e != hipSuccess) return e;
   }
   return hipGetLastError();
