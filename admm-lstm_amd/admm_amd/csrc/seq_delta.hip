@@ -12,9 +12,7 @@ template <int DT, int KP, int C, bool SAVE>
 struct PrepLds {
   using S = DeltaShape<DT, KP, C, SAVE>;
   static constexpr int ld = C + 4;                 // row length of the f32 tiles
-  static constexpr int kq = 2 * S::NP * C * KP * 2;
-  static constexpr int xp = 2 * C * ld * 4 + (C / 2) * kLdY * 4;
-  static constexpr int mats = xp + (3 + S::NPP) * C * C * 2;
+  static constexpr int kq = 2 * S::NP * C * KP * 2, mats = (2 * C * ld + (C / 2) * kLdY) * 4;
   static constexpr int vec = kq > mats ? kq : mats;
   static constexpr int bytes = vec + 4 * C * 4;
 };
@@ -28,18 +26,32 @@ __device__ __forceinline__ f32x4 mm16(const float* a, int lda, const float* b, i
   return acc;
 }
 
+// eight values of a f32 tile as planes: of row r, columns c..c + 7, or (T) of column r, rows c..c + 7
+template <int NP, bool T>
+__device__ __forceinline__ void tile_planes(const float* m, int ld, int r, int c, bf16x8 (&p)[NP]) {
+  f32x8 v;
+  if (T) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = m[(c + i) * ld + r];
+  } else {
+    v = cat8(*reinterpret_cast<const f32x4*>(m + r * ld + c), *reinterpret_cast<const f32x4*>(m + r * ld + c + 4));
+  }
+  planes8<NP>(v, p);
+}
+
+// Bound by the chain of small products, exchanges and barriers of a chunk: several workgroups on a compute unit cover for each
+// other, so the f32 tiles lie where K and Q were, and fragments are cut straight from them.
 template <int DT, int KP, int C, bool SAVE>
-__global__ __launch_bounds__(4 * C) void k_delta_prep(DeltaArgs a) {
+__global__ __launch_bounds__(4 * C, DT == SEQ_FP32 ? 2 : 3) void k_delta_prep(DeltaArgs a) {
   using S = DeltaShape<DT, KP, C, SAVE>;
   using L = PrepLds<DT, KP, C, SAVE>;
   using T = typename Elem<DT>::T;
-  constexpr int NP = S::NP, W = S::RT, kThreads = 64 * W, kLd = L::ld, kTile = C * KP, kMat = C * C;
+  constexpr int NP = S::NP, W = S::RT, kThreads = 64 * W, kLd = L::ld, kTile = C * KP;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   __bf16* const kq = reinterpret_cast<__bf16*>(lds);
-  float* const A = reinterpret_cast<float*>(lds);           // after the Gram products: over K and Q
+  float* const A = reinterpret_cast<float*>(lds);           // after the Gram products: over K and Q; later P
   float* const X = A + C * kLd;
   float* const Y = X + C * kLd;
-  __bf16* const xp = reinterpret_cast<__bf16*>(lds + L::xp);   // planes of X, then of P
   float* const ghi = reinterpret_cast<float*>(lds + L::vec);
   float* const glo = ghi + C;
   float* const bet = glo + C;
@@ -57,34 +69,54 @@ __global__ __launch_bounds__(4 * C) void k_delta_prep(DeltaArgs a) {
   const int64_t bt = a.rows.batch(n), r0 = begin + t0;
 
   // K and Q rows as planes in LDS
-  if (tid < C) kbad[tid] = 0;
-  __syncthreads();
   {
+    constexpr int N = C * (KP / 8) / kThreads;   // pieces of eight of each, for a thread
     const T* kp = static_cast<const T*>(a.k) + bt * a.ks[0] + r0 * a.ks[1] + hk * a.ks[2];
     const T* qp = static_cast<const T*>(a.q) + bt * a.qs[0] + r0 * a.qs[1] + hk * a.qs[2];
-    for (int i = tid; i < 2 * C * (KP / 8); i += kThreads) {
-      const int w = i / (C * (KP / 8)), r = i / (KP / 8) % C, p = i % (KP / 8);
-      const T* src = w ? qp + (int64_t)r * a.qs[1] : kp + (int64_t)r * a.ks[1];
-      f32x8 x = {};
-      const int left = a.K - 8 * p;
-      if (r < rows && left > 0) x = load8(src + 8 * p, left, w ? a.wide_q : a.wide_k);
-      if (!w && zero_if_finite(x.lo) + zero_if_finite(x.hi) != 0.f) kbad[r] = 1;
-      bf16x8 pl[NP];
-      planes8<NP>(x, pl);
+    const int p = tid % (KP / 8), left = a.K - 8 * p;
+    f32x8 v[2][N];
 #pragma unroll
-      for (int j = 0; j < NP; ++j) *reinterpret_cast<bf16x8*>(kq + (w * NP + j) * kTile + tile_at<KP>(r, p)) = pl[j];
+    for (int i = 0; i < N; ++i) {
+      const int r = tid / (KP / 8) + i * (kThreads / (KP / 8));
+      v[0][i] = v[1][i] = f32x8{};
+      if (r < rows && left > 0) {
+        v[0][i] = load8(kp + r * a.ks[1] + 8 * p, left, a.wide_k);
+        v[1][i] = load8(qp + r * a.qs[1] + 8 * p, left, a.wide_q);
+      }
+    }
+    float odd[N], any = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int r = tid / (KP / 8) + i * (kThreads / (KP / 8));
+      odd[i] = zero_if_finite(v[0][i].lo) + zero_if_finite(v[0][i].hi);
+      any += odd[i];
+      bf16x8 pl[NP];
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        planes8<NP>(v[w][i], pl);
+#pragma unroll
+        for (int j = 0; j < NP; ++j) *reinterpret_cast<bf16x8*>(kq + (w * NP + j) * kTile + tile_at<KP>(r, p)) = pl[j];
+      }
+    }
+    if (tid < C) kbad[tid] = 0;
+    if (__syncthreads_or(any != 0.f)) {   // rows of k that are not finite: zeros, and marked
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (odd[i] != 0.f) kbad[tid / (KP / 8) + i * (kThreads / (KP / 8))] = 1;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int r = tid / (KP / 8) + i * (kThreads / (KP / 8));
+        if (!kbad[r]) continue;
+#pragma unroll
+        for (int j = 0; j < NP; ++j) *reinterpret_cast<u32x4*>(kq + j * kTile + tile_at<KP>(r, p)) = u32x4{0, 0, 0, 0};
+      }
+      __syncthreads();
     }
   }
-  __syncthreads();
-  for (int i = tid; i < C * NP * (KP / 8); i += kThreads) {
-    const int r = i / (NP * (KP / 8)), j = i / (KP / 8) % NP;
-    if (kbad[r]) *reinterpret_cast<u32x4*>(kq + j * kTile + tile_at<KP>(r, i % (KP / 8))) = u32x4{0, 0, 0, 0};
-  }
-  __syncthreads();
   // their fragments
   {
     char* dst = a.kq + (c * a.Hk + hk) * (int64_t)S::kKQ + lane * 16;
-#pragma unroll 1
     for (int f = wave; f < S::fEnd; f += W) {
       bf16x8 v[NP];
       if (f < S::fKT) {
@@ -116,12 +148,12 @@ __global__ __launch_bounds__(4 * C) void k_delta_prep(DeltaArgs a) {
       qk[j] = mfma_planes<NP, NP, 3>(qa, kb, qk[j]);
     }
   }
+  mfma_settle();
 
   const int group = a.Hv / a.Hk;
   for (int e = 0; e < group; ++e) {
     const int h = hk * group + e;
     const int64_t ch = c * a.Hv + h;
-    __syncthreads();   // K, Q (first round) or the last head's tiles are done with
     if (wave == 0) {
       const bool in = lane < rows;
       float gv = in ? a.g[bt * a.gs[0] + (r0 + lane) * a.gs[1] + h * a.gs[2]] : 0.f;
@@ -144,26 +176,19 @@ __global__ __launch_bounds__(4 * C) void k_delta_prep(DeltaArgs a) {
       vec[128 + lane] = bv;
       vec[192 + lane] = lane == 1 ? (float)bad : expf((float)last);
     }
-    __syncthreads();
-    for (int i = tid; i < C * kLd; i += kThreads) X[i] = 0.f;
+    __syncthreads();   // and K, Q (first round) or the last head's tiles are done with
+    float pv[S::RT][4];
 #pragma unroll
-    for (int j = 0; j < S::RT; ++j) {
+    for (int j = 0; j < S::RT; ++j)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int row = 16 * wave + 4 * g + r, col = 16 * j + m;
         const bool lower = col <= row;
         const float d = lower ? expf((ghi[row] - ghi[col]) + (glo[row] - glo[col])) : 0.f;
         A[row * kLd + col] = col < row ? bet[row] * d * kk[j][r] : 0.f;
-        const float p = lower ? a.scale * d * qk[j][r] : 0.f;
-        __bf16* pp = xp + 3 * kMat + tile_at<C>(row, col >> 3) + (col & 7);
-        const __bf16 p0 = (__bf16)p;
-        const float q1 = p - (float)p0;
-        const __bf16 p1 = (__bf16)q1;
-        pp[0] = p0;
-        pp[kMat] = p1;
-        if constexpr (S::NPP > 2) pp[2 * kMat] = (__bf16)(q1 - (float)p1);
+        X[row * kLd + col] = 0.f;
+        pv[j][r] = lower ? a.scale * d * qk[j][r] : 0.f;
       }
-    }
     __syncthreads();
     // X = (I + A)^-1: the diagonal 16 x 16 blocks by substitution (a lane has one column), then joined in pairs
     if (wave == 0 && g < S::RT) {
@@ -173,7 +198,12 @@ __global__ __launch_bounds__(4 * C) void k_delta_prep(DeltaArgs a) {
       for (int i = 0; i < 16; ++i) {
         float t = i == m ? 1.f : 0.f;
 #pragma unroll
-        for (int j = 0; j < i; ++j) t = fmaf(-blk[i * kLd + j], x[j], t);
+        for (int q = 0; q < (i + 3) / 4; ++q) {
+          const f32x4 v = *reinterpret_cast<const f32x4*>(blk + i * kLd + 4 * q);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (4 * q + j < i) t = fmaf(-v[j], x[4 * q + j], t);
+        }
         x[i] = t;
       }
 #pragma unroll
@@ -201,36 +231,36 @@ __global__ __launch_bounds__(4 * C) void k_delta_prep(DeltaArgs a) {
       const f32x4 z = mm16(X + (32 + 16 * ti) * kLd + 32, kLd, Y + 16 * tj, kLdY, 2, lane);
 #pragma unroll
       for (int r = 0; r < 4; ++r) X[(32 + 16 * ti + 4 * g + r) * kLd + 16 * tj + m] = -z[r];
-      __syncthreads();
     }
-    for (int i = tid; i < C * C / 8; i += kThreads) {
-      const int r = i / (C / 8), p = i % (C / 8);
-      const f32x4* src = reinterpret_cast<const f32x4*>(X + r * kLd + 8 * p);
-      bf16x8 pl[3];
-      planes8<3>(cat8(src[0], src[1]), pl);
+    // P where A was (all of A has been read before the last barrier)
 #pragma unroll
-      for (int j = 0; j < 3; ++j) *reinterpret_cast<bf16x8*>(xp + j * kMat + tile_at<C>(r, p)) = pl[j];
-    }
+    for (int j = 0; j < S::RT; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) A[(16 * wave + 4 * g + r) * kLd + 16 * j + m] = pv[j][r];
     __syncthreads();
     char* dst = a.xp + ch * (int64_t)S::kXP + lane * 16;
-#pragma unroll 1
-    for (int f = wave; f < (SAVE ? 4 : 2) * S::TRI; f += W) {
-      const int kind = f / S::TRI, e = f % S::TRI;   // X, P, X^T, P^T
-      const int np = kind & 1 ? S::NPP : 3;
-      const __bf16* src = xp + (kind & 1 ? 3 * kMat : 0);
-      char* p = dst + (kind == 0 ? S::pX : kind == 1 ? S::pP : kind == 2 ? S::pXT : S::pPT) * 1024 + e * np * 1024;
-      for (int j = 0; j < np; ++j) {
-        bf16x8 v[1];
-        if (kind < 2) {
-          const int t = e < 2 ? e : 2 + ((e - 2) >> 1), s = e < 2 ? 0 : (e - 2) & 1;
-          frag<C, 1, kMat>(src + j * kMat, perm_row(t, m), s, g, v);
-        } else {
-          const int t = C == 32 || e >= 4 ? (C == 32 ? e : e - 2) : e >> 1, s = C == 32 ? 0 : e >= 4 ? 1 : e & 1;
-          frag_t<C, 1, kMat>(src + j * kMat, t, s, g, m, v);
-        }
-        *reinterpret_cast<bf16x8*>(p + j * 1024) = v[0];
+    // a fragment's tile and inner step: rows (kind 0, 1: X, P) or columns (2, 3: X^T, P^T)
+    auto cut = [&](auto np, auto transposed, const float* mat, int first, int f) {
+      constexpr int N = decltype(np)::value;
+      constexpr bool TR = decltype(transposed)::value;
+      const int t = C == 32 ? f : TR ? (f >= 4 ? f - 2 : f >> 1) : (f < 2 ? f : 2 + ((f - 2) >> 1));
+      const int s = C == 32 ? 0 : TR ? (f >= 4 ? 1 : f & 1) : (f < 2 ? 0 : (f - 2) & 1);
+      bf16x8 v[N];
+      tile_planes<N, TR>(mat, kLd, perm_row(t, m), 32 * s + 8 * g, v);
+#pragma unroll
+      for (int j = 0; j < N; ++j) *reinterpret_cast<bf16x8*>(dst + (first + f * N + j) * 1024) = v[j];
+    };
+    for (int f = wave; f < 2 * S::TRI; f += W) {
+      if (f < S::TRI) cut(std::integral_constant<int, 3>(), std::false_type(), X, S::pX, f);
+      else cut(std::integral_constant<int, S::NPP>(), std::false_type(), A, S::pP, f - S::TRI);
+    }
+    if constexpr (SAVE) {
+      for (int f = wave; f < 2 * S::TRI; f += W) {
+        if (f < S::TRI) cut(std::integral_constant<int, 3>(), std::true_type(), X, S::pXT, f);
+        else cut(std::integral_constant<int, 3>(), std::true_type(), A, S::pPT, f - S::TRI);
       }
     }
+    if (e + 1 < group) __syncthreads();   // before the next head's sums and tiles
   }
 }
 
@@ -546,16 +576,13 @@ __global__ __launch_bounds__(8 * C, 2) void k_delta_scan(DeltaArgs a) {
   }
 }
 
-// rows of packed sequences that belong to none: before the first and behind the last.  row: bytes of a row
-__global__ void k_delta_outside(DeltaRows rows, void* p, int64_t row) {
-  const int64_t first = rows.at(0), last = rows.at(rows.N);
-  const int64_t n = (first + (rows.T - (last > first ? last : first))) * row;
-  char* q = static_cast<char*>(p);
-  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i * 2 < n; i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t b = i * 2;
-    const int64_t at = b < first * row ? b : b - first * row + (last > first ? last : first) * row;
-    *reinterpret_cast<uint16_t*>(q + at) = 0;
-  }
+// zeros in the rows of packed sequences that belong to none, before the first and behind the last, of up to five tensors
+__global__ void k_delta_outside(DeltaRows rows, DeltaOutside t) {
+  const int64_t first = rows.at(0), end = rows.at(rows.N), last = end > first ? end : first;
+  const int64_t row = t.row[blockIdx.y], n = (first + rows.T - last) * row;   // row: bytes, even
+  char* q = static_cast<char*>(t.p[blockIdx.y]);
+  for (int64_t b = 2 * (blockIdx.x * (int64_t)blockDim.x + threadIdx.x); b < n; b += 2 * (int64_t)gridDim.x * blockDim.x)
+    *reinterpret_cast<uint16_t*>(q + (b < first * row ? b : b + (last - first) * row)) = 0;
 }
 
 template <int DT, int KP, int C, int NC, bool SAVE>
@@ -590,8 +617,8 @@ hipError_t forward(const DeltaArgs& a, int KP, bool save, hipStream_t s) {
 
 }  // namespace
 
-hipError_t delta_outside(const DeltaRows& rows, void* p, int64_t row_bytes, hipStream_t s) {
-  k_delta_outside<<<64, 256, 0, s>>>(rows, p, row_bytes);
+hipError_t delta_outside(const DeltaRows& rows, const DeltaOutside& t, hipStream_t s) {
+  k_delta_outside<<<dim3(64, t.n), 256, 0, s>>>(rows, t);
   return hipGetLastError();
 }
 

@@ -84,6 +84,12 @@ struct DeltaRows {
   }
 };
 
+struct DeltaOutside {
+  int n;
+  void* p[5];
+  int64_t row[5];   // bytes of a row
+};
+
 struct DeltaArgs {
   DeltaRows rows;
   int Hk, Hv, K, V, VP;   // VP: V rounded up to 16

@@ -12,7 +12,7 @@
 namespace seq {
 hipError_t delta_forward(const DeltaArgs& a, int dtype, int KP, bool save, hipStream_t s);
 hipError_t delta_backward(const DeltaGradArgs& ga, int dtype, int KP, bool wide_v, bool wide_o, hipStream_t s);
-hipError_t delta_outside(const DeltaRows& rows, void* p, int64_t row_bytes, hipStream_t s);
+hipError_t delta_outside(const DeltaRows& rows, const DeltaOutside& t, hipStream_t s);
 hipError_t delta_step(const SeqDeltaStep& d, hipStream_t s);
 hipError_t dropout(int dtype, const void* x, const void* res, void* y, int64_t n, uint32_t below, uint64_t seed, uint64_t offset,
                    const int64_t* seed_dev, hipStream_t s);
@@ -231,7 +231,8 @@ int seq_delta_forward(const SeqDelta* d, int32_t saved, void* work, int64_t work
   a.final = final_state;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (d->offsets && d->T) {
-    const int e = hip_result(delta_outside(a.rows, o, (int64_t)d->Hv * d->V * elem_size(d->dtype), s), "delta_rule");
+    const DeltaOutside t = {1, {o}, {(int64_t)d->Hv * d->V * elem_size(d->dtype)}};
+    const int e = hip_result(delta_outside(a.rows, t, s), "delta_rule");
     if (e) return e;
   }
   if (!d->sequences) return SEQ_OK;
@@ -277,10 +278,8 @@ int seq_delta_backward(const SeqDelta* d, const void* work, int64_t work_bytes, 
   }
   if (rc || !d->offsets || !some) return rc;
   const int64_t size = elem_size(d->dtype), kb = (int64_t)d->Hk * d->K * size, vb = (int64_t)d->Hv * d->V * size, hb = (int64_t)d->Hv * 4;
-  void* const out[5] = {dq, dk, dv, dg, dbeta};
-  const int64_t row[5] = {kb, kb, vb, hb, hb};
-  for (int i = 0; i < 5 && !rc; ++i) rc = hip_result(delta_outside(ga.f.rows, out[i], row[i], s), "delta_rule backward");
-  return rc;
+  const DeltaOutside t = {5, {dq, dk, dv, dg, dbeta}, {kb, kb, vb, hb, hb}};
+  return hip_result(delta_outside(ga.f.rows, t, s), "delta_rule backward");
 }
 
 int seq_delta_step(const SeqDeltaStep* d, void* stream) {
