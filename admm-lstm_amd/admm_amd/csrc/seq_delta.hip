@@ -435,7 +435,7 @@ __global__ __launch_bounds__(8 * C, 2) void k_delta_scan(DeltaArgs a) {
         for (int i = 0; i < NC; ++i) {
 #pragma unroll
           for (int r = 3; r >= 0; --r)
-            if (ks[i][r] - ks[i][r] != 0.f) {
+            if (ks[i][r] * 0.f != 0.f) {   // (not a - a, which may contract to the rounding error of a product)
               ks[i][r] = 0.f;
               bad[i] = row0 + r < bad[i] ? row0 + r : bad[i];
             }

@@ -52,6 +52,13 @@ __device__ __forceinline__ double running_sum(float v, int lane, double& last) {
 
 // ---- fragments in the work memory and operands B in LDS
 
+// sum over the 16 lanes of a row of the wave, in all of them: rotations within the row, which cost an addition no more time
+template <int N>
+__device__ __forceinline__ float add_turned(float v) {
+  return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x120 + N, 0xf, 0xf, false));
+}
+__device__ __forceinline__ float sum16(float v) { return add_turned<1>(add_turned<2>(add_turned<4>(add_turned<8>(v)))); }
+
 // keeps a branch around what hardly ever runs (the compiler would rather run both sides and select)
 __device__ __forceinline__ void rare_path() { asm volatile(""); }
 

@@ -295,11 +295,6 @@ struct GradLds {
   static constexpr int bytes = vec + (7 + 5 * S::RT) * C * 4 + 32;
 };
 
-__device__ __forceinline__ float sum16(float v) {
-#pragma unroll
-  for (int d = 1; d < 16; d *= 2) v += __shfl_xor(v, d);
-  return v;
-}
 
 template <int NP, int TILE>
 __device__ __forceinline__ float whole(const __bf16* p) {
@@ -642,7 +637,6 @@ hipError_t back(const DeltaGradArgs& ga, hipStream_t s) {
 
 template <int DT, int KP, int C>
 hipError_t backward(const DeltaGradArgs& ga, bool wide_v, bool wide_o, hipStream_t s) {
-  using T = typename Elem<DT>::T;
   constexpr int bytes = GradLds<DT, KP, C>::bytes;
   const DeltaArgs& a = ga.f;
   hipError_t e = a.wide_cols ? back<DT, KP, C, 2>(ga, s) : back<DT, KP, C, 1>(ga, s);
@@ -650,13 +644,15 @@ hipError_t backward(const DeltaGradArgs& ga, bool wide_v, bool wide_o, hipStream
   e = allow_lds(k_delta_grad<DT, KP, C>, bytes);
   if (e != hipSuccess) return e;
   if (a.chunks) k_delta_grad<DT, KP, C><<<(unsigned)(a.chunks * a.Hv), 4 * C, bytes, s>>>(ga, wide_v, wide_o);
-  if (ga.dq32) {
-    const int64_t rows = a.rows.off ? a.rows.T : a.rows.N * a.rows.T, n = rows * a.Hk * a.K;
-    const int64_t want = (n + 255) / 256;
-    if (n) k_delta_heads<T><<<(unsigned)(want < 8192 ? want : 8192), 256, 0, s>>>(
-               ga.dq32, ga.dk32, static_cast<T*>(ga.dq), static_cast<T*>(ga.dk), n, a.Hv / a.Hk, a.K);
-  }
   return hipGetLastError();
+}
+
+template <class T>
+void heads(const DeltaGradArgs& ga, hipStream_t s) {
+  const DeltaArgs& a = ga.f;
+  const int64_t rows = a.rows.off ? a.rows.T : a.rows.N * a.rows.T, n = rows * a.Hk * a.K, want = (n + 255) / 256;
+  if (n) k_delta_heads<T><<<(unsigned)(want < 8192 ? want : 8192), 256, 0, s>>>(
+             ga.dq32, ga.dk32, static_cast<T*>(ga.dq), static_cast<T*>(ga.dk), n, a.Hv / a.Hk, a.K);
 }
 
 template <int DT, int KP>
@@ -676,6 +672,14 @@ hipError_t delta_backward(const DeltaGradArgs& ga, int dtype, int KP, bool wide_
   return dtype == SEQ_BF16 ? backward<SEQ_BF16>(ga, KP, wide_v, wide_o, s)
          : dtype == SEQ_FP16 ? backward<SEQ_FP16>(ga, KP, wide_v, wide_o, s)
                              : backward<SEQ_FP32>(ga, KP, wide_v, wide_o, s);
+}
+
+// dq and dk of the query/key heads from their value heads' shares
+hipError_t delta_heads(const DeltaGradArgs& ga, int dtype, hipStream_t s) {
+  if (dtype == SEQ_BF16) heads<__bf16>(ga, s);
+  else if (dtype == SEQ_FP16) heads<_Float16>(ga, s);
+  else heads<float>(ga, s);
+  return hipGetLastError();
 }
 
 }  // namespace seq

@@ -12,6 +12,9 @@
 namespace seq {
 hipError_t delta_forward(const DeltaArgs& a, int dtype, int KP, bool save, hipStream_t s);
 hipError_t delta_backward(const DeltaGradArgs& ga, int dtype, int KP, bool wide_v, bool wide_o, hipStream_t s);
+hipError_t delta_heads(const DeltaGradArgs& ga, int dtype, hipStream_t s);
+hipError_t delta_short_forward(const DeltaArgs& a, int dtype, int KP, hipStream_t s);
+hipError_t delta_short_backward(const DeltaGradArgs& ga, int dtype, int KP, bool wide_s, hipStream_t s);
 hipError_t delta_outside(const DeltaRows& rows, const DeltaOutside& t, hipStream_t s);
 hipError_t delta_step(const SeqDeltaStep& d, hipStream_t s);
 hipError_t dropout(int dtype, const void* x, const void* res, void* y, int64_t n, uint32_t below, uint64_t seed, uint64_t offset,
@@ -75,7 +78,7 @@ int check_heads(int Hk, int Hv, int K, int V, int dtype) {
 
 struct DeltaSizes {
   int KP, C;
-  bool wide_cols;
+  bool brief, wide_cols;   // brief: one kernel for a whole sequence (at most 32 rows, not packed), without work memory
   int64_t per, chunks, VP, kq, xp, vec, s0, u, heads, need;
 };
 
@@ -91,6 +94,7 @@ int delta_sizes(const SeqDelta* d, bool saved, DeltaSizes& z) {
   z.KP = d->K <= 32 ? 32 : d->K <= 64 ? 64 : 128;
   // sequences of at most 32 rows (or packed ones of at most 32 on average) would leave half of a 64-row chunk empty
   z.C = d->T <= 32 || (d->offsets && d->T <= 32 * d->sequences) ? 32 : 64;
+  z.brief = !d->offsets && d->T > 0 && d->T <= 32;
   const int NP = d->dtype + 1, NO = d->dtype == SEQ_FP32 ? 3 : 2, tri = z.C == 64 ? 6 : 2;
   z.per = (d->T + z.C - 1) / z.C;
   z.VP = (d->V + 15) / 16 * 16;
@@ -106,6 +110,7 @@ int delta_sizes(const SeqDelta* d, bool saved, DeltaSizes& z) {
   z.u = up256(z.chunks * d->Hv * 4 * z.C * z.VP);
   const int64_t rows = d->batch * d->T;
   z.heads = d->Hv > d->Hk ? up256(rows * d->Hv * d->K * 4) : 0;
+  if (z.brief) z.kq = z.xp = z.vec = z.s0 = z.u = 0;
   z.need = z.kq + z.xp + z.vec + (saved ? z.s0 + z.u : 0);
   return SEQ_OK;
 }
@@ -236,6 +241,7 @@ int seq_delta_forward(const SeqDelta* d, int32_t saved, void* work, int64_t work
     if (e) return e;
   }
   if (!d->sequences) return SEQ_OK;
+  if (z.brief) return hip_result(delta_short_forward(a, d->dtype, z.KP, s), "delta_rule");
   return hip_result(delta_forward(a, d->dtype, z.KP, saved != 0, s), "delta_rule");
 }
 
@@ -273,8 +279,16 @@ int seq_delta_backward(const SeqDelta* d, const void* work, int64_t work_bytes, 
   ga.d_o = d_o, ga.d_final = d_final;
   ga.dq = dq, ga.dk = dk, ga.dv = dv, ga.dg = dg, ga.dbeta = dbeta, ga.d_initial = d_initial;
   if (d->sequences) {
-    const bool wide_o = aligned16(d_o) && d->V % 8 == 0;
-    rc = hip_result(delta_backward(ga, d->dtype, z.KP, wide_rows(d, d->V, d->v, d->v_stride), wide_o, s), "delta_rule backward");
+    hipError_t e;
+    if (z.brief) {
+      const bool wide_s = d->V % 4 == 0 && aligned16(d->initial) && aligned16(d_final);
+      e = delta_short_backward(ga, d->dtype, z.KP, wide_s, s);
+    } else {
+      const bool wide_o = aligned16(d_o) && d->V % 8 == 0;
+      e = delta_backward(ga, d->dtype, z.KP, wide_rows(d, d->V, d->v, d->v_stride), wide_o, s);
+    }
+    if (e == hipSuccess && z.heads) e = delta_heads(ga, d->dtype, s);
+    rc = hip_result(e, "delta_rule backward");
   }
   if (rc || !d->offsets || !some) return rc;
   const int64_t size = elem_size(d->dtype), kb = (int64_t)d->Hk * d->K * size, vb = (int64_t)d->Hv * d->V * size, hb = (int64_t)d->Hv * 4;
