@@ -161,12 +161,9 @@ struct ColumnRows {
 __device__ __forceinline__ f32x4 load_state(const float* p, int K, int V, int col, int t, int g) {
   f32x4 st = {0.f, 0.f, 0.f, 0.f};
   if (!p) return st;
-  const int c = col < V ? col : V - 1;
+  const int c = col < V ? col : V - 1, at = perm_row(t, 4 * g) * V + c, last = (K - 1) * V + c;   // K V <= 2^23
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const int kd = perm_row(t, 4 * g + r);
-    st[r] = p[(int64_t)(kd < K ? kd : K - 1) * V + c];
-  }
+  for (int r = 0; r < 4; ++r) st[r] = p[min(at + r * V, last)];
 #pragma unroll
   for (int r = 0; r < 4; ++r) st[r] = col < V && perm_row(t, 4 * g + r) < K ? st[r] : 0.f;
   return st;

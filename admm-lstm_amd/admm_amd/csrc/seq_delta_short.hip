@@ -10,6 +10,8 @@
 // rows, 4 heads of 64 x 64, f32, forward and backward: 1.15 ms through work memory.
 #include "seq_delta_dev.hpp"
 
+#include <type_traits>
+
 namespace seq {
 namespace {
 
@@ -46,7 +48,6 @@ __device__ __forceinline__ void short_prep(const DeltaArgs& a, int64_t n, int h,
   ShortVec* const sv = reinterpret_cast<ShortVec*>(lds + L::vec);
   const int tid = threadIdx.x, lane = tid & 63, wave = wave_id(), m = lane & 15, g = lane >> 4;
   const int rows = (int)a.rows.T;
-  if (tid < kS) sv->kbad[tid] = 0;
   constexpr int P = KP / 8, N = kS * P * 2 / 256 < 1 ? 1 : kS * P * 2 / 256;   // pieces of eight for a thread: K, then Q
   f32x8 v[N];
   float odd[N], any = 0.f;
@@ -57,6 +58,8 @@ __device__ __forceinline__ void short_prep(const DeltaArgs& a, int64_t n, int h,
     v[i] = f32x8{};
     if (r < rows && left > 0) v[i] = load8(base[w] + r * (w ? a.qs[1] : a.ks[1]) + 8 * p, left, w ? a.wide_q : a.wide_k);
   }
+  if (tid < kS) sv->kbad[tid] = 0;
+  lds_barrier();
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const int e = tid + 256 * i, w = e / (kS * P), r = e / P % kS, p = e % P;
@@ -67,16 +70,20 @@ __device__ __forceinline__ void short_prep(const DeltaArgs& a, int64_t n, int h,
 #pragma unroll
     for (int j = 0; j < NP; ++j) *reinterpret_cast<bf16x8*>(kq + (w * NP + j) * kTile + tile_at<KP>(r, p)) = pl[j];
   }
-  if (__syncthreads_or(any != 0.f)) {   // rows of k that are not finite: zeros, and marked
+  if (__ballot(any != 0.f)) {   // rows of k that are not finite: marked, and zeros
+    rare_path();
 #pragma unroll
     for (int i = 0; i < N; ++i)
       if (odd[i] != 0.f) sv->kbad[(tid + 256 * i) / P % kS] = 1;
-    __syncthreads();
+  }
+  lds_barrier();
+  if (__ballot(sv->kbad[lane % kS])) {
+    rare_path();
     for (int e = tid; e < kS * P * NP; e += 256) {
       const int r = e / (P * NP);
       if (sv->kbad[r]) *reinterpret_cast<u32x4*>(kq + e / P % NP * kTile + tile_at<KP>(r, e % P)) = u32x4{0, 0, 0, 0};
     }
-    __syncthreads();
+    lds_barrier();
   }
   if (wave == 3) {
     const bool in = lane < rows;
@@ -113,7 +120,7 @@ __device__ __forceinline__ void short_prep(const DeltaArgs& a, int64_t n, int h,
     }
   }
   mfma_settle();
-  __syncthreads();
+  lds_barrier();
   float pv[4];
   const int c = wave < 3 ? 16 * tj + m : 16 + m, r0 = wave < 3 ? 16 * ti + 4 * g : 4 * g;   // wave 3: the zeros right of the diagonal
 #pragma unroll
@@ -125,7 +132,7 @@ __device__ __forceinline__ void short_prep(const DeltaArgs& a, int64_t n, int h,
     X[row * kSld + c] = 0.f;
     pv[r] = lower ? a.scale * d * qk[r] : 0.f;
   }
-  __syncthreads();
+  lds_barrier();
   // X = (I + A)^-1, as in k_delta_prep
   if (wave == 0) {
     if (g < 2) {
@@ -157,11 +164,11 @@ __device__ __forceinline__ void short_prep(const DeltaArgs& a, int64_t n, int h,
 #pragma unroll
     for (int r = 0; r < 4; ++r) X[(16 + 4 * g + r) * kSld + m] = -z[r];
   }
-  __syncthreads();
+  lds_barrier();
   // planes of X, and of P (where A was: all of A has been read)
 #pragma unroll
   for (int r = 0; r < 4; ++r) A[(r0 + r) * kSld + c] = pv[r];
-  __syncthreads();
+  lds_barrier();
   __bf16* const xp = reinterpret_cast<__bf16*>(lds + L::xp);
   {
     const int w = tid / 128, r = tid / 4 % 32, p = tid % 4;
@@ -172,25 +179,42 @@ __device__ __forceinline__ void short_prep(const DeltaArgs& a, int64_t n, int h,
     for (int j = 0; j < 3; ++j)
       if (!w || j < L::NPP) *reinterpret_cast<bf16x8*>(xp + (w * 3 + j) * kMat + tile_at<kS>(r, p)) = pl[j];
   }
-  __syncthreads();
+  lds_barrier();
 }
 
-// A lane's rows perm_row(t, 4 g + r), t < 2, of its column: all loads in flight at once
+// Element `at` of an array that begins at a scalar address: with 32-bit offsets an access needs one register, not two (the host
+// sees to it that a sequence's rows lie within 2^30 elements)
 template <class T>
-__device__ __forceinline__ void load_rows(const T* p, int64_t stride, int rows, bool in, int g, f32x4 (&v)[2]) {
-  T raw[2][4];
-#pragma unroll
-  for (int t = 0; t < 2; ++t)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int row = perm_row(t, 4 * g + r);
-      raw[t][r] = p[(row < rows ? row : rows - 1) * stride];
-    }
-#pragma unroll
-  for (int t = 0; t < 2; ++t)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) v[t][r] = in && perm_row(t, 4 * g + r) < rows ? (float)raw[t][r] : 0.f;
+__device__ __forceinline__ T& item(T* base, uint32_t at) {
+  using Byte = std::conditional_t<std::is_const_v<T>, const char, char>;
+  return *reinterpret_cast<T*>(reinterpret_cast<Byte*>(base) + (uint32_t)(at * (uint32_t)sizeof(T)));
 }
+// perm_row(t, 4 g + r) = 8 g + step(t) + r
+__device__ constexpr int step(int t) { return 32 * (t >> 1) + 4 * (t & 1); }
+
+// A lane's rows perm_row(t, 4 g + r), t < N, of its column: fetched at addresses inside, so that no branch separates the loads,
+// and zeros outside when they are taken
+template <class T, int N>
+struct ShortRows {
+  T raw[N][4];
+  __device__ __forceinline__ void fetch(const T* p, uint32_t stride, int rows, int c, int g) {
+    const uint32_t at = 8 * g * stride + c, last = (rows - 1) * stride + c;
+#pragma unroll
+    for (int t = 0; t < N; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) raw[t][r] = item(p, min(at + (step(t) + r) * stride, last));
+  }
+  __device__ __forceinline__ void take(int rows, bool in, int g, f32x4 (&v)[N]) const {
+#pragma unroll
+    for (int t = 0; t < N; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[t][r] = in && 8 * g + step(t) + r < rows ? (float)raw[t][r] : 0.f;
+  }
+};
+
+// Offsets made from these are made where they are used: worked out once before the loop over the columns, which mostly runs
+// once, they took more registers than there are
+__device__ __forceinline__ void here(int& g, int& x) { asm volatile("" : "+v"(g), "+v"(x)); }
 
 __device__ __forceinline__ f32x4 vec4(const float* v, int t, int g) { return *reinterpret_cast<const f32x4*>(v + perm_row(t, 4 * g)); }
 
@@ -242,11 +266,25 @@ __global__ __launch_bounds__(256, 2) void k_delta_short(DeltaArgs a) {
   using T = typename Elem<DT>::T;
   constexpr int NP = L::NP, NO = L::NO, KT = L::KT;
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  const int lane = threadIdx.x & 63, wave = wave_id(), x = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = wave_id();
+  int x = lane & 15, g = lane >> 4;
   const int64_t n = blockIdx.x / a.Hv;
   const int h = (int)(blockIdx.x % a.Hv), hk = h / (a.Hv / a.Hk), rows = (int)a.rows.T;
   const int64_t head = n * a.Hv + h;
+  const float* s0 = a.initial ? a.initial + head * a.K * a.V : nullptr;
+  const T* v_in = static_cast<const T*>(a.v) + n * a.vs[0] + h * a.vs[2];
+  T* const o_out = static_cast<T*>(a.o) + ((int64_t)n * rows * a.Hv + h) * a.V;
+  float* const final = a.final + head * a.K * a.V;
+  const uint32_t orow = a.Hv * a.V;
   f32x4 kk, qk;
+  ShortRows<float, KT> sn = {};
+  ShortRows<T, 2> vn;
+  auto fetch = [&](int c0) {   // ahead of their use
+    const int c = min(c0 + x, a.V - 1);
+    if (s0) sn.fetch(s0, a.V, a.K, c, g);
+    vn.fetch(v_in, (uint32_t)a.vs[1], rows, c, g);
+  };
+  fetch(16 * wave);
   short_prep<DT, KP, false>(a, n, h, hk, lds, kk, qk);
   const __bf16* K = reinterpret_cast<const __bf16*>(lds);
   const __bf16* Q = K + NP * L::kTile;
@@ -254,12 +292,13 @@ __global__ __launch_bounds__(256, 2) void k_delta_short(DeltaArgs a) {
   const ShortVec* sv = reinterpret_cast<const ShortVec*>(lds + L::vec);
   const float nan = __builtin_nanf("");
   for (int c0 = 16 * wave; c0 < a.V; c0 += 64) {
+    here(g, x);
     const int col = c0 + x;
     const bool in = col < a.V;
     f32x4 st[KT], v[2], u[2], o[2] = {};
-#pragma unroll
-    for (int t = 0; t < KT; ++t) st[t] = load_state(a.initial ? a.initial + head * a.K * a.V : nullptr, a.K, a.V, col, t, g);
-    load_rows(static_cast<const T*>(a.v) + n * a.vs[0] + h * a.vs[2] + (in ? col : a.V - 1), a.vs[1], rows, in, g, v);
+    sn.take(a.K, in, g, st);
+    vn.take(rows, in, g, v);
+    if (c0 + 64 < a.V) fetch(c0 + 64);
     int bad;
     short_u<DT, KP, false>(lds, st, v, g, x, u, bad);
     // o = scale exp(G_i) Q S + P u
@@ -294,24 +333,20 @@ __global__ __launch_bounds__(256, 2) void k_delta_short(DeltaArgs a) {
       mfma_rows<NP, 3, 3, KT>([&](int t) -> const bf16x8(&)[NP] { return ft[t]; }, up, st);
     }
     mfma_settle();
-    T* op = static_cast<T*>(a.o) + ((int64_t)n * rows * a.Hv + h) * a.V + col;
-    const int64_t orow = (int64_t)a.Hv * a.V;
-    float* fp = a.final + head * a.K * a.V + col;
     if (in) {
+      const uint32_t oat = 8 * g * orow + col, fat = 8 * g * a.V + col;
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int row = perm_row(t, 4 * g + r);
-          if (row < rows) op[row * orow] = (T)(row >= bad ? nan : o[t][r]);
+          const int row = 8 * g + step(t) + r;
+          if (row < rows) item(o_out, oat + (step(t) + r) * orow) = (T)(row >= bad ? nan : o[t][r]);
         }
 #pragma unroll
       for (int t = 0; t < KT; ++t)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int kd = perm_row(t, 4 * g + r);
-          if (kd < a.K) fp[(int64_t)kd * a.V] = st[t][r];
-        }
+        for (int r = 0; r < 4; ++r)
+          if (8 * g + step(t) + r < a.K) item(final, fat + (step(t) + r) * a.V) = st[t][r];
     }
   }
 }
@@ -332,12 +367,30 @@ __global__ __launch_bounds__(256, 2) void k_delta_short_grad(DeltaGradArgs ga, b
   constexpr int NP = L::NP, NO = L::NO, KT = L::KT, NT = KT >= 4 ? KT / 4 : 1, kTile = L::kTile, kCol = L::kCol;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const DeltaArgs& a = ga.f;
-  const int lane = threadIdx.x & 63, wave = wave_id(), x = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = wave_id();
+  int x = lane & 15, g = lane >> 4;
   const int64_t n = blockIdx.x / a.Hv;
   const int h = (int)(blockIdx.x % a.Hv), hk = h / (a.Hv / a.Hk), rows = (int)a.rows.T;
-  const int64_t head = n * a.Hv + h, orow = (int64_t)a.Hv * a.V, first = ((int64_t)n * rows * a.Hv + h) * a.V;
+  const int64_t head = n * a.Hv + h, first = (n * rows * a.Hv + h) * a.V;
+  const uint32_t orow = a.Hv * a.V;
   const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+  const float* s0 = a.initial ? a.initial + head * a.K * a.V : nullptr;
+  const float* df = ga.d_final ? ga.d_final + head * a.K * a.V : nullptr;
+  const T* v_in = static_cast<const T*>(a.v) + n * a.vs[0] + h * a.vs[2];
+  const T* do_in = static_cast<const T*>(ga.d_o) + first;
+  float* const di_out = ga.d_initial ? ga.d_initial + head * a.K * a.V : nullptr;
+  T* const dv_out = static_cast<T*>(ga.dv) + first;
   f32x4 kk, qk;
+  ShortRows<float, KT> sn = {}, dn = {};
+  ShortRows<T, 2> vn, on;
+  auto fetch = [&](int v0) {   // ahead of their use
+    const int c = min(v0 + 16 * wave + x, a.V - 1);
+    if (s0) sn.fetch(s0, a.V, a.K, c, g);
+    if (df) dn.fetch(df, a.V, a.K, c, g);
+    vn.fetch(v_in, (uint32_t)a.vs[1], rows, c, g);
+    on.fetch(do_in, orow, rows, c, g);
+  };
+  fetch(0);
   short_prep<DT, KP, true>(a, n, h, hk, lds, kk, qk);
   const __bf16* K = reinterpret_cast<const __bf16*>(lds);
   const __bf16* Q = K + NP * kTile;
@@ -347,11 +400,35 @@ __global__ __launch_bounds__(256, 2) void k_delta_short_grad(DeltaGradArgs ga, b
   __bf16* const cu = reinterpret_cast<__bf16*>(lds + L::cols);   // planes [64 columns][32 rows] of u, dR, do
   __bf16* const cr = cu + 3 * kCol;
   __bf16* const co = cr + 3 * kCol;
-  const float* s0 = a.initial ? a.initial + head * a.K * a.V : nullptr;
-  const float* df = ga.d_final ? ga.d_final + head * a.K * a.V : nullptr;
   const float nan = __builtin_nanf("");
 
   const bool active = wave * NT < KT;
+  // rows kd of S and dS, eight columns of step s
+  f32x8 sr[NT], dr8[NT];
+  auto fetch_rows = [&](const float* p, int c, f32x8 (&to)[NT]) {
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      to[j] = f32x8{};
+      if (!p) continue;
+      const int kd = 16 * (wave * NT + j) + x, row = min(kd, a.K - 1) * a.V;
+      const bool in = active && kd < a.K;
+      if (wide_s) {
+        const f32x4 lo = *reinterpret_cast<const f32x4*>(p + row + min(c, a.V - 4));
+        const f32x4 hi = *reinterpret_cast<const f32x4*>(p + row + min(c + 4, a.V - 4));
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          to[j][r] = in && c < a.V ? lo[r] : 0.f;
+          to[j][4 + r] = in && c + 4 < a.V ? hi[r] : 0.f;
+        }
+      } else {
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          const float one = p[row + min(c + r, a.V - 1)];
+          to[j][r] = in && c + r < a.V ? one : 0.f;
+        }
+      }
+    }
+  };
   f32x4 X1[2][NT], Y[2][NT], Z[2][NT], M = zero, N = zero;
   float rv[2][4] = {}, dot = 0.f;
 #pragma unroll
@@ -360,18 +437,15 @@ __global__ __launch_bounds__(256, 2) void k_delta_short_grad(DeltaGradArgs ga, b
     for (int j = 0; j < NT; ++j) X1[i][j] = Y[i][j] = Z[i][j] = zero;
 
   for (int v0 = 0; v0 < a.V; v0 += 64) {
+    here(g, x);
     const int col = v0 + 16 * wave + x;
     const bool in = col < a.V;
     if (v0 + 16 * wave < a.V) {
       f32x4 st[KT], ds[KT], v[2], d[2], u[2], du[2], dr[2] = {zero, zero};
-#pragma unroll
-      for (int t = 0; t < KT; ++t) {
-        st[t] = load_state(s0, a.K, a.V, col, t, g);
-        ds[t] = load_state(df, a.K, a.V, col, t, g);
-      }
-      const int c = in ? col : a.V - 1;
-      load_rows(static_cast<const T*>(a.v) + n * a.vs[0] + h * a.vs[2] + c, a.vs[1], rows, in, g, v);
-      load_rows(static_cast<const T*>(ga.d_o) + first + c, orow, rows, in, g, d);
+      sn.take(a.K, in, g, st);
+      dn.take(a.K, in, g, ds);
+      vn.take(rows, in, g, v);
+      on.take(rows, in, g, d);
       int bad;
       short_u<DT, KP, true>(lds, st, v, g, x, u, bad);
       mfma_settle();
@@ -423,14 +497,14 @@ __global__ __launch_bounds__(256, 2) void k_delta_short_grad(DeltaGradArgs ga, b
         const f32x4 dv = vec4(sv->beta, t, g) * dr[t];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int row = perm_row(t, 4 * g + r);
+          const int row = 8 * g + step(t) + r;
           rv[t][r] = fmaf(dr[t][r], v[t][r], rv[t][r]);
-          if (in && row < rows) static_cast<T*>(ga.dv)[first + row * orow + col] = (T)dv[r];
+          if (in && row < rows) item(dv_out, 8 * g * orow + col + (step(t) + r) * orow) = (T)dv[r];
         }
         d[t] *= a.scale * vec4(sv->into, t, g);
         dr[t] = -vec4(sv->into, t, g) * dv;
       }
-      if (ga.d_initial) {
+      if (di_out) {
         bf16x8 ep[3], rp[3];
         planes8<3>(cat8(d[0], d[1]), ep);
         planes8<3>(cat8(dr[0], dr[1]), rp);
@@ -448,8 +522,7 @@ __global__ __launch_bounds__(256, 2) void k_delta_short_grad(DeltaGradArgs ga, b
         for (int t = 0; t < KT; ++t)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const int kd = perm_row(t, 4 * g + r);
-            if (in && kd < a.K) ga.d_initial[(head * a.K + kd) * a.V + col] = ds[t][r];
+            if (in && 8 * g + step(t) + r < a.K) item(di_out, 8 * g * a.V + col + (step(t) + r) * a.V) = ds[t][r];
           }
       }
     } else {
@@ -457,52 +530,50 @@ __global__ __launch_bounds__(256, 2) void k_delta_short_grad(DeltaGradArgs ga, b
 #pragma unroll
       for (int j = 0; j < 6 + NP; ++j) *reinterpret_cast<bf16x8*>(cu + j * kCol + tile_at<kS>(16 * wave + x, g)) = none;
     }
-    __syncthreads();
+    here(g, x);
+    fetch_rows(s0, v0 + 8 * g, sr);
+    fetch_rows(df, v0 + 8 * g, dr8);
+    lds_barrier();
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      bf16x8 fo[2][NP], fr[2][3], fu[2][3];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        frag_col<kS, NP, kCol>(co, i, s, g, x, fo[i]);
-        frag_col<kS, 3, kCol>(cr, i, s, g, x, fr[i]);
-        frag_col<kS, 3, kCol>(cu, i, s, g, x, fu[i]);
+      if (s == 1) {
+        fetch_rows(s0, v0 + 32 + 8 * g, sr);
+        fetch_rows(df, v0 + 32 + 8 * g, dr8);
       }
       if (wave < 3) {   // the tile of kk and qk
-        if (wave == 0) {
-          M = mfma_planes<NP, 3, 3>(fo[0], fu[0], M);
-          N = mfma_planes<3, 3, 3>(fr[0], fu[0], N);
-        } else if (wave == 1) {
-          M = mfma_planes<NP, 3, 3>(fo[1], fu[0], M);
-          N = mfma_planes<3, 3, 3>(fr[1], fu[0], N);
-        } else {
-          M = mfma_planes<NP, 3, 3>(fo[1], fu[1], M);
-          N = mfma_planes<3, 3, 3>(fr[1], fu[1], N);
-        }
+        bf16x8 fo[NP], fr[3], fu[3];
+        frag_col<kS, NP, kCol>(co, wave > 0, s, g, x, fo);
+        frag_col<kS, 3, kCol>(cr, wave > 0, s, g, x, fr);
+        frag_col<kS, 3, kCol>(cu, wave > 1, s, g, x, fu);
+        M = mfma_planes<NP, 3, 3>(fo, fu, M);
+        N = mfma_planes<3, 3, 3>(fr, fu, N);
       }
       if (active) {
-        const int c = v0 + 32 * s + 8 * g, left = a.V - c;
+        bf16x8 sp[NT][3], dp[NT][3];
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-          const int kd = 16 * (wave * NT + j) + x;
-          f32x8 sr = {}, dr = {};
-          if (left > 0 && kd < a.K) {
-            if (s0) sr = load8(s0 + (int64_t)kd * a.V + c, left, wide_s);
-            if (df) dr = load8(df + (int64_t)kd * a.V + c, left, wide_s);
-          }
-          bf16x8 sp[3], dp[3];
-          planes8<3>(sr, sp);
-          planes8<3>(dr, dp);
+          planes8<3>(sr[j], sp[j]);
+          planes8<3>(dr8[j], dp[j]);
+        }
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            X1[i][j] = mfma_planes<NP, 3, 3>(fo[i], sp, X1[i][j]);
-            Y[i][j] = mfma_planes<3, 3, 3>(fr[i], sp, Y[i][j]);
-            Z[i][j] = mfma_planes<3, 3, 3>(fu[i], dp, Z[i][j]);
+        for (int i = 0; i < 2; ++i) {   // one row tile's operands at a time: more do not fit in the registers
+          bf16x8 fo[NP], fr[3], fu[3];
+          frag_col<kS, NP, kCol>(co, i, s, g, x, fo);
+          frag_col<kS, 3, kCol>(cr, i, s, g, x, fr);
+          frag_col<kS, 3, kCol>(cu, i, s, g, x, fu);
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            X1[i][j] = mfma_planes<NP, 3, 3>(fo, sp[j], X1[i][j]);
+            Y[i][j] = mfma_planes<3, 3, 3>(fr, sp[j], Y[i][j]);
+            Z[i][j] = mfma_planes<3, 3, 3>(fu, dp[j], Z[i][j]);
           }
+          __builtin_amdgcn_sched_barrier(0);
         }
       }
     }
     mfma_settle();
-    __syncthreads();   // the next columns, or m and n, go where these were
+    if (v0 + 64 < a.V) fetch(v0 + 64);
+    lds_barrier();   // the next columns, or m and n, go where these were
   }
 
   float* const qx = reinterpret_cast<float*>(lds + L::sums);   // by wave and row: q . X, k . Y, k . Z, dR . v
@@ -579,8 +650,11 @@ __global__ __launch_bounds__(256, 2) void k_delta_short_grad(DeltaGradArgs ga, b
         kz[wave * kS + row] = sz;
       }
     }
-  __syncthreads();
+  lds_barrier();
   if (active) {
+    const int64_t at32 = (n * rows * a.Hv + h) * a.K, at16 = (n * rows * a.Hk + hk) * a.K;
+    float *const dq32 = ga.dq32 + at32, *const dk32 = ga.dk32 + at32;
+    T *const dq = static_cast<T*>(ga.dq) + at16, *const dk = static_cast<T*>(ga.dk) + at16;
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       bf16x8 kb[NP], qb[NP];
@@ -610,13 +684,13 @@ __global__ __launch_bounds__(256, 2) void k_delta_short_grad(DeltaGradArgs ga, b
           const int kd = 16 * (wave * NT + j) + x;
           if (row >= rows || kd >= a.K) continue;
           if (ga.dq32) {
-            const int64_t at = ((n * rows + row) * a.Hv + h) * a.K + kd;
-            ga.dq32[at] = X1[i][j][r];
-            ga.dk32[at] = Y[i][j][r];
+            const uint32_t at = row * (uint32_t)(a.Hv * a.K) + kd;
+            item(dq32, at) = X1[i][j][r];
+            item(dk32, at) = Y[i][j][r];
           } else {
-            const int64_t at = ((n * rows + row) * a.Hk + hk) * a.K + kd;
-            static_cast<T*>(ga.dq)[at] = (T)X1[i][j][r];
-            static_cast<T*>(ga.dk)[at] = (T)Y[i][j][r];
+            const uint32_t at = row * (uint32_t)(a.Hk * a.K) + kd;
+            item(dq, at) = (T)X1[i][j][r];
+            item(dk, at) = (T)Y[i][j][r];
           }
         }
       }
