@@ -2,6 +2,8 @@
 #pragma once
 #include "seq_delta.hpp"
 
+#include <type_traits>
+
 namespace seq {
 namespace {
 
@@ -58,6 +60,17 @@ __device__ __forceinline__ float add_turned(float v) {
   return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x120 + N, 0xf, 0xf, false));
 }
 __device__ __forceinline__ float sum16(float v) { return add_turned<1>(add_turned<2>(add_turned<4>(add_turned<8>(v)))); }
+
+// Offsets made from these are made where they are used: worked out once before a loop they take more registers than there are
+__device__ __forceinline__ void here(int& g, int& x) { asm volatile("" : "+v"(g), "+v"(x)); }
+
+// Element `at` of an array that begins at a scalar address: with 32-bit offsets an access needs one register, not two.  at times
+// the element's size is below 2^32
+template <class T>
+__device__ __forceinline__ T& item(T* base, uint32_t at) {
+  using Byte = std::conditional_t<std::is_const_v<T>, const char, char>;
+  return *reinterpret_cast<T*>(reinterpret_cast<Byte*>(base) + (uint32_t)(at * (uint32_t)sizeof(T)));
+}
 
 // keeps a branch around what hardly ever runs (the compiler would rather run both sides and select)
 __device__ __forceinline__ void rare_path() { asm volatile(""); }

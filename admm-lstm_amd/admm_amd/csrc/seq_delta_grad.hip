@@ -305,7 +305,7 @@ __device__ __forceinline__ float whole(const __bf16* p) {
 }
 
 template <int DT, int KP, int C>
-__global__ __launch_bounds__(4 * C) void k_delta_grad(DeltaGradArgs ga, bool wide_v, bool wide_o) {
+__global__ __launch_bounds__(4 * C, C == 64 ? 2 : 1) void k_delta_grad(DeltaGradArgs ga, bool wide_v, bool wide_o) {
   using S = DeltaShape<DT, KP, C, true>;
   using L = GradLds<DT, KP, C>;
   using T = typename Elem<DT>::T;
@@ -325,7 +325,8 @@ __global__ __launch_bounds__(4 * C) void k_delta_grad(DeltaGradArgs ga, bool wid
   float *const rv = ghi + 5 * C, *const cols = ghi + 6 * C, *const rsum = ghi + 7 * C, *const rnb = rsum + RT * C;
   float *const qx = rnb + RT * C, *const ky = qx + RT * C, *const kz = ky + RT * C, *const sds = kz + RT * C;
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = wave_id(), x = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
+  int x = lane & 15, g = lane >> 4;
   const int64_t c = blockIdx.x / a.Hv;
   const int h = (int)(blockIdx.x % a.Hv), hk = h / (a.Hv / a.Hk);
   const int64_t n = a.rows.find(c);
@@ -383,6 +384,16 @@ __global__ __launch_bounds__(4 * C) void k_delta_grad(DeltaGradArgs ga, bool wid
     for (int v0 = 0; v0 < a.VP; v0 += kSlice) {
       const int lv = a.V - v0 - 8 * p;
       f32x8 dov = {}, drv = {}, uv = {}, vv = {};
+      here(g, x);
+      f32x8 sv[NT] = {}, dv[NT] = {};
+      if (active && v0 + 8 * g < a.VP) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          const uint32_t o = (16 * (wave * NT + j) + x) * a.VP + v0 + 8 * g;
+          sv[j] = load8(&item(s0, o), 8, true);
+          dv[j] = load8(&item(dse, o), 8, true);
+        }
+      }
       if (v0 + 8 * p < a.VP) {
         drv = load8(rp + v0, 8, true);
         uv = load8(up + v0, 8, true);
@@ -394,7 +405,7 @@ __global__ __launch_bounds__(4 * C) void k_delta_grad(DeltaGradArgs ga, bool wid
 #pragma unroll
       for (int i = 0; i < 8; ++i) rdot = fmaf(drv[i], vv[i], rdot);
       bf16x8 po[NP], p3[3];
-      __syncthreads();   // the last slice is done with
+      lds_barrier();   // the last slice is done with
       planes8<NP>(dov, po);
 #pragma unroll
       for (int i = 0; i < NP; ++i) *reinterpret_cast<bf16x8*>(dO + i * kST + at) = po[i];
@@ -404,23 +415,17 @@ __global__ __launch_bounds__(4 * C) void k_delta_grad(DeltaGradArgs ga, bool wid
       planes8<3>(uv, p3);
 #pragma unroll
       for (int i = 0; i < 3; ++i) *reinterpret_cast<bf16x8*>(uu + i * kST + at) = p3[i];
-      __syncthreads();
+      lds_barrier();
       bf16x8 fu[3];
       frag<kSlice, 3, kST>(uu, 16 * wave + x, 0, g, fu);
       bf16x8 sp[NT][3], dp[NT][3];
       if (active) {
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-          f32x8 sv = {}, dv = {};
-          if (v0 + 8 * g < a.VP) {
-            const int64_t o = (int64_t)(16 * (wave * NT + j) + x) * a.VP + v0 + 8 * g;
-            sv = load8(s0 + o, 8, true);
-            dv = load8(dse + o, 8, true);
-          }
 #pragma unroll
-          for (int i = 0; i < 8; ++i) dot = fmaf(sv[i], dv[i], dot);
-          planes8<3>(sv, sp[j]);
-          planes8<3>(dv, dp[j]);
+          for (int i = 0; i < 8; ++i) dot = fmaf(sv[j][i], dv[j][i], dot);
+          planes8<3>(sv[j], sp[j]);
+          planes8<3>(dv[j], dp[j]);
         }
       }
 #pragma unroll
@@ -441,6 +446,7 @@ __global__ __launch_bounds__(4 * C) void k_delta_grad(DeltaGradArgs ga, bool wid
             Z[i][j] = mfma_planes<3, 3, 3>(fi, dp[j], Z[i][j]);
           }
         }
+        __builtin_amdgcn_sched_barrier(0);   // (the next row tile's operands would not fit in the registers too)
       }
     }
   }
@@ -450,8 +456,9 @@ __global__ __launch_bounds__(4 * C) void k_delta_grad(DeltaGradArgs ga, bool wid
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) dot += __shfl_xor(dot, d);
   if (lane == 0) sds[wave] = dot;
-  __syncthreads();   // K and Q are in; the staged values are done with
+  lds_barrier();   // K and Q are in; the staged values are done with
 
+  here(g, x);
   // m and n: the lane's column j = 16 wave + x, rows 16 i + 4 g..+3
   {
     const int j = 16 * wave + x;
@@ -503,8 +510,9 @@ __global__ __launch_bounds__(4 * C) void k_delta_grad(DeltaGradArgs ga, bool wid
     csum += __shfl_xor(csum, 32);
     if (g == 0) cols[j] = csum;
   }
-  __syncthreads();
+  lds_barrier();
 
+  here(g, x);
   // dq and dk: the lane's column 16 (wave NT + j) + x, rows 16 i + 4 g..+3
 #pragma unroll
   for (int i = 0; i < RT; ++i)
@@ -581,7 +589,7 @@ __global__ __launch_bounds__(4 * C) void k_delta_grad(DeltaGradArgs ga, bool wid
         }
       }
   }
-  __syncthreads();
+  lds_barrier();
   if (wave == 0) {
     const int at = lane < C ? lane : 0;
     auto waves = [&](const float* p) {

@@ -10,8 +10,6 @@
 // rows, 4 heads of 64 x 64, f32, forward and backward: 1.15 ms through work memory.
 #include "seq_delta_dev.hpp"
 
-#include <type_traits>
-
 namespace seq {
 namespace {
 
@@ -182,13 +180,6 @@ __device__ __forceinline__ void short_prep(const DeltaArgs& a, int64_t n, int h,
   lds_barrier();
 }
 
-// Element `at` of an array that begins at a scalar address: with 32-bit offsets an access needs one register, not two (the host
-// sees to it that a sequence's rows lie within 2^30 elements)
-template <class T>
-__device__ __forceinline__ T& item(T* base, uint32_t at) {
-  using Byte = std::conditional_t<std::is_const_v<T>, const char, char>;
-  return *reinterpret_cast<T*>(reinterpret_cast<Byte*>(base) + (uint32_t)(at * (uint32_t)sizeof(T)));
-}
 // perm_row(t, 4 g + r) = 8 g + step(t) + r
 __device__ constexpr int step(int t) { return 32 * (t >> 1) + 4 * (t & 1); }
 
@@ -211,10 +202,6 @@ struct ShortRows {
       for (int r = 0; r < 4; ++r) v[t][r] = in && 8 * g + step(t) + r < rows ? (float)raw[t][r] : 0.f;
   }
 };
-
-// Offsets made from these are made where they are used: worked out once before the loop over the columns, which mostly runs
-// once, they took more registers than there are
-__device__ __forceinline__ void here(int& g, int& x) { asm volatile("" : "+v"(g), "+v"(x)); }
 
 __device__ __forceinline__ f32x4 vec4(const float* v, int t, int g) { return *reinterpret_cast<const f32x4*>(v + perm_row(t, 4 * g)); }
 
