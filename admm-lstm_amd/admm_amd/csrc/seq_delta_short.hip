@@ -6,8 +6,11 @@
 // time costs less than writing and reading it back) and goes on to the gradients; what it sums over the value axis passes
 // through LDS 64 columns at a time.
 //
-// Bound by memory where there are many sequences: each input read and each result written once a pass.  2048 windows of 32
-// rows, 4 heads of 64 x 64, f32, forward and backward: 1.15 ms through work memory.
+// Bound by the latency of the chain of products, two to four waves on a SIMD; what had cost most was registers spilled to
+// scratch memory (offsets that the compiler worked out before the loops).  f32, forward and forward with backward, in us, against
+// the kernels over chunks of 32 rows with their work memory: 2048 sequences of 32 rows, 4 heads of 64 x 64: 144 and 550 (321 and
+// 1024); 1024 of 32 rows, 4 heads of 128 x 128: 210 and 946 (493 and 1565); 256 of them, V = 512: 184 and 736 (405 and 1333);
+// 1024 of 8 rows: 184 and 887 (475 and 1517); 8 sequences: 10 (14).  At memory's rate the first would take 50 and 210.
 #include "seq_delta_dev.hpp"
 
 namespace seq {
@@ -347,8 +350,9 @@ __device__ __forceinline__ float joined(const __bf16* p) {
 }
 
 // Names as in k_delta_back and k_delta_grad.
+// K = 128: one wave a SIMD, with the registers of two (two of them spilled 230 registers each, and took 2197 for 946 us)
 template <int DT, int KP>
-__global__ __launch_bounds__(256, 2) void k_delta_short_grad(DeltaGradArgs ga, bool wide_s) {
+__global__ __launch_bounds__(256, KP == 128 ? 1 : 2) void k_delta_short_grad(DeltaGradArgs ga, bool wide_s) {
   using L = ShortLds<DT, KP, true>;
   using T = typename Elem<DT>::T;
   constexpr int NP = L::NP, NO = L::NO, KT = L::KT, NT = KT >= 4 ? KT / 4 : 1, kTile = L::kTile, kCol = L::kCol;

@@ -95,6 +95,7 @@ int delta_sizes(const SeqDelta* d, bool saved, DeltaSizes& z) {
   z.KP = d->K <= 32 ? 32 : d->K <= 64 ? 64 : 128;
   // sequences of at most 32 rows (or packed ones of at most 32 on average) would leave half of a 64-row chunk empty
   z.C = d->T <= 32 || (d->offsets && d->T <= 32 * d->sequences) ? 32 : 64;
+  // (faster in every size tried, seq_delta_short.hip; it works with 32-bit offsets within a sequence)
   z.brief = !d->offsets && d->T > 0 && d->T <= 32 && std::max({d->v_stride[1], (int64_t)d->Hv * d->V, (int64_t)d->Hv * d->K}) < 1 << 25;
   const int NP = d->dtype + 1, NO = d->dtype == SEQ_FP32 ? 3 : 2, tri = z.C == 64 ? 6 : 2;
   z.per = (d->T + z.C - 1) / z.C;
