@@ -9,11 +9,13 @@ i,f,g,o, then out [H,O]; then ``xavier_normal_`` over ``parameters()``), so
 gfx950 time-step kernel of libadmmlstm.so (``admm_forward``); they require HIP
 device tensors.  ``with_grad=True`` (``blocks/lstm.py:48-63``) is the autograd
 path the reference uses for its gradient-descent baselines; it is plain PyTorch.
+There ``dropout=p`` drops part of h_T before the output layer while the model trains
+(``blocks/dropout.py``); 0, the default, changes nothing.
 """
 from __future__ import annotations
 
 import ctypes
-from typing import Dict
+from typing import Dict, Union
 
 import torch
 from torch import nn
@@ -23,12 +25,17 @@ GATES4 = ('i', 'f', 'g', 'o')
 
 
 class LSTM(nn.Module):
-    def __init__(self, input_size: int, hidden_size: int, output_size: int, with_grad: bool = False) -> None:
+    def __init__(self, input_size: int, hidden_size: int, output_size: int, with_grad: bool = False,
+                 *, dropout: float = 0.0) -> None:
         super().__init__()
+        if not 0.0 <= dropout <= 1.0:
+            raise ValueError(f'dropout must be between 0 and 1 (got {dropout})')
+        if dropout and not with_grad:
+            raise ValueError('dropout needs with_grad=True: the other paths have no training mode')
         self.input_size, self.hidden_size, self.output_size = input_size, hidden_size, output_size
         self.init_parameters()
         self.sigmoid, self.tanh = nn.Sigmoid(), nn.Tanh()
-        self.with_grad = with_grad
+        self.with_grad, self.dropout = with_grad, dropout
 
     def init_parameters(self) -> None:
         D, H, O = self.input_size, self.hidden_size, self.output_size
@@ -53,14 +60,17 @@ class LSTM(nn.Module):
         self.out = nn.Parameter(value)
 
     # -- forward
-    def forward(self, x: torch.Tensor, c: torch.Tensor = None, h: torch.Tensor = None) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, c: torch.Tensor = None, h: torch.Tensor = None,
+                *, dropout_seed: Union[int, torch.Tensor, None] = None) -> torch.Tensor:
+        """``dropout_seed``: of the dropped values' mask (blocks/dropout.py); None draws one from torch's generator."""
         if self.with_grad:
-            return self.grad_forward(x, c, h)
+            return self.grad_forward(x, c, h, dropout_seed=dropout_seed)
         if c is None and h is None:
             return _native_predict(self, x)
         return self.init_gate_variables(x, c, h)['a']
 
-    def grad_forward(self, x: torch.Tensor, c: torch.Tensor = None, h: torch.Tensor = None) -> torch.Tensor:
+    def grad_forward(self, x: torch.Tensor, c: torch.Tensor = None, h: torch.Tensor = None,
+                     *, dropout_seed: Union[int, torch.Tensor, None] = None) -> torch.Tensor:
         assert x.size(2) == self.input_size
         B, T, _ = x.shape
         c = torch.zeros(B, self.hidden_size, dtype=x.dtype, device=x.device) if c is None else c
@@ -70,6 +80,10 @@ class LSTM(nn.Module):
             pre = {q: xt @ getattr(self, f'x2{q}') + h @ getattr(self, f'h2{q}') for q in GATES4}
             c = self.sigmoid(pre['f']) * c + self.sigmoid(pre['i']) * self.tanh(pre['g'])
             h = self.sigmoid(pre['o']) * self.tanh(c)
+        if self.training and self.dropout:
+            from blocks.dropout import dropout
+            seed = int(torch.randint(2 ** 63 - 1, ())) if dropout_seed is None else dropout_seed
+            h = dropout(h, self.dropout, seed)
         return h @ self.out
 
     @torch.no_grad()

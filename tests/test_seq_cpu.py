@@ -179,7 +179,20 @@ def test_unit_refuses_host_tensors_and_bad_c_calls():
     bad(b'weights', D=0)
     bad(b'weights', F=(1 << 20) + 1)
     bad(b'too many', M=(1 << 31) - 1, F=1 << 20)
-    u = N.SeqUnit(M=4, D=7, F=7, x_ld=7, wg_ld=7, wu_ld=7)
+    u = N.SeqUnit(M=40, D=7, F=7, x_ld=7, wg_ld=7, wu_ld=7)   # (up to 32 rows need no work memory)
     assert lib.seq_unit_workspace(ctypes.byref(u), 1, ctypes.byref(n)) == 0 and n.value > 0
     assert lib.seq_unit_forward(ctypes.byref(u), None, 0, None, None, None) == -1 and b'work memory' in lib.seq_last_error()
     assert lib.seq_unit_backward(ctypes.byref(u), 256, n.value, None, None, 7, None, None, None, None) == -1
+
+
+def test_lstm_dropout_refusals_and_default():
+    from blocks.lstm import LSTM
+    for kw, said in ((dict(with_grad=True, dropout=1.5), 'between 0 and 1'), (dict(dropout=0.5), 'with_grad')):
+        with pytest.raises(ValueError, match=said):
+            LSTM(3, 4, 1, **kw)
+    torch.manual_seed(0)
+    a = LSTM(3, 4, 1, with_grad=True)
+    torch.manual_seed(0)
+    b = LSTM(3, 4, 1, with_grad=True, dropout=0.5).eval()
+    x = torch.randn(2, 5, 3)
+    assert torch.equal(a(x), b(x)) and list(a.state_dict()) == list(b.state_dict())
