@@ -68,6 +68,16 @@ __global__ __launch_bounds__(4 * C, DT == SEQ_FP32 ? 2 : 3) void k_delta_prep(De
   const int rows = (int)(len - t0 < C ? len - t0 : C);
   const int64_t bt = a.rows.batch(n), r0 = begin + t0;
 
+  // the first head's decays and strengths; later ones are fetched while the one before is worked on
+  const bool own = wave == 0 && lane < rows;
+  float gn = 0.f, bn = 0.f;
+  auto fetch = [&](int h) {
+    gn = own ? a.g[bt * a.gs[0] + (r0 + lane) * a.gs[1] + h * a.gs[2]] : 0.f;
+    bn = own ? a.beta[bt * a.bs[0] + (r0 + lane) * a.bs[1] + h * a.bs[2]] : 0.f;
+  };
+  const int group = a.Hv / a.Hk;
+  fetch(hk * group);
+
   // K and Q rows as planes in LDS
   {
     constexpr int N = C * (KP / 8) / kThreads;   // pieces of eight of each, for a thread
@@ -84,6 +94,8 @@ __global__ __launch_bounds__(4 * C, DT == SEQ_FP32 ? 2 : 3) void k_delta_prep(De
         v[1][i] = load8(qp + r * a.qs[1] + 8 * p, left, a.wide_q);
       }
     }
+    if (tid < C) kbad[tid] = 0;
+    lds_barrier();
     float odd[N], any = 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -98,12 +110,15 @@ __global__ __launch_bounds__(4 * C, DT == SEQ_FP32 ? 2 : 3) void k_delta_prep(De
         for (int j = 0; j < NP; ++j) *reinterpret_cast<bf16x8*>(kq + (w * NP + j) * kTile + tile_at<KP>(r, p)) = pl[j];
       }
     }
-    if (tid < C) kbad[tid] = 0;
-    if (__syncthreads_or(any != 0.f)) {   // rows of k that are not finite: zeros, and marked
+    if (__ballot(any != 0.f)) {   // rows of k that are not finite: marked, and zeros
+      rare_path();
 #pragma unroll
       for (int i = 0; i < N; ++i)
         if (odd[i] != 0.f) kbad[tid / (KP / 8) + i * (kThreads / (KP / 8))] = 1;
-      __syncthreads();
+    }
+    lds_barrier();
+    if (__ballot(kbad[lane % C])) {
+      rare_path();
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const int r = tid / (KP / 8) + i * (kThreads / (KP / 8));
@@ -111,7 +126,7 @@ __global__ __launch_bounds__(4 * C, DT == SEQ_FP32 ? 2 : 3) void k_delta_prep(De
 #pragma unroll
         for (int j = 0; j < NP; ++j) *reinterpret_cast<u32x4*>(kq + j * kTile + tile_at<KP>(r, p)) = u32x4{0, 0, 0, 0};
       }
-      __syncthreads();
+      lds_barrier();
     }
   }
   // their fragments
@@ -150,14 +165,11 @@ __global__ __launch_bounds__(4 * C, DT == SEQ_FP32 ? 2 : 3) void k_delta_prep(De
   }
   mfma_settle();
 
-  const int group = a.Hv / a.Hk;
   for (int e = 0; e < group; ++e) {
     const int h = hk * group + e;
     const int64_t ch = c * a.Hv + h;
     if (wave == 0) {
-      const bool in = lane < rows;
-      float gv = in ? a.g[bt * a.gs[0] + (r0 + lane) * a.gs[1] + h * a.gs[2]] : 0.f;
-      float bv = in ? a.beta[bt * a.bs[0] + (r0 + lane) * a.bs[1] + h * a.bs[2]] : 0.f;
+      float gv = gn, bv = bn;
       gv = gv < kMinG ? kMinG : gv;
       const uint64_t odd = __ballot((gv - gv) + (bv - bv) != 0.f || (lane < C && kbad[lane < C ? lane : 0]));
       const int bad = odd ? __ffsll((unsigned long long)odd) - 1 : C;
@@ -176,7 +188,8 @@ __global__ __launch_bounds__(4 * C, DT == SEQ_FP32 ? 2 : 3) void k_delta_prep(De
       vec[128 + lane] = bv;
       vec[192 + lane] = lane == 1 ? (float)bad : expf((float)last);
     }
-    __syncthreads();   // and K, Q (first round) or the last head's tiles are done with
+    lds_barrier();   // and K, Q (first round) or the last head's tiles are done with
+    if (e + 1 < group) fetch(h + 1);
     float pv[S::RT][4];
 #pragma unroll
     for (int j = 0; j < S::RT; ++j)
@@ -189,7 +202,7 @@ __global__ __launch_bounds__(4 * C, DT == SEQ_FP32 ? 2 : 3) void k_delta_prep(De
         X[row * kLd + col] = 0.f;
         pv[j][r] = lower ? a.scale * d * qk[j][r] : 0.f;
       }
-    __syncthreads();
+    lds_barrier();
     // X = (I + A)^-1: the diagonal 16 x 16 blocks by substitution (a lane has one column), then joined in pairs
     if (wave == 0 && g < S::RT) {
       float x[16];
@@ -209,25 +222,25 @@ __global__ __launch_bounds__(4 * C, DT == SEQ_FP32 ? 2 : 3) void k_delta_prep(De
 #pragma unroll
       for (int i = 0; i < 16; ++i) X[(16 * g + i) * kLd + 16 * g + m] = x[i];
     }
-    __syncthreads();
+    lds_barrier();
     if (wave < C / 32) {   // [X11 0; -X22 A21 X11  X22], 16 rows each
       const f32x4 y = mm16(A + (32 * wave + 16) * kLd + 32 * wave, kLd, X + 32 * wave * kLd + 32 * wave, kLd, 1, lane);
 #pragma unroll
       for (int r = 0; r < 4; ++r) Y[(16 * wave + 4 * g + r) * kLdY + m] = y[r];
     }
-    __syncthreads();
+    lds_barrier();
     if (wave < C / 32) {
       const f32x4 z = mm16(X + (32 * wave + 16) * kLd + 32 * wave + 16, kLd, Y + 16 * wave * kLdY, kLdY, 1, lane);
 #pragma unroll
       for (int r = 0; r < 4; ++r) X[(32 * wave + 16 + 4 * g + r) * kLd + 32 * wave + m] = -z[r];
     }
-    __syncthreads();
+    lds_barrier();
     if constexpr (C == 64) {   // the same of 32 rows each, a wave has one 16 x 16 tile
       const int ti = wave >> 1, tj = wave & 1;
       const f32x4 y = mm16(A + (32 + 16 * ti) * kLd, kLd, X + 16 * tj, kLd, 2, lane);
 #pragma unroll
       for (int r = 0; r < 4; ++r) Y[(16 * ti + 4 * g + r) * kLdY + 16 * tj + m] = y[r];
-      __syncthreads();
+      lds_barrier();
       const f32x4 z = mm16(X + (32 + 16 * ti) * kLd + 32, kLd, Y + 16 * tj, kLdY, 2, lane);
 #pragma unroll
       for (int r = 0; r < 4; ++r) X[(32 + 16 * ti + 4 * g + r) * kLd + 16 * tj + m] = -z[r];
@@ -237,7 +250,7 @@ __global__ __launch_bounds__(4 * C, DT == SEQ_FP32 ? 2 : 3) void k_delta_prep(De
     for (int j = 0; j < S::RT; ++j)
 #pragma unroll
       for (int r = 0; r < 4; ++r) A[(16 * wave + 4 * g + r) * kLd + 16 * j + m] = pv[j][r];
-    __syncthreads();
+    lds_barrier();
     char* dst = a.xp + ch * (int64_t)S::kXP + lane * 16;
     // a fragment's tile and inner step: rows (kind 0, 1: X, P) or columns (2, 3: X^T, P^T)
     auto cut = [&](auto np, auto transposed, const float* mat, int first, int f) {
@@ -260,7 +273,7 @@ __global__ __launch_bounds__(4 * C, DT == SEQ_FP32 ? 2 : 3) void k_delta_prep(De
         else cut(std::integral_constant<int, 3>(), std::true_type(), A, S::pPT, f - S::TRI);
       }
     }
-    if (e + 1 < group) __syncthreads();   // before the next head's sums and tiles
+    if (e + 1 < group) lds_barrier();   // before the next head's sums and tiles
   }
 }
 
