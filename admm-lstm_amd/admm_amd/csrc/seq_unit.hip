@@ -10,6 +10,8 @@
 // Bound by the matrix cores where the layer is wide (12 M D F operations a training step), by the weights where there are few
 // rows.  f32 operands are split into three bf16 planes by a pass before (six products, seq_dev.hpp), and 16-bit operands whose
 // rows are not 16-byte aligned are copied to padded rows.
+#include <type_traits>
+
 #include "seq_gemm.hpp"
 #include "seq_unit.hpp"
 #include "seq_unit_act.hpp"
@@ -64,8 +66,8 @@ __device__ __forceinline__ void store4(T* p, f32x4 v, int n, bool wide) {
   }
 }
 
-template <int DT, int WM, int WN, int MT, int NT, bool KEEP>
-__global__ __launch_bounds__(64 * WM * WN) void k_unit(GemmArgs g, int kind, typename Elem<DT>::T* y, float* pre, bool wide) {
+template <int DT, int ACT, int WM, int WN, int MT, int NT, bool KEEP>
+__global__ __launch_bounds__(64 * WM * WN) void k_unit(GemmArgs g, typename Elem<DT>::T* y, float* pre, bool wide) {
   using G = Gemm<DT, WM, WN, MT, NT, true, false, true, false>;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lane = threadIdx.x & 63, wave = wave_id(), x = lane & 15, q = lane >> 4, wm = wave / WN, wn = wave % WN;
@@ -84,7 +86,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_unit(GemmArgs g, int kind, typ
       const f32x4 a = acc[i][j], b = acc[i][j + NT / 2];
       f32x4 r;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) r[e] = act(kind, a[e]) * b[e];
+      for (int e = 0; e < 4; ++e) r[e] = act(ACT, a[e]) * b[e];
       const int64_t at = (int64_t)row * g.N + col;
       store4(y + at, r, n, wide);
       if (KEEP) {
@@ -119,7 +121,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_unit_gemm(GemmArgs g, typename
 }
 
 // da = dy b act'(a), db = dy act(a), as rows of F8 values (f32: planes)
-template <int DT>
+template <int DT, int ACT>
 __global__ __launch_bounds__(256) void k_unit_back(UnitArgs u) {
   using T = typename Elem<DT>::T;
   const int64_t pieces = u.F8 / 8, all = u.M * pieces, plane = u.M * u.F8, MF = (int64_t)u.M * u.F;
@@ -135,7 +137,7 @@ __global__ __launch_bounds__(256) void k_unit_back(UnitArgs u) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       float f, df;
-      act_grad(u.act, a[j], f, df);
+      act_grad(ACT, a[j], f, df);
       da[j] = j < left ? d[j] * b[j] * df : 0.f;
       db[j] = j < left ? d[j] * f : 0.f;
     }
@@ -177,6 +179,13 @@ void planes(const char* (&p)[3], bool copied, const void* x, const char* copy, i
   for (int i = 0; i < 3; ++i) p[i] = copied ? copy + i * plane * 2 : static_cast<const char*>(x);
 }
 
+// f of the activation as a constant: a tile's 64 activations a lane are straight code, three times as long with all of them in it
+template <class F>
+hipError_t for_act(int act, F&& f) {
+  return act == SEQ_SILU ? f(std::integral_constant<int, SEQ_SILU>()) : act == SEQ_GELU ? f(std::integral_constant<int, SEQ_GELU>())
+                                                                                     : f(std::integral_constant<int, SEQ_SIGMOID>());
+}
+
 void tiles(GemmArgs& g, int BM, int BN) {
   g.tiles_m = (g.M + BM - 1) / BM;
   g.tiles_n = (g.N + BN - 1) / BN;
@@ -190,10 +199,13 @@ hipError_t launch_unit(GemmArgs g, const UnitArgs& u, hipStream_t s) {
   const bool wide = u.F % 4 == 0;
   auto go = [&](auto* f) {
     const hipError_t e = lds_for(f, G::kLds);
-    if (e == hipSuccess) f<<<(unsigned)(g.tiles_m * g.tiles_n), G::kThreads, G::kLds, s>>>(g, u.act, static_cast<T*>(u.y), u.pre, wide);
+    if (e == hipSuccess) f<<<(unsigned)(g.tiles_m * g.tiles_n), G::kThreads, G::kLds, s>>>(g, static_cast<T*>(u.y), u.pre, wide);
     return e;
   };
-  return u.pre ? go(k_unit<DT, WM, WN, MT, NT, true>) : go(k_unit<DT, WM, WN, MT, NT, false>);
+  return for_act(u.act, [&](auto act) {
+    constexpr int A = decltype(act)::value;
+    return u.pre ? go(k_unit<DT, A, WM, WN, MT, NT, true>) : go(k_unit<DT, A, WM, WN, MT, NT, false>);
+  });
 }
 
 template <int DT, int WM, int WN, int MT, int NT, bool AI, bool BI, bool SPLIT>
@@ -209,14 +221,17 @@ hipError_t launch_gemm(GemmArgs g, void* c0, void* c1, hipStream_t s) {
 }
 
 // Tile sizes of an m x n result (n: both projections' columns): 0: 256 x 256 (8 waves, one workgroup a compute unit), 1: 128 x
-// 128 (4 waves, two), 2: 64 x 64 (4 waves, four).  The one whose rounds over the 256 units take the least: a round is the work of a
-// unit's workgroups over the share of the matrix cores' rate that the tile reaches (measured at M 4096, D 2048: 1, 0.7, 0.35 of
-// that of the first; smaller tiles read more of LDS for a product).
-int tile_for(int64_t m, int64_t n) {
+// 128 (4 waves, two), 2: 64 x 64 (4 waves, four), 3: 192 x 256 (8 waves, one; not where A is transposed on its way).  The one
+// whose rounds over the 256 units take the least: a round is the work of a unit's workgroups over the share of the first one's
+// rate that the tile reaches.
+int tile_for(int64_t m, int64_t n, bool with3) {
   auto rounds = [](int64_t tiles, int slots) { return (double)((tiles + slots - 1) / slots); };
-  auto count = [&](int t) { return ((m + t - 1) / t) * ((n + t - 1) / t); };
-  const double cost[3] = {rounds(count(256), 256), rounds(count(128), 512) * 2 / 4 / 0.7, rounds(count(64), 1024) * 4 / 16 / 0.35};
-  return cost[0] <= cost[1] && cost[0] <= cost[2] ? 0 : cost[1] <= cost[2] ? 1 : 2;
+  auto count = [&](int r, int c) { return ((m + r - 1) / r) * ((n + c - 1) / c); };
+  const double cost[4] = {rounds(count(256, 256), 256), rounds(count(128, 128), 512) * 2 / 4 / 0.7, rounds(count(64, 64), 1024) * 4 / 16 / 0.35,
+                          rounds(count(192, 256), 256) * 3 / 4 / 0.95};
+  int best = 0;
+  for (int t = 1; t < (with3 ? 4 : 3); ++t) best = cost[t] < cost[best] ? t : best;
+  return best;
 }
 
 template <int DT>
@@ -234,22 +249,26 @@ hipError_t forward(const UnitArgs& u, hipStream_t s) {
   planes(g.a[0], u.copy_x, u.x, u.xp, u.M * u.D8);
   planes(g.b[0], u.copy_w, u.wg, u.wgp, u.D * u.F8);
   planes(g.b[1], u.copy_w, u.wu, u.wup, u.D * u.F8);
-  const int tile = tile_for(u.M, 2 * (int64_t)u.F);
-  const hipError_t e = tile == 0 ? launch_unit<DT, 2, 4, 8, 4>(g, u, s)
-                       : tile == 1 ? launch_unit<DT, 2, 2, 4, 4>(g, u, s) : launch_unit<DT, 2, 2, 2, 2>(g, u, s);
+  const int tile = tile_for(u.M, 2 * (int64_t)u.F, true);
+  const hipError_t e = tile == 0   ? launch_unit<DT, 2, 4, 8, 4>(g, u, s)
+                       : tile == 1 ? launch_unit<DT, 2, 2, 4, 4>(g, u, s)
+                       : tile == 2 ? launch_unit<DT, 2, 2, 2, 2>(g, u, s) : launch_unit<DT, 2, 4, 6, 4>(g, u, s);
   return e != hipSuccess ? e : hipGetLastError();
 }
 
 template <int DT>
 hipError_t backward(const UnitArgs& u, hipStream_t s) {
   constexpr int np = DT == SEQ_FP32 ? 3 : 1;
-  if (u.M) k_unit_back<DT><<<blocks_for(u.M * u.F8 / 8), 256, 0, s>>>(u);
+  hipError_t e = !u.M ? hipSuccess : for_act(u.act, [&](auto act) {
+    k_unit_back<DT, decltype(act)::value><<<blocks_for(u.M * u.F8 / 8), 256, 0, s>>>(u);
+    return hipGetLastError();
+  });
+  if (e != hipSuccess) return e;
   if (u.copy_x) copy<DT>(u.x, u.x_ld, u.M, u.D, u.D8, u.xp, s);
   if (u.copy_w) {
     copy<DT>(u.wg, u.w_ld, u.D, u.F, u.F8, u.wgp, s);
     copy<DT>(u.wu, u.wu_ld, u.D, u.F, u.F8, u.wup, s);
   }
-  hipError_t e = hipSuccess;
   if (u.dx) {
     GemmArgs g = {};
     g.M = u.M, g.N = u.D, g.K = u.F;
@@ -260,10 +279,11 @@ hipError_t backward(const UnitArgs& u, hipStream_t s) {
     planes(g.a[1], true, nullptr, u.dbp, u.M * u.F8);
     planes(g.b[0], u.copy_w, u.wg, u.wgp, u.D * u.F8);
     planes(g.b[1], u.copy_w, u.wu, u.wup, u.D * u.F8);
-    const int tile = tile_for(u.M, u.D);
-    e = tile == 0 ? launch_gemm<DT, 2, 4, 8, 4, true, true, true>(g, u.dx, nullptr, s)
+    const int tile = tile_for(u.M, u.D, true);
+    e = tile == 0   ? launch_gemm<DT, 2, 4, 8, 4, true, true, true>(g, u.dx, nullptr, s)
         : tile == 1 ? launch_gemm<DT, 2, 2, 4, 4, true, true, true>(g, u.dx, nullptr, s)
-                    : launch_gemm<DT, 2, 2, 2, 2, true, true, true>(g, u.dx, nullptr, s);
+        : tile == 2 ? launch_gemm<DT, 2, 2, 2, 2, true, true, true>(g, u.dx, nullptr, s)
+                    : launch_gemm<DT, 2, 4, 6, 4, true, true, true>(g, u.dx, nullptr, s);
     if (e != hipSuccess) return e;
   }
   if (u.dwg) {
@@ -275,7 +295,7 @@ hipError_t backward(const UnitArgs& u, hipStream_t s) {
     planes(g.a[0], u.copy_x, u.x, u.xp, u.M * u.D8);
     planes(g.b[0], true, nullptr, u.dap, u.M * u.F8);
     planes(g.b[1], true, nullptr, u.dbp, u.M * u.F8);
-    const int tile = tile_for(u.D, 2 * (int64_t)u.F);
+    const int tile = tile_for(u.D, 2 * (int64_t)u.F, false);
     e = tile == 0 ? launch_gemm<DT, 2, 4, 8, 4, false, false, false>(g, u.dwg, u.dwu, s)
         : tile == 1 ? launch_gemm<DT, 2, 2, 4, 4, false, false, false>(g, u.dwg, u.dwu, s)
                     : launch_gemm<DT, 2, 2, 2, 2, false, false, false>(g, u.dwg, u.dwu, s);
