@@ -120,6 +120,11 @@ __global__ __launch_bounds__(64 * WM * WN) void k_unit_gemm(GemmArgs g, typename
   }
 }
 
+__device__ __forceinline__ f32x8 once8(const float* p, int n, bool wide) {
+  if (!(wide && n >= 8)) return load8(p, n, false);
+  const f32x4 a = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(p)), b = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(p + 4));
+  return cat8(a, b);
+}
 // da = dy b act'(a), db = dy act(a), as rows of F8 values (f32: planes)
 template <int DT, int ACT>
 __global__ __launch_bounds__(256) void k_unit_back(UnitArgs u) {
@@ -131,7 +136,7 @@ __global__ __launch_bounds__(256) void k_unit_back(UnitArgs u) {
   for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
     const int64_t r = small ? (uint32_t)i / (uint32_t)pieces : i / pieces, p = i - r * pieces;
     const int left = u.F - (int)(8 * p);
-    const f32x8 a = load8(u.pre + r * u.F + 8 * p, left, wide), b = load8(u.pre + MF + r * u.F + 8 * p, left, wide);
+    const f32x8 a = once8(u.pre + r * u.F + 8 * p, left, wide), b = once8(u.pre + MF + r * u.F + 8 * p, left, wide);
     const f32x8 d = load8(dy + r * u.dy_ld + 8 * p, left, wide_dy);
     f32x8 da, db;
 #pragma unroll
