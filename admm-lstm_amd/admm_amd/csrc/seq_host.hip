@@ -20,8 +20,12 @@ hipError_t delta_outside(const DeltaRows& rows, const DeltaOutside& t, hipStream
 hipError_t delta_step(const SeqDeltaStep& d, hipStream_t s);
 hipError_t dropout(int dtype, const void* x, const void* res, void* y, int64_t n, uint32_t below, uint64_t seed, uint64_t offset,
                    const int64_t* seed_dev, hipStream_t s);
-hipError_t unit_forward(const UnitArgs& u, hipStream_t s);
-hipError_t unit_backward(const UnitArgs& u, hipStream_t s);
+hipError_t unit_forward_bf16(const UnitArgs& u, hipStream_t s);
+hipError_t unit_forward_fp16(const UnitArgs& u, hipStream_t s);
+hipError_t unit_forward_fp32(const UnitArgs& u, hipStream_t s);
+hipError_t unit_backward_bf16(const UnitArgs& u, hipStream_t s);
+hipError_t unit_backward_fp16(const UnitArgs& u, hipStream_t s);
+hipError_t unit_backward_fp32(const UnitArgs& u, hipStream_t s);
 int unit_few_splits(int D, int F, int dtype);
 hipError_t unit_few(const UnitArgs& u, int splits, float* sums, hipStream_t s);
 }  // namespace seq
@@ -344,7 +348,8 @@ int seq_unit_forward(const SeqUnit* u, void* work, int64_t work_bytes, void* y, 
   unit_args(u, z, work, a);
   a.y = y, a.pre = pre;
   if (z.few) return hip_result(unit_few(a, z.few, static_cast<float*>(work), static_cast<hipStream_t>(stream)), "gated_unit");
-  return hip_result(unit_forward(a, static_cast<hipStream_t>(stream)), "gated_unit");
+  auto* f = a.dtype == SEQ_BF16 ? unit_forward_bf16 : a.dtype == SEQ_FP16 ? unit_forward_fp16 : unit_forward_fp32;
+  return hip_result(f(a, static_cast<hipStream_t>(stream)), "gated_unit");
 }
 
 int seq_unit_backward(const SeqUnit* u, void* work, int64_t work_bytes, const float* pre, const void* dy, int64_t dy_ld,
@@ -360,7 +365,8 @@ int seq_unit_backward(const SeqUnit* u, void* work, int64_t work_bytes, const fl
   a.pre = const_cast<float*>(pre);   // read only
   a.dy = dy, a.dy_ld = dy_ld;
   a.dx = u->M ? dx : nullptr, a.dwg = dwg, a.dwu = dwu;
-  return hip_result(unit_backward(a, static_cast<hipStream_t>(stream)), "gated_unit backward");
+  auto* f = a.dtype == SEQ_BF16 ? unit_backward_bf16 : a.dtype == SEQ_FP16 ? unit_backward_fp16 : unit_backward_fp32;
+  return hip_result(f(a, static_cast<hipStream_t>(stream)), "gated_unit backward");
 }
 
 }  // extern "C"

@@ -1,4 +1,4 @@
-// seq_unit.hip -- the gated unit y = act(x Wg) * (x Wu): both projections, the activation and the product in one kernel,
+// seq_unit_kernels.hpp -- the gated unit y = act(x Wg) * (x Wu): both projections, the activation and the product in one kernel,
 // and its gradients.
 //
 // Forward: a workgroup forms the same tile of both projections (one tile of x in LDS serves both) and only their product
@@ -10,6 +10,9 @@
 // Bound by the matrix cores where the layer is wide (12 M D F operations a training step), by the weights where there are few
 // rows.  f32 operands are split into three bf16 planes by a pass before (six products, seq_dev.hpp), and 16-bit operands whose
 // rows are not 16-byte aligned are copied to padded rows.
+//
+// Compiled by one source for each type (seq_unit_bf16.hip, _fp16, _fp32), so that they compile side by side.
+#pragma once
 #include <type_traits>
 
 #include "seq_gemm.hpp"
@@ -310,12 +313,4 @@ hipError_t backward(const UnitArgs& u, hipStream_t s) {
 }
 
 }  // namespace
-
-hipError_t unit_forward(const UnitArgs& u, hipStream_t s) {
-  return u.dtype == SEQ_BF16 ? forward<SEQ_BF16>(u, s) : u.dtype == SEQ_FP16 ? forward<SEQ_FP16>(u, s) : forward<SEQ_FP32>(u, s);
-}
-hipError_t unit_backward(const UnitArgs& u, hipStream_t s) {
-  return u.dtype == SEQ_BF16 ? backward<SEQ_BF16>(u, s) : u.dtype == SEQ_FP16 ? backward<SEQ_FP16>(u, s) : backward<SEQ_FP32>(u, s);
-}
-
 }  // namespace seq
