@@ -26,7 +26,7 @@ hipError_t unit_forward_fp32(const UnitArgs& u, hipStream_t s);
 hipError_t unit_backward_bf16(const UnitArgs& u, hipStream_t s);
 hipError_t unit_backward_fp16(const UnitArgs& u, hipStream_t s);
 hipError_t unit_backward_fp32(const UnitArgs& u, hipStream_t s);
-int unit_few_splits(int D, int F, int dtype);
+int unit_few_splits(int M, int D, int F, int dtype);
 hipError_t unit_few(const UnitArgs& u, int splits, float* sums, hipStream_t s);
 }  // namespace seq
 
@@ -97,14 +97,26 @@ int delta_sizes(const SeqDelta* d, bool saved, DeltaSizes& z) {
   if (d->offsets ? d->batch != 1 : d->sequences != d->batch)
     return fail(SEQ_EINVAL, d->offsets ? "packed sequences need batch 1 (got %lld)" : "sequences must equal batch (%lld)", (long long)d->batch);
   z.KP = d->K <= 32 ? 32 : d->K <= 64 ? 64 : 128;
-  // sequences of at most 32 rows (or packed ones of at most 32 on average) would leave half of a 64-row chunk empty
-  z.C = d->T <= 32 || (d->offsets && d->T <= 32 * d->sequences) ? 32 : 64;
+  // Chunks of 32 rows where sequences are so short that half of 64 would be empty, and where there are more column tiles than two
+  // rounds of the chip's: less is done then in each chunk (X is formed in C^3, P u in C^2 a row), while with few tiles the number of
+  // chunks counts.  With gradients these take more for the chunks' states than that saves, but in f32, heads of 32 and short
+  // sequences.  In us, 32 and 64 rows, forward alone and with gradients, 1024 rows but for the last:
+  //   32 heads of 128 x 128, bf16: 62, 214 and 47, 151;  128 such heads, bf16: 142, 710 and 143, 583, f32: 243, 928 and 298, 1006;
+  //   512 heads of 64 x 64, bf16: 274, 1273 and 342, 1093, f32: 457, 1536 and 501, 1741;
+  //   1024 heads of 64 x 64, 48 rows, bf16: 39, 151 and 63, 174, f32: 57, 220 and 79, 274.
+  const int64_t tiles = d->sequences * d->Hv * ((d->V + 15) / 16);
+  const bool many = tiles > 512 && (!saved || d->dtype == SEQ_FP32 || d->K <= 32 || d->T <= 64 || (d->offsets && d->T <= 64 * d->sequences));
+  z.C = many || d->T <= 32 || (d->offsets && d->T <= 32 * d->sequences) ? 32 : 64;
   // (faster in every size tried, seq_delta_short.hip; it works with 32-bit offsets within a sequence)
   z.brief = !d->offsets && d->T > 0 && d->T <= 32 && std::max({d->v_stride[1], (int64_t)d->Hv * d->V, (int64_t)d->Hv * d->K}) < 1 << 25;
   const int NP = d->dtype + 1, NO = d->dtype == SEQ_FP32 ? 3 : 2, tri = z.C == 64 ? 6 : 2;
   z.per = (d->T + z.C - 1) / z.C;
   z.VP = (d->V + 15) / 16 * 16;
-  z.wide_cols = d->sequences * d->Hv * (z.VP / 16) > 512;
+  // Two column tiles a workgroup, which share its loads, where one each would be more than a round.  In us, one and two, forward
+  // alone and with gradients, 1024 rows of 128 x 128, bf16: 256 tiles 48, 159 and 65, 187; 512: 79, 355 and 69, 303; 768: 111, 530
+  // and 117, 501; 1024: 162, 695 and 144, 583.  Packed sequences are of uneven length, and the short ones' units are soon free for
+  // others (504 tiles of 9 sequences: 62 us and 91)
+  z.wide_cols = tiles > (d->offsets ? 512 : 256);
   z.chunks = d->offsets ? (d->sequences && d->T ? d->T / z.C + d->sequences + 1 : 0) : z.per * d->batch;
   if (z.chunks > kMaxBlocks / d->Hv || (d->sequences + 8) > kMaxBlocks / ((int64_t)d->Hv * (z.VP / 16) * 8))
     return fail(SEQ_EINVAL, "too many sequences, rows or heads for one launch");
@@ -193,7 +205,7 @@ int unit_sizes(const SeqUnit* u, bool backward, UnitSizes& z) {
   z.da = backward ? up256(u->M * z.F8 * 2 * np) : 0;
   z.need = z.x + 2 * z.w + 2 * z.da;
   // up to 32 rows: two tiles of 16 beside each weight fragment are still bound by the weights
-  z.few = !backward && u->M <= 32 ? unit_few_splits(u->D, u->F, u->dtype) : 0;
+  z.few = backward ? 0 : unit_few_splits(u->M, u->D, u->F, u->dtype);
   if (z.few) z.need = z.few > 1 ? up256(2LL * z.few * u->M * u->F * 4) : 0;
   return SEQ_OK;
 }

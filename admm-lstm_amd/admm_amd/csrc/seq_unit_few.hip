@@ -15,6 +15,7 @@ namespace seq {
 namespace {
 
 constexpr int kWavesF = 4;
+constexpr int kRowS = 66;   // a register of all lanes in LDS: two banks on, so that neighbouring columns lie in different banks
 template <int DT> constexpr int few_cols() { return DT == SEQ_FP32 ? 64 : 128; }   // columns of a workgroup
 template <int DT> constexpr int few_frags() { return DT == SEQ_FP32 ? 4 : 8; }     // fragments side by side
 
@@ -116,7 +117,7 @@ __global__ __launch_bounds__(64 * kWavesF) void k_unit_few(UnitArgs u, int split
     }
   }
   mfma_settle();
-  constexpr int kPart = MT * 2 * NF * 4 * 64;
+  constexpr int kPart = MT * 2 * NF * 4 * kRowS;
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -124,7 +125,7 @@ __global__ __launch_bounds__(64 * kWavesF) void k_unit_few(UnitArgs u, int split
 #pragma unroll
       for (int j = 0; j < NF; ++j)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) part[wave * kPart + (((m * 2 + e) * NF + j) * 4 + r) * 64 + lane] = acc[m][e][j][r];
+        for (int r = 0; r < 4; ++r) part[wave * kPart + (((m * 2 + e) * NF + j) * 4 + r) * kRowS + lane] = acc[m][e][j][r];
   __syncthreads();
   // row m, column n of the group: lane 16 g + m % 16, register r and fragment j with n = NF (4 g + r) + j
   const int rows = u.M < 16 * MT ? u.M : 16 * MT;
@@ -134,7 +135,7 @@ __global__ __launch_bounds__(64 * kWavesF) void k_unit_few(UnitArgs u, int split
     float v[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const int at = ((((m >> 4) * 2 + e) * NF + n % NF) * 4 + (n / NF & 3)) * 64 + (n / NF >> 2) * 16 + (m & 15);
+      const int at = ((((m >> 4) * 2 + e) * NF + n % NF) * 4 + (n / NF & 3)) * kRowS + (n / NF >> 2) * 16 + (m & 15);
       v[e] = (part[at] + part[kPart + at]) + (part[2 * kPart + at] + part[3 * kPart + at]);
     }
     const int64_t to = (int64_t)m * u.F + c, MF = (int64_t)u.M * u.F;
@@ -171,7 +172,7 @@ __global__ __launch_bounds__(256) void k_unit_sum(UnitArgs u, int splits, const 
 template <int DT, int MT>
 hipError_t launch(const UnitArgs& u, int splits, float* sums, hipStream_t s) {
   using T = typename Elem<DT>::T;
-  constexpr int bytes = kWavesF * MT * 2 * few_frags<DT>() * 4 * 64 * 4;
+  constexpr int bytes = kWavesF * MT * 2 * few_frags<DT>() * 4 * kRowS * 4;
   hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k_unit_few<DT, MT>), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != hipSuccess) return e;
   const int groups = (u.F + few_cols<DT>() - 1) / few_cols<DT>();
@@ -185,10 +186,15 @@ hipError_t launch(const UnitArgs& u, int splits, float* sums, hipStream_t s) {
 
 }  // namespace
 
-// Workgroups along the inner axis: enough for three on every compute unit, and at least two steps of 32 for each of their waves
-int unit_few_splits(int D, int F, int dtype) {
+// Workgroups along the inner axis, 0 where tiles are faster.  Enough for three on every compute unit (for half of that with more
+// than 16 rows, whose sums are twice as long), and at least two steps of 32 for each of their waves.  In us, against 64-row tiles:
+// bf16, D 2048, F 8192: 1 to 16 rows 19 to 22 (28), 32 rows 25 (28); D 4096, F 1024, 32 rows: 18 (34); but D 512, F 1408, 1 to 32
+// rows: 9 to 13 (7), D 1024, F 4096, 16 rows: 12 (11), so not up to D 1024.  f32, whose tiles have six products: D 512, F 1408, 32
+// rows: 13 (35); D 2048, F 8192: 35 to 54 (170).  32 rows of the first with 4, 8 and 16 along the inner axis: 25, 32, 45.
+int unit_few_splits(int M, int D, int F, int dtype) {
+  if (M > 32 || (dtype != SEQ_FP32 && D <= 1024)) return 0;
   const int cols = dtype == SEQ_FP32 ? 64 : 128, groups = (F + cols - 1) / cols;
-  const int most = D / (dtype == SEQ_FP32 ? 128 : 256), want = (768 + groups - 1) / groups;
+  const int most = D / (dtype == SEQ_FP32 ? 128 : 256), all = M > 16 ? 384 : 768, want = (all + groups - 1) / groups;
   const int s = want < most ? want : most;
   return s < 1 ? 1 : s > 32 ? 32 : s;
 }

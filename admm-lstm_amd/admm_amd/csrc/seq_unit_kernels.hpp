@@ -258,12 +258,14 @@ hipError_t launch_gemm(GemmArgs g, void* c0, void* c1, hipStream_t s) {
 // Tile sizes of an m x n result (n: both projections' columns): 0: 256 x 256 (8 waves, one workgroup a compute unit), 1: 128 x
 // 128 (4 waves, two), 2: 64 x 64 (4 waves, four), 3: 192 x 256 (8 waves, one; not where A is transposed on its way).  The one
 // whose rounds over the 256 units take the least: a round is the work of a unit's workgroups over the share of the first one's
-// rate that the tile reaches.
+// rate that the tile reaches, from these times (us, D 2048, F 4096, bf16 and f32, tiles 0 to 3):
+//   M 4096: 130, 139, 240, 148 and 695, 774, 1986, 780;  M 2048: 71, 87, 141, 99 and 383, 403, 801, 506;
+//   M 1536 (a whole round of tile 3): 64, 61, 95, 54 and 330, 342, 576, 284.
 int tile_for(int64_t m, int64_t n, bool with3) {
   auto rounds = [](int64_t tiles, int slots) { return (double)((tiles + slots - 1) / slots); };
   auto count = [&](int r, int c) { return ((m + r - 1) / r) * ((n + c - 1) / c); };
-  const double cost[4] = {rounds(count(256, 256), 256), rounds(count(128, 128), 512) * 2 / 4 / 0.7, rounds(count(64, 64), 1024) * 4 / 16 / 0.35,
-                          rounds(count(192, 256), 256) * 3 / 4 / 0.95};
+  const double cost[4] = {rounds(count(256, 256), 256), rounds(count(128, 128), 512) * 2 / 4 / 0.9, rounds(count(64, 64), 1024) * 4 / 16 / 0.5,
+                          rounds(count(192, 256), 256) * 3 / 4 / 0.98};
   int best = 0;
   for (int t = 1; t < (with3 ? 4 : 3); ++t) best = cost[t] < cost[best] ? t : best;
   return best;
