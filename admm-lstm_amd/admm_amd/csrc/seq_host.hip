@@ -204,7 +204,6 @@ int unit_sizes(const SeqUnit* u, bool backward, UnitSizes& z) {
   z.w = z.copy_w ? up256(u->D * z.F8 * 2 * np) : 0;
   z.da = backward ? up256(u->M * z.F8 * 2 * np) : 0;
   z.need = z.x + 2 * z.w + 2 * z.da;
-  // up to 32 rows: two tiles of 16 beside each weight fragment are still bound by the weights
   z.few = backward ? 0 : unit_few_splits(u->M, u->D, u->F, u->dtype);
   if (z.few) z.need = z.few > 1 ? up256(2LL * z.few * u->M * u->F * 4) : 0;
   return SEQ_OK;

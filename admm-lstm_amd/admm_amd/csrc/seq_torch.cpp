@@ -162,8 +162,7 @@ struct RuleFunction : torch::autograd::Function<RuleFunction> {
                                const std::optional<Tensor>& initial_, const std::optional<Tensor>& offsets_, double scale) {
     const Tensor initial = initial_.value_or(Tensor()), offsets = offsets_.value_or(Tensor());
     auto [o, final_state, work] = RuleCall(q, k, v, g, beta, initial, offsets, scale).forward(true);
-    ctx->save_for_backward({q, k, v, g, beta, initial, offsets});
-    ctx->saved_data["work"] = work;
+    ctx->save_for_backward({q, k, v, g, beta, initial, offsets, work});   // work too: freed with them after the backward pass
     ctx->saved_data["scale"] = scale;
     ctx->set_materialize_grads(false);
     return {o, final_state};
@@ -171,7 +170,7 @@ struct RuleFunction : torch::autograd::Function<RuleFunction> {
   static variable_list backward(AutogradContext* ctx, const variable_list& d_out) {
     const variable_list in = ctx->get_saved_variables();
     RuleCall call(in[0], in[1], in[2], in[3], in[4], in[5], in[6], ctx->saved_data["scale"].toDouble());
-    const Tensor work = ctx->saved_data["work"].toTensor();
+    const Tensor work = in[7];
     Tensor d_o = d_out[0].defined() ? d_out[0].contiguous() : at::zeros(call.v.sizes(), call.v.options());
     Tensor d_final = d_out[1].defined() ? d_out[1].contiguous() : Tensor();
     int64_t need = 0;
@@ -270,8 +269,9 @@ Tensor gated_delta_step(const py::handle& q_, const py::handle& k_, const py::ha
   d.slots = data(slots);
   d.state = state.data_ptr<float>();
   d.o = o.data_ptr();
+  state.unsafeGetTensorImpl()->bump_version();   // autograd sees that saved views of it are stale (raises for an inference tensor
+                                                 // outside of inference mode, before it is written)
   check(seq_delta_step(&d, stream_of(q)), "gated_delta_step");
-  state.unsafeGetTensorImpl()->bump_version();   // autograd sees that saved views of it are stale
   return o;
 }
 
@@ -305,15 +305,14 @@ struct UnitCall {
 struct UnitFunction : torch::autograd::Function<UnitFunction> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& wg, const Tensor& wu, int64_t act) {
     auto [y, pre] = UnitCall(x, wg, wu, (int)act).forward(true);
-    ctx->save_for_backward({x, wg, wu});
-    ctx->saved_data["pre"] = pre;
+    ctx->save_for_backward({x, wg, wu, pre});
     ctx->saved_data["act"] = act;
     return y;
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& d_out) {
     const variable_list in = ctx->get_saved_variables();
     UnitCall call(in[0], in[1], in[2], (int)ctx->saved_data["act"].toInt());
-    const Tensor pre = ctx->saved_data["pre"].toTensor(), dy = rows_last(d_out[0]), w = call.work(true);
+    const Tensor pre = in[3], dy = rows_last(d_out[0]), w = call.work(true);
     variable_list grads(4);
     if (ctx->needs_input_grad(0)) grads[0] = at::empty(in[0].sizes(), in[0].options());
     if (ctx->needs_input_grad(1) || ctx->needs_input_grad(2))

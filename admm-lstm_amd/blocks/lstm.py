@@ -25,6 +25,8 @@ GATES4 = ('i', 'f', 'g', 'o')
 
 
 class LSTM(nn.Module):
+    dropout = 0.0   # also of models pickled before there was one
+
     def __init__(self, input_size: int, hidden_size: int, output_size: int, with_grad: bool = False,
                  *, dropout: float = 0.0) -> None:
         super().__init__()
@@ -62,7 +64,8 @@ class LSTM(nn.Module):
     # -- forward
     def forward(self, x: torch.Tensor, c: torch.Tensor = None, h: torch.Tensor = None,
                 *, dropout_seed: Union[int, torch.Tensor, None] = None) -> torch.Tensor:
-        """``dropout_seed``: of the dropped values' mask (blocks/dropout.py); None draws one from torch's generator."""
+        """``dropout_seed``: of the dropped values' mask (blocks/dropout.py); None draws one from torch's
+        generator (a captured call needs one on the device)."""
         if self.with_grad:
             return self.grad_forward(x, c, h, dropout_seed=dropout_seed)
         if c is None and h is None:

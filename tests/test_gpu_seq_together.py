@@ -151,3 +151,75 @@ def test_lstm_drops_part_of_its_last_state():
     a, b = m(x), m(x)
     torch.manual_seed(11)
     assert torch.equal(m(x), a) and not torch.equal(a, b)   # a new mask each call, from torch's generator
+
+
+def test_what_the_gradients_need_is_freed_with_them():
+    """The work memory and the kept projections go after the backward pass, though the results (and their graph) live on."""
+    from blocks import delta_rule, gated_unit
+    q, k, v, g, beta, s0 = R.delta_inputs(2, 2048, 4, 4, 64, 64, torch.bfloat16, seed=70)
+    v.requires_grad_()
+    x, w = torch.randn(4096, 64, device='cuda', requires_grad=True), torch.randn(64, 512, device='cuda')
+    for call, leaf in ((lambda: delta_rule.gated_delta_rule(q, k, v, g, beta, initial_state=s0)[0], v), (lambda: gated_unit.gated_unit(x, w, w), x)):
+        torch.autograd.grad(call().sum(), leaf)
+        before = torch.cuda.memory_allocated()
+        y = call()
+        held = torch.cuda.memory_allocated() - before
+        torch.autograd.grad(y.sum(), leaf)
+        after = torch.cuda.memory_allocated() - before
+        assert after <= held / 2 and after <= 2 * y.numel() * y.element_size()   # y itself (and its final state)
+
+
+def test_inference_mode():
+    """Results as under no_grad; a state made there is refused outside, before it is written."""
+    from blocks import delta_rule
+    q, k, v, g, beta, s0 = R.delta_inputs(2, 40, 1, 2, 16, 16, torch.float32, seed=71)
+    with torch.no_grad():
+        want = delta_rule.gated_delta_rule(q, k, v, g, beta, initial_state=s0)
+    with torch.inference_mode():
+        o, state = delta_rule.gated_delta_rule(q, k, v, g, beta, initial_state=s0)
+        assert torch.equal(o, want[0]) and torch.equal(state, want[1])
+        kept = state.clone()
+        first = delta_rule.gated_delta_step(q[:, 0], k[:, 0], v[:, 0], g[:, 0], beta[:, 0], state)
+    assert torch.isfinite(first).all() and not torch.equal(state, kept)
+    kept = state.clone()
+    with pytest.raises(RuntimeError, match='nference'):
+        delta_rule.gated_delta_step(q[:, 0], k[:, 0], v[:, 0], g[:, 0], beta[:, 0], state)
+    assert torch.equal(state, kept)
+
+
+def test_rows_expanded_from_one():
+    """Rows and gradients whose stride is zero."""
+    from blocks import gated_unit
+    row, w, u = torch.randn(1, 64, device='cuda'), torch.randn(64, 72, device='cuda'), torch.randn(64, 72, device='cuda')
+    for M in (7, 100):
+        x = row.expand(M, 64).requires_grad_()
+        y = gated_unit.gated_unit(x, w, u)
+        assert torch.equal(y, y[:1].expand(M, 72))
+        one = torch.randn(1, 72, device='cuda')
+        (a,) = torch.autograd.grad(y, x, one.expand(M, 72), retain_graph=True)
+        (b,) = torch.autograd.grad(y, x, one.expand(M, 72).contiguous())
+        assert torch.equal(a, b)
+
+
+def test_two_threads_at_once():
+    """Calls from two threads on streams of their own."""
+    import threading
+    from blocks import delta_rule
+    ins = [R.delta_inputs(2, T, 1, 2, 32, 32, torch.bfloat16, seed=72 + T) for T in (30, 200)]
+    want = [delta_rule.gated_delta_rule(*i[:5], initial_state=i[5]) for i in ins]
+    torch.cuda.synchronize()
+    got = [None, None]
+
+    def work(n):
+        with torch.cuda.stream(torch.cuda.Stream()), torch.no_grad():
+            for _ in range(20):
+                got[n] = delta_rule.gated_delta_rule(*ins[n][:5], initial_state=ins[n][5])
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(n,)) for n in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for a, b in zip(want, got):
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
