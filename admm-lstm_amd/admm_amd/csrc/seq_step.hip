@@ -2,7 +2,8 @@
 //
 // Bound by the state: K V values of 32 bits read and written per stream and head, everything else is a few rows.  A
 // workgroup takes COLS columns of one head's state, all rows of it in registers (a lane: 4 columns of some rows), so
-// that one load and one store of the state are all the traffic, and S^T k and S^T q come out of one reduction: with S' = exp(g) S and u = beta (v - S'^T k), S = S' + k u^T and S^T q = S'^T q + (k . q) u.
+// that one load and one store of the state are all the traffic, and S^T k and S^T q come out of one reduction: with
+// S' = exp(g) S and u = beta (v - S'^T k), S = S' + k u^T and S^T q = S'^T q + (k . q) u.
 #include "seq_delta.hpp"
 
 namespace seq {

@@ -11,6 +11,9 @@
 // rows.  f32 operands are split into three bf16 planes by a pass before (six products, seq_dev.hpp), and 16-bit operands whose
 // rows are not 16-byte aligned are copied to padded rows.
 //
+// 8192 x 2048 x 8192, bf16: forward with the projections kept 635 us (865 TFLOP/s; without them 550), dx 500 us and dWg, dWu 530 us
+// (1.1 and 1.04 PFLOP/s; a large library product reaches 1.2 to 1.3), the elementwise pass 204 us (4.6 TB/s).
+//
 // Compiled by one source for each type (seq_unit_bf16.hip, _fp16, _fp32), so that they compile side by side.
 #pragma once
 #include <type_traits>

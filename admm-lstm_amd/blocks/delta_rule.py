@@ -7,6 +7,9 @@ For each sequence and value head, with the state S [K, V] (float32)::
 ``gated_delta_rule`` runs whole sequences (training and prompts) and carries gradients; ``gated_delta_step`` runs one
 token of each of many streams and updates their states in place (serving).  Both need HIP device tensors and run in
 libseqops.so (hand-written gfx950 kernels) on the current stream of the tensors' device.
+
+All of it can be captured into a graph.  As with PyTorch's own operators, a backward pass is captured only while no eager
+autograd graph of the same leaves is alive (it would tie the captured work to the stream of the eager one).
 """
 from __future__ import annotations
 
