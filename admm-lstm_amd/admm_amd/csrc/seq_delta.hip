@@ -41,7 +41,7 @@ __device__ __forceinline__ void tile_planes(const float* m, int ld, int r, int c
 
 // Bound by the chain of small products, exchanges and barriers of a chunk: several workgroups on a compute unit cover for each
 // other, so the f32 tiles lie where K and Q were, and fragments are cut straight from them.
-// 128 chunks of 16 query/key and 32 value heads of 128, bf16: 75 us, 15 us of it one workgroup's way through; 270 MB written.
+// 128 chunks of 16 query/key and 32 value heads of 128, bf16: 75 us, about 15 us of it one workgroup's way through; 230 MB written.
 template <int DT, int KP, int C, bool SAVE>
 __global__ __launch_bounds__(4 * C, DT == SEQ_FP32 ? 2 : 3) void k_delta_prep(DeltaArgs a) {
   using S = DeltaShape<DT, KP, C, SAVE>;
