@@ -182,7 +182,7 @@ bool delta_inputs(const SeqDelta* d) { return d->batch * d->T == 0 || (d->q && d
 struct UnitSizes {
   bool copy_x, copy_w;
   int few;   // the forward of a few rows: workgroups along the inner axis; 0: tiles
-  int64_t D8, F8, x, w, da, need;
+  int64_t D8, F8, x, w, da, sums, need;
 };
 
 int unit_sizes(const SeqUnit* u, bool backward, UnitSizes& z) {
@@ -203,7 +203,9 @@ int unit_sizes(const SeqUnit* u, bool backward, UnitSizes& z) {
   z.x = z.copy_x ? up256(u->M * z.D8 * 2 * np) : 0;
   z.w = z.copy_w ? up256(u->D * z.F8 * 2 * np) : 0;
   z.da = backward ? up256(u->M * z.F8 * 2 * np) : 0;
-  z.need = z.x + 2 * z.w + 2 * z.da;
+  const int parts = backward ? unit_parts(u->M, u->D, u->F, u->dtype).parts : 1;
+  z.sums = parts > 1 ? up256(parts * 8LL * u->D * u->F) : 0;
+  z.need = z.x + 2 * z.w + 2 * z.da + z.sums;
   z.few = backward ? 0 : unit_few_splits(u->M, u->D, u->F, u->dtype);
   if (z.few) z.need = z.few > 1 ? up256(2LL * z.few * u->M * u->F * 4) : 0;
   return SEQ_OK;
@@ -221,6 +223,7 @@ void unit_args(const SeqUnit* u, const UnitSizes& z, void* work, UnitArgs& a) {
   a.wup = a.wgp + z.w;
   a.dap = a.wup + z.w;
   a.dbp = a.dap + z.da;
+  a.sums = reinterpret_cast<float*>(a.dbp + z.da);
 }
 
 }  // namespace

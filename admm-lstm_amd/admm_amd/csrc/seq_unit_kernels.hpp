@@ -5,7 +5,7 @@
 // leaves it; where gradients follow, the projections a = x Wg and b = x Wu are kept too, in f32 (rounded to 16 bits they would
 // cost the gradients more than their own rounding).  Backward: da = dy b act'(a) and db = dy act(a) elementwise, rounded to
 // the inputs' type (one rounding more than the result's own), then dx = da Wg^T + db Wu^T as one product over both, and
-// dWg = x^T da, dWu = x^T db in one launch.
+// dWg = x^T da, dWu = x^T db in one launch (in parts of the rows where the layer is narrow, unit_parts).
 //
 // Bound by the matrix cores where the layer is wide (12 M D F operations a training step), by the weights where there are few
 // rows.  f32 operands are split into three bf16 planes by a pass before (six products, seq_dev.hpp), and 16-bit operands whose
@@ -130,17 +130,32 @@ __global__ __launch_bounds__(64 * WM * WN) void k_unit(GemmArgs g, typename Elem
     }
 }
 
-// AI, BI, SPLIT as in Gemm; otherwise blockIdx.y picks the matrix B and the result
+// AI, BI, SPLIT as in Gemm; otherwise blockIdx.y picks the matrix B and the result, and blockIdx.z a part of the inner axis, whose
+// sums go to `sums` [part][matrix][M][N] where there are several
 template <int DT, int WM, int WN, int MT, int NT, bool AI, bool BI, bool SPLIT>
-__global__ __launch_bounds__(64 * WM * WN) void k_unit_gemm(GemmArgs g, typename Elem<DT>::T* c0, typename Elem<DT>::T* c1, bool wide) {
+__global__ __launch_bounds__(64 * WM * WN) void k_unit_gemm(GemmArgs g, typename Elem<DT>::T* c0, typename Elem<DT>::T* c1, float* sums, bool wide) {
   using G = Gemm<DT, WM, WN, MT, NT, AI, BI, false, SPLIT>;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lane = threadIdx.x & 63, wave = wave_id(), x = lane & 15, q = lane >> 4, wm = wave / WN, wn = wave % WN;
   int tm, tn;
   G::place(g, tm, tn);
   f32x4 acc[MT][NT];
+  if constexpr (!SPLIT && !AI && !BI) {
+    if (gridDim.z > 1) {
+      const int tiles = (g.K + kBK - 1) / kBK, first = (int)((int64_t)tiles * blockIdx.z / gridDim.z), end = (int)((int64_t)tiles * (blockIdx.z + 1) / gridDim.z);
+      const int64_t k0 = (int64_t)first * kBK;
+#pragma unroll
+      for (int p = 0; p < 3; ++p) {
+        g.a[0][p] += k0 * g.lda * 2;
+        g.b[0][p] += k0 * g.ldb * 2;
+        g.b[1][p] += k0 * g.ldb * 2;
+      }
+      g.K = (int)((int64_t)end * kBK < g.K ? (int64_t)end * kBK - k0 : g.K - k0);
+    }
+  }
   G::run(g, tm, tn, blockIdx.y, lds, acc);
   typename Elem<DT>::T* c = blockIdx.y ? c1 : c0;
+  if (sums) sums += (2 * (int64_t)blockIdx.z + blockIdx.y) * g.M * g.N;
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
     const int row = tm * G::BM + 16 * (wm * MT + i) + x;
@@ -148,7 +163,9 @@ __global__ __launch_bounds__(64 * WM * WN) void k_unit_gemm(GemmArgs g, typename
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       const int col = tn * G::BN + 16 * (wn * NT + j) + 4 * q, n = g.N - col;
-      if (n > 0) store4(c + (int64_t)row * g.N + col, acc[i][j], n, wide);
+      if (n <= 0) continue;
+      if (sums) store4(sums + (int64_t)row * g.N + col, acc[i][j], n, wide);
+      else store4(c + (int64_t)row * g.N + col, acc[i][j], n, wide);
     }
   }
 }
@@ -158,6 +175,17 @@ __device__ __forceinline__ f32x8 once8(const float* p, int n, bool wide) {
   const f32x4 a = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(p)), b = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(p + 4));
   return cat8(a, b);
 }
+// the parts' sums [part][matrix][n], added up in order
+template <class T>
+__global__ __launch_bounds__(256) void k_unit_join(const float* sums, int parts, int64_t n, T* c0, T* c1) {
+  for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < 2 * n; i += (int64_t)gridDim.x * 256) {
+    float v = 0.f;
+#pragma unroll 8
+    for (int p = 0; p < parts; ++p) v += sums[2 * n * p + i];
+    (i < n ? c0 : c1 - n)[i] = (T)v;
+  }
+}
+
 // da = dy b act'(a), db = dy act(a), as rows of F8 values (f32: planes)
 template <int DT, int ACT>
 __global__ __launch_bounds__(256) void k_unit_back(UnitArgs u) {
@@ -247,31 +275,16 @@ hipError_t launch_unit(GemmArgs g, const UnitArgs& u, hipStream_t s) {
 }
 
 template <int DT, int WM, int WN, int MT, int NT, bool AI, bool BI, bool SPLIT>
-hipError_t launch_gemm(GemmArgs g, void* c0, void* c1, hipStream_t s) {
+hipError_t launch_gemm(GemmArgs g, void* c0, void* c1, hipStream_t s, int parts = 1, float* sums = nullptr) {
   using T = typename Elem<DT>::T;
   using G = Gemm<DT, WM, WN, MT, NT, AI, BI, false, SPLIT>;
   tiles(g, G::BM, G::BN);
   auto* f = k_unit_gemm<DT, WM, WN, MT, NT, AI, BI, SPLIT>;
   const hipError_t e = lds_for(f, G::kLds);
   if (e != hipSuccess) return e;
-  f<<<dim3((unsigned)(g.tiles_m * g.tiles_n), c1 ? 2 : 1), G::kThreads, G::kLds, s>>>(g, static_cast<T*>(c0), static_cast<T*>(c1), g.N % 4 == 0);
+  f<<<dim3((unsigned)(g.tiles_m * g.tiles_n), c1 ? 2 : 1, (unsigned)parts), G::kThreads, G::kLds, s>>>(
+      g, static_cast<T*>(c0), static_cast<T*>(c1), sums, g.N % 4 == 0);
   return hipSuccess;
-}
-
-// Tile sizes of an m x n result (n: both projections' columns): 0: 256 x 256 (8 waves, one workgroup a compute unit), 1: 128 x
-// 128 (4 waves, two), 2: 64 x 64 (4 waves, four), 3: 192 x 256 (8 waves, one; not where A is transposed on its way).  The one
-// whose rounds over the 256 units take the least: a round is the work of a unit's workgroups over the share of the first one's
-// rate that the tile reaches, from these times (us, D 2048, F 4096, bf16 and f32, tiles 0 to 3):
-//   M 4096: 130, 139, 240, 148 and 695, 774, 1986, 780;  M 2048: 71, 87, 141, 99 and 383, 403, 801, 506;
-//   M 1536 (a whole round of tile 3): 64, 61, 95, 54 and 330, 342, 576, 284.
-int tile_for(int64_t m, int64_t n, bool with3) {
-  auto rounds = [](int64_t tiles, int slots) { return (double)((tiles + slots - 1) / slots); };
-  auto count = [&](int r, int c) { return ((m + r - 1) / r) * ((n + c - 1) / c); };
-  const double cost[4] = {rounds(count(256, 256), 256), rounds(count(128, 128), 512) * 2 / 4 / 0.9, rounds(count(64, 64), 1024) * 4 / 16 / 0.5,
-                          rounds(count(192, 256), 256) * 3 / 4 / 0.98};
-  int best = 0;
-  for (int t = 1; t < (with3 ? 4 : 3); ++t) best = cost[t] < cost[best] ? t : best;
-  return best;
 }
 
 template <int DT>
@@ -289,7 +302,7 @@ hipError_t forward(const UnitArgs& u, hipStream_t s) {
   planes(g.a[0], u.copy_x, u.x, u.xp, u.M * u.D8);
   planes(g.b[0], u.copy_w, u.wg, u.wgp, u.D * u.F8);
   planes(g.b[1], u.copy_w, u.wu, u.wup, u.D * u.F8);
-  const int tile = tile_for(u.M, 2 * (int64_t)u.F, true);
+  const int tile = tile_for(u.M, 2 * (int64_t)u.F, true, 1, nullptr);
   const hipError_t e = tile == 0   ? launch_unit<DT, 2, 4, 8, 4>(g, u, s)
                        : tile == 1 ? launch_unit<DT, 2, 2, 4, 4>(g, u, s)
                        : tile == 2 ? launch_unit<DT, 2, 2, 2, 2>(g, u, s) : launch_unit<DT, 2, 4, 6, 4>(g, u, s);
@@ -319,7 +332,7 @@ hipError_t backward(const UnitArgs& u, hipStream_t s) {
     planes(g.a[1], true, nullptr, u.dbp, u.M * u.F8);
     planes(g.b[0], u.copy_w, u.wg, u.wgp, u.D * u.F8);
     planes(g.b[1], u.copy_w, u.wu, u.wup, u.D * u.F8);
-    const int tile = tile_for(u.M, u.D, true);
+    const int tile = tile_for(u.M, u.D, true, 1, nullptr);
     e = tile == 0   ? launch_gemm<DT, 2, 4, 8, 4, true, true, true>(g, u.dx, nullptr, s)
         : tile == 1 ? launch_gemm<DT, 2, 2, 4, 4, true, true, true>(g, u.dx, nullptr, s)
         : tile == 2 ? launch_gemm<DT, 2, 2, 2, 2, true, true, true>(g, u.dx, nullptr, s)
@@ -335,10 +348,14 @@ hipError_t backward(const UnitArgs& u, hipStream_t s) {
     planes(g.a[0], u.copy_x, u.x, u.xp, u.M * u.D8);
     planes(g.b[0], true, nullptr, u.dap, u.M * u.F8);
     planes(g.b[1], true, nullptr, u.dbp, u.M * u.F8);
-    const int tile = tile_for(u.D, 2 * (int64_t)u.F, false);
-    e = tile == 0 ? launch_gemm<DT, 2, 4, 8, 4, false, false, false>(g, u.dwg, u.dwu, s)
-        : tile == 1 ? launch_gemm<DT, 2, 2, 4, 4, false, false, false>(g, u.dwg, u.dwu, s)
-                    : launch_gemm<DT, 2, 2, 2, 2, false, false, false>(g, u.dwg, u.dwu, s);
+    const UnitParts way = unit_parts(u.M, u.D, u.F, u.dtype);
+    float* const sums = way.parts > 1 ? u.sums : nullptr;
+    e = way.tile == 0   ? launch_gemm<DT, 2, 4, 8, 4, false, false, false>(g, u.dwg, u.dwu, s, way.parts, sums)
+        : way.tile == 1 ? launch_gemm<DT, 2, 2, 4, 4, false, false, false>(g, u.dwg, u.dwu, s, way.parts, sums)
+                        : launch_gemm<DT, 2, 2, 2, 2, false, false, false>(g, u.dwg, u.dwu, s, way.parts, sums);
+    using T = typename Elem<DT>::T;
+    const int64_t n = (int64_t)u.D * u.F;
+    if (e == hipSuccess && sums) k_unit_join<T><<<blocks_for(2 * n), 256, 0, s>>>(sums, way.parts, n, static_cast<T*>(u.dwg), static_cast<T*>(u.dwu));
     if (e != hipSuccess) return e;
   }
   return hipGetLastError();

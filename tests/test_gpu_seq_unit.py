@@ -157,3 +157,12 @@ def test_captured_training_step(unit):
         want = step()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want)), i
+
+
+@pytest.mark.parametrize('dtype', [BF16, FP16, FP32])
+@pytest.mark.parametrize('shape', [(1024, 40, 72), (5000, 64, 96), (33001, 24, 33), (9999, 300, 260)])
+def test_many_rows_of_a_narrow_layer(unit, shape, dtype):
+    """The weights' gradients summed in parts: few tiles, a long sum, its parts not of one length."""
+    M, D, F = shape
+    x, wg, wu, dy = _inputs(M, D, F, dtype, seed=31)
+    _check(unit, x, wg, wu, dy, 'silu')
