@@ -28,8 +28,22 @@ namespace {
 
 // rows of n values with the stride ld, as rows of n8 >= n values, the rest zero: 16-bit values as they are, f32 as three planes
 // (`plane` elements apart)
+struct CopyJob {
+  const void* src;
+  __bf16* dst;
+  int64_t ld, rows, n8, plane;
+  int n;
+};
+struct CopyJobs {   // one launch for up to three operands: blockIdx.y
+  CopyJob job[3];
+};
 template <int DT>
-__global__ __launch_bounds__(256) void k_unit_copy(const void* src, int64_t ld, int64_t rows, int n, int64_t n8, __bf16* dst, int64_t plane) {
+__global__ __launch_bounds__(256) void k_unit_copy(CopyJobs jobs) {
+  const CopyJob& job = jobs.job[blockIdx.y];
+  const void* const src = job.src;
+  __bf16* const dst = job.dst;
+  const int64_t ld = job.ld, rows = job.rows, n8 = job.n8, plane = job.plane;
+  const int n = job.n;
   using T = typename Elem<DT>::T;
   const T* s = static_cast<const T*>(src);
   const int64_t pieces = n8 / 8, all = rows * pieces;
@@ -231,8 +245,20 @@ unsigned blocks_for(int64_t n) {
 }
 
 template <int DT>
-void copy(const void* src, int64_t ld, int64_t rows, int n, int64_t n8, char* dst, hipStream_t s) {
-  if (rows && n8) k_unit_copy<DT><<<blocks_for(rows * n8 / 8), 256, 0, s>>>(src, ld, rows, n, n8, reinterpret_cast<__bf16*>(dst), rows * n8);
+void copies(const UnitArgs& u, hipStream_t s) {
+  CopyJobs jobs = {};
+  int count = 0;
+  int64_t most = 0;
+  auto add = [&](const void* src, int64_t ld, int64_t rows, int n, int64_t n8, char* dst) {
+    jobs.job[count++] = {src, reinterpret_cast<__bf16*>(dst), ld, rows, n8, rows * n8, n};
+    most = rows * n8 / 8 > most ? rows * n8 / 8 : most;
+  };
+  if (u.copy_x) add(u.x, u.x_ld, u.M, u.D, u.D8, u.xp);
+  if (u.copy_w) {
+    add(u.wg, u.w_ld, u.D, u.F, u.F8, u.wgp);
+    add(u.wu, u.wu_ld, u.D, u.F, u.F8, u.wup);
+  }
+  if (most) k_unit_copy<DT><<<dim3(blocks_for(most), (unsigned)count), 256, 0, s>>>(jobs);
 }
 
 template <class F>
@@ -289,11 +315,7 @@ hipError_t launch_gemm(GemmArgs g, void* c0, void* c1, hipStream_t s, int parts 
 
 template <int DT>
 hipError_t forward(const UnitArgs& u, hipStream_t s) {
-  if (u.copy_x) copy<DT>(u.x, u.x_ld, u.M, u.D, u.D8, u.xp, s);
-  if (u.copy_w) {
-    copy<DT>(u.wg, u.w_ld, u.D, u.F, u.F8, u.wgp, s);
-    copy<DT>(u.wu, u.wu_ld, u.D, u.F, u.F8, u.wup, s);
-  }
+  copies<DT>(u, s);
   GemmArgs g = {};
   g.M = u.M, g.N = u.F, g.K = u.D;
   g.planes = DT == SEQ_FP32 ? 3 : 1;
@@ -317,11 +339,7 @@ hipError_t backward(const UnitArgs& u, hipStream_t s) {
     return hipGetLastError();
   });
   if (e != hipSuccess) return e;
-  if (u.copy_x) copy<DT>(u.x, u.x_ld, u.M, u.D, u.D8, u.xp, s);
-  if (u.copy_w) {
-    copy<DT>(u.wg, u.w_ld, u.D, u.F, u.F8, u.wgp, s);
-    copy<DT>(u.wu, u.wu_ld, u.D, u.F, u.F8, u.wup, s);
-  }
+  copies<DT>(u, s);
   if (u.dx) {
     GemmArgs g = {};
     g.M = u.M, g.N = u.D, g.K = u.F;
