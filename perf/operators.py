@@ -278,19 +278,12 @@ def _plain_dropout(x, p, seed, offset, residual):
 
 # ------------------------------------------------------------------------------------------------- one pass
 
-_modules = None
-
-
 def _package():
-    """The entry points, imported once as at the top of a user's program."""
-    global _modules
-    if _modules is None:
-        path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), 'admm-lstm_amd')
-        if path not in sys.path:
-            sys.path.insert(0, path)
-        from blocks import delta_rule, dropout, gated_unit
-        _modules = delta_rule, gated_unit, dropout
-    return _modules
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), 'admm-lstm_amd')
+    if path not in sys.path:
+        sys.path.insert(0, path)
+    from blocks import delta_rule, dropout, gated_unit
+    return delta_rule, gated_unit, dropout
 
 
 def run(s):
