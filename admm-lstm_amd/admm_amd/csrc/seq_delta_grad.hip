@@ -11,8 +11,9 @@
 //     dk = exp(G - G_i) u dS^T - exp(G_i) beta dR S^T + m^T Q + (n + n^T) K
 //     dbeta_i = dR_i . v_i - exp(G_i) k_i . (S dR_i) - sum_j D_ij N_ij (k_i . k_j)
 //     dG_i = q_i . (scale exp(G_i) S do_i) - beta_i exp(G_i) k_i . (S dR_i) - exp(G - G_i) k_i . (dS u_i)
-//            + sum_j (m q.k + n k.k)_ij - sum_j (m q.k + n k.k)_ji
+//            + sum_{j < i} (m q.k + n k.k)_ij - sum_{j > i} (m q.k + n k.k)_ji
 //     dG += exp(G) <S, dS> + sum_i exp(G - G_i) k_i . (dS u_i),    dg_t = dG + sum_{i >= t} dG_i.
+// (The diagonal has no decay in it: it would cancel in dG_i, but leave its rounding in a dg that strong decays make small.)
 #include "seq_delta_dev.hpp"
 
 namespace seq {
@@ -493,7 +494,7 @@ __global__ __launch_bounds__(4 * C, C == 64 ? 2 : 1) void k_delta_grad(DeltaGrad
         const float m = row >= j ? a.scale * d * M[i][r] : 0.f;
         const float nb = row > j ? -d * N[i][r] : 0.f;
         const float nn = bet[row] * nb;
-        const float e = row >= j ? fmaf(m, qk[i][r], nn * kk[i][r]) : 0.f;
+        const float e = row > j ? fmaf(m, qk[i][r], nn * kk[i][r]) : 0.f;
         csum += e;
         const float rs = sum16(e), rb = sum16(row > j ? nb * kk[i][r] : 0.f);
         if (x == 0) {

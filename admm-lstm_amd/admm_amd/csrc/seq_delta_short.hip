@@ -582,7 +582,7 @@ __global__ __launch_bounds__(256, KP == 128 ? 1 : 2) void k_delta_short_grad(Del
       const float d = row >= c ? expf((sv->ghi[row] - sv->ghi[c]) + (sv->glo[row] - sv->glo[c])) : 0.f;
       const float mv = row >= c ? a.scale * d * M[r] : 0.f;
       const float nb = row > c ? -d * N[r] : 0.f, nn = sv->beta[row] * nb;
-      const float e = row >= c ? fmaf(mv, qk[r], nn * kk[r]) : 0.f;
+      const float e = row > c ? fmaf(mv, qk[r], nn * kk[r]) : 0.f;
       csum += e;
       const float se = sum16(e), sb = sum16(row > c ? nb * kk[r] : 0.f);
       if (x == 0 && wave < 3) {
