@@ -2,8 +2,8 @@
 //
 // C = sum over segments of A_s B_s, A_s [M, K], B_s [K, N], each operand stored along either axis: its tiles go from global
 // memory straight into LDS as they are stored (16 bytes a lane, pieces swizzled), and an operand whose inner axis is not the
-// contiguous one is transposed on its way out of LDS.  Segments are the two halves of an inner axis (gradient of x) and, for
-// f32 operands held as three bf16 planes, the six plane pairs (seq_dev.hpp).
+// contiguous one is transposed on its way out of LDS.  Segments are the two halves of an inner axis (gradient of x) and the pairs
+// of planes (seq_dev.hpp): six for f32 operands held as three bf16 planes, three for two planes (gradients of fp16).
 //
 // Operands are swapped in the matrix instruction (A = B^T tile), so that a lane ends up with four neighbouring columns of one row
 // of C: 8- or 16-byte stores.
@@ -18,7 +18,7 @@ struct GemmArgs {
   const char *a[2][3], *b[2][3];   // [matrix][plane]
   int64_t lda, ldb;                // in elements
   int M, N, K;
-  int planes;                      // 1, or 3 (six plane pairs)
+  int planes;                      // 1, 2 (three plane pairs) or 3 (six)
   int tiles_m, tiles_n;
 };
 
@@ -129,7 +129,7 @@ struct Gemm {
   __device__ static void run(const GemmArgs& g, int tm, int tn, int b_of, char* lds, f32x4 (&acc)[MT][NT]) {
     const int lane = threadIdx.x & 63, wave = wave_id(), x = lane & 15, q = lane >> 4;
     const int wm = wave / WN, wn = wave % WN;
-    const int kt = (g.K + kBK - 1) / kBK, terms = g.planes == 1 ? 1 : 6, total = kt * terms * (SPLIT ? 2 : 1);
+    const int kt = (g.K + kBK - 1) / kBK, terms = g.planes * (g.planes + 1) / 2, total = kt * terms * (SPLIT ? 2 : 1);
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -144,10 +144,10 @@ struct Gemm {
     const char *pa = nullptr, *pb = nullptr, *pb1 = nullptr;
     auto issue = [&](char* buf) {
       if (left <= 0) {
-        const int mat = SPLIT ? seg / terms : 0, term = SPLIT ? seg % terms : seg;
-        // plane pairs, smallest first: (2,0) (0,2) (1,1) (1,0) (0,1) (0,0)
-        const int ia = terms == 1 ? 0 : term == 0 ? 2 : term == 2 || term == 3 ? 1 : 0;
-        const int ib = terms == 1 ? 0 : term == 1 ? 2 : term == 2 || term == 4 ? 1 : 0;
+        const int mat = SPLIT ? seg / terms : 0, term = (SPLIT ? seg % terms : seg) + 6 - terms;
+        // plane pairs, smallest first: (2,0) (0,2) (1,1) (1,0) (0,1) (0,0); of two planes the last three, of one the last
+        const int ia = term == 0 ? 2 : term == 2 || term == 3 ? 1 : 0;
+        const int ib = term == 1 ? 2 : term == 2 || term == 4 ? 1 : 0;
         pa = g.a[mat][ia] + a0;
         pb = g.b[SPLIT ? mat : b_of][ib] + b0;
         pb1 = g.b[1][ib] + b0;

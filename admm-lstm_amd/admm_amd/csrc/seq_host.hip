@@ -194,12 +194,12 @@ int unit_sizes(const SeqUnit* u, bool backward, UnitSizes& z) {
     return fail(SEQ_EINVAL, "weights of %d x %d: 1 to %d are supported", u->D, u->F, SEQ_UNIT_MAX);
   if (u->M / 64 + 1 > kMaxBlocks / (u->F / 64 + 1) || u->M / 64 + 1 > kMaxBlocks / (u->D / 64 + 1))
     return fail(SEQ_EINVAL, "too many rows for one launch");
-  const int np = u->dtype == SEQ_FP32 ? 3 : 1;
+  const int np = u->dtype == SEQ_FP32 ? 3 : backward && u->dtype == SEQ_FP16 ? 2 : 1;   // planes of x and the weights
   z.D8 = (u->D + 7) / 8 * 8;
   z.F8 = (u->F + 7) / 8 * 8;
   // rows that loads of 16 bytes at 32-bit offsets do not fit
-  z.copy_x = np == 3 || !aligned16(u->x) || u->x_ld % 8 || u->D % 8 || u->x_ld > 1 << 22;
-  z.copy_w = np == 3 || !aligned16(u->wg) || !aligned16(u->wu) || u->wg_ld % 8 || u->wu_ld != u->wg_ld || u->F % 8 || u->wg_ld > 1 << 22;
+  z.copy_x = np > 1 || !aligned16(u->x) || u->x_ld % 8 || u->D % 8 || u->x_ld > 1 << 22;
+  z.copy_w = np > 1 || !aligned16(u->wg) || !aligned16(u->wu) || u->wg_ld % 8 || u->wu_ld != u->wg_ld || u->F % 8 || u->wg_ld > 1 << 22;
   z.x = z.copy_x ? up256(u->M * z.D8 * 2 * np) : 0;
   z.w = z.copy_w ? up256(u->D * z.F8 * 2 * np) : 0;
   z.da = backward ? up256(u->M * z.F8 * 2 * np) : 0;

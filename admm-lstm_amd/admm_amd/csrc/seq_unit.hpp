@@ -8,7 +8,7 @@ struct UnitArgs {
   int M, D, F, act, dtype;
   const void *x, *wg, *wu;
   int64_t x_ld, w_ld, wu_ld;
-  bool copy_x, copy_w;          // operands that need padded copies (f32: always, as planes)
+  bool copy_x, copy_w;          // operands that need padded copies (those held as planes: always)
   char *xp, *wgp, *wup;         // their copies
   int64_t D8, F8;               // row lengths of the copies, in elements
   float *pre;                   // a, then b [M, F] (NULL: not kept)
@@ -40,7 +40,7 @@ inline int tile_for(int64_t m, int64_t n, bool with3, int parts, double* time) {
 }
 
 // dWg and dWu have few tiles where the layer is narrow, and sum over all M rows: the sums are formed in parts, which a second
-// kernel adds up (in order), where that takes less time.  A round of 256 x 256 takes 30 ns a row (f32: six times that), the parts
+// kernel adds up (in order), where that takes less time.  A round of 256 x 256 takes 30 ns a row (fp16: three times that, f32: six), the parts
 // are written and read at memory's rate, and another launch takes 5 us.  All gradients together, in us, and with one part:
 //   f32: 262144 x 256 x 512: 2431 (19342), 65536 x 128 x 256: 351 (3723), 8192 x 512 x 1365: 621 (790), 1500 x 256 x 512: 102 (130);
 //   bf16: 724 (3483), 111 (561), 174 (190), 61 (57).
@@ -53,7 +53,7 @@ inline UnitParts unit_parts(int64_t M, int D, int F, int dtype) {
   for (int p = 1; p <= 64 && (p == 1 || M / p >= 512); p *= 2) {
     double rounds;
     const int tile = tile_for(D, 2 * (int64_t)F, false, p, &rounds);
-    const double us = rounds / p * M * (dtype == SEQ_FP32 ? 0.18 : 0.03) + (p > 1 ? 5 + p * 16e-6 * D * F / 5 : 0);
+    const double us = rounds / p * M * (dtype == SEQ_FP32 ? 0.18 : dtype == SEQ_FP16 ? 0.09 : 0.03) + (p > 1 ? 5 + p * 16e-6 * D * F / 5 : 0);
     if (p == 1 || us < least) best = {tile, p}, least = us;
   }
   return best;

@@ -3,13 +3,18 @@
 //
 // Forward: a workgroup forms the same tile of both projections (one tile of x in LDS serves both) and only their product
 // leaves it; where gradients follow, the projections a = x Wg and b = x Wu are kept too, in f32 (rounded to 16 bits they would
-// cost the gradients more than their own rounding).  Backward: da = dy b act'(a) and db = dy act(a) elementwise, rounded to
-// the inputs' type (one rounding more than the result's own), then dx = da Wg^T + db Wu^T as one product over both, and
-// dWg = x^T da, dWu = x^T db in one launch (in parts of the rows where the layer is narrow, unit_parts).
+// cost the gradients more than their own rounding).  Backward: da = dy b act'(a) and db = dy act(a) elementwise, then
+// dx = da Wg^T + db Wu^T as one product over both, and dWg = x^T da, dWu = x^T db in one launch (in parts of the rows where the
+// layer is narrow, unit_parts).  da and db are held
+//   in bf16 as bf16: one rounding more than the result's own (1.4 times its error), for half the products of two planes;
+//   in fp16 as two bf16 planes, 16 bits, x and W too (exactly): da has a range of its own, products of three values, and fp16 would
+//     lose small gradients and overflow where dx does not.  Three products for one (seq_dev.hpp): all gradients of 8192 x 2048 x
+//     8192 take 2.9 ms, with da and db in fp16 1.2 ms;
+//   in f32 as three.
 //
 // Bound by the matrix cores where the layer is wide (12 M D F operations a training step), by the weights where there are few
-// rows.  f32 operands are split into three bf16 planes by a pass before (six products, seq_dev.hpp), and 16-bit operands whose
-// rows are not 16-byte aligned are copied to padded rows.
+// rows.  Planes of the operands are formed by a pass before, and 16-bit operands whose rows are not 16-byte aligned are copied to
+// padded rows.
 //
 // 8192 x 2048 x 8192, bf16: forward with the projections kept 635 us (865 TFLOP/s; without them 550), dx 500 us and dWg, dWu 530 us
 // (1.1 and 1.04 PFLOP/s; a large library product reaches 1.2 to 1.3), the elementwise pass 204 us (4.6 TB/s).
@@ -26,8 +31,8 @@ namespace seq {
 
 namespace {
 
-// rows of n values with the stride ld, as rows of n8 >= n values, the rest zero: 16-bit values as they are, f32 as three planes
-// (`plane` elements apart)
+// rows of n values with the stride ld, as rows of n8 >= n values, the rest zero: 16-bit values as they are (NP = 1), or NP bf16
+// planes (`plane` elements apart)
 struct CopyJob {
   const void* src;
   __bf16* dst;
@@ -37,7 +42,7 @@ struct CopyJob {
 struct CopyJobs {   // one launch for up to three operands: blockIdx.y
   CopyJob job[3];
 };
-template <int DT>
+template <int DT, int NP>
 __global__ __launch_bounds__(256) void k_unit_copy(CopyJobs jobs) {
   const CopyJob& job = jobs.job[blockIdx.y];
   const void* const src = job.src;
@@ -53,13 +58,13 @@ __global__ __launch_bounds__(256) void k_unit_copy(CopyJobs jobs) {
     const int64_t r = small ? (uint32_t)i / (uint32_t)pieces : i / pieces, p = i - r * pieces;
     const int left = n - (int)(8 * p);
     __bf16* d = dst + r * n8 + 8 * p;
-    if constexpr (DT == SEQ_FP32) {
+    if constexpr (NP > 1) {
       f32x8 v = {};
       if (left > 0) v = load8(s + r * ld + 8 * p, left, wide);
-      bf16x8 pl[3];
-      planes8<3>(v, pl);
+      bf16x8 pl[NP];
+      planes8<NP>(v, pl);
 #pragma unroll
-      for (int j = 0; j < 3; ++j) *reinterpret_cast<bf16x8*>(d + j * plane) = pl[j];
+      for (int j = 0; j < NP; ++j) *reinterpret_cast<bf16x8*>(d + j * plane) = pl[j];
     } else {
       const uint16_t* h = reinterpret_cast<const uint16_t*>(s) + r * ld + 8 * p;
       uint16_t v[8];
@@ -144,11 +149,14 @@ __global__ __launch_bounds__(64 * WM * WN) void k_unit(GemmArgs g, typename Elem
     }
 }
 
+// the matrix instructions' operands in the products of the gradients: bf16 or planes of it
+template <int DT> constexpr int kGradType = DT == SEQ_FP16 ? SEQ_BF16 : DT;
+
 // AI, BI, SPLIT as in Gemm; otherwise blockIdx.y picks the matrix B and the result, and blockIdx.z a part of the inner axis, whose
 // sums go to `sums` [part][matrix][M][N] where there are several
 template <int DT, int WM, int WN, int MT, int NT, bool AI, bool BI, bool SPLIT>
 __global__ __launch_bounds__(64 * WM * WN) void k_unit_gemm(GemmArgs g, typename Elem<DT>::T* c0, typename Elem<DT>::T* c1, float* sums, bool wide) {
-  using G = Gemm<DT, WM, WN, MT, NT, AI, BI, false, SPLIT>;
+  using G = Gemm<kGradType<DT>, WM, WN, MT, NT, AI, BI, false, SPLIT>;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lane = threadIdx.x & 63, wave = wave_id(), x = lane & 15, q = lane >> 4, wm = wave / WN, wn = wave % WN;
   int tm, tn;
@@ -200,7 +208,7 @@ __global__ __launch_bounds__(256) void k_unit_join(const float* sums, int parts,
   }
 }
 
-// da = dy b act'(a), db = dy act(a), as rows of F8 values (f32: planes)
+// da = dy b act'(a), db = dy act(a), as rows of F8 values, in bf16 planes
 template <int DT, int ACT>
 __global__ __launch_bounds__(256) void k_unit_back(UnitArgs u) {
   using T = typename Elem<DT>::T;
@@ -222,19 +230,14 @@ __global__ __launch_bounds__(256) void k_unit_back(UnitArgs u) {
       db[j] = j < left ? d[j] * f : 0.f;
     }
     const int64_t at = r * u.F8 + 8 * p;
-    if constexpr (DT == SEQ_FP32) {
-      bf16x8 pa[3], pb[3];
-      planes8<3>(da, pa);
-      planes8<3>(db, pb);
+    constexpr int NP = Elem<DT>::kPlanes;
+    bf16x8 pa[NP], pb[NP];
+    planes8<NP>(da, pa);
+    planes8<NP>(db, pb);
 #pragma unroll
-      for (int j = 0; j < 3; ++j) {
-        *reinterpret_cast<bf16x8*>(reinterpret_cast<__bf16*>(u.dap) + j * plane + at) = pa[j];
-        *reinterpret_cast<bf16x8*>(reinterpret_cast<__bf16*>(u.dbp) + j * plane + at) = pb[j];
-      }
-    } else {
-      typedef T T8 __attribute__((ext_vector_type(8)));
-      *reinterpret_cast<T8*>(reinterpret_cast<T*>(u.dap) + at) = __builtin_convertvector(da, T8);
-      *reinterpret_cast<T8*>(reinterpret_cast<T*>(u.dbp) + at) = __builtin_convertvector(db, T8);
+    for (int j = 0; j < NP; ++j) {
+      *reinterpret_cast<bf16x8*>(reinterpret_cast<__bf16*>(u.dap) + j * plane + at) = pa[j];
+      *reinterpret_cast<bf16x8*>(reinterpret_cast<__bf16*>(u.dbp) + j * plane + at) = pb[j];
     }
   }
 }
@@ -244,7 +247,7 @@ unsigned blocks_for(int64_t n) {
   return (unsigned)(want < 256 * 32 ? want : 256 * 32);
 }
 
-template <int DT>
+template <int DT, int NP>
 void copies(const UnitArgs& u, hipStream_t s) {
   CopyJobs jobs = {};
   int count = 0;
@@ -258,7 +261,7 @@ void copies(const UnitArgs& u, hipStream_t s) {
     add(u.wg, u.w_ld, u.D, u.F, u.F8, u.wgp);
     add(u.wu, u.wu_ld, u.D, u.F, u.F8, u.wup);
   }
-  if (most) k_unit_copy<DT><<<dim3(blocks_for(most), (unsigned)count), 256, 0, s>>>(jobs);
+  if (most) k_unit_copy<DT, NP><<<dim3(blocks_for(most), (unsigned)count), 256, 0, s>>>(jobs);
 }
 
 template <class F>
@@ -303,7 +306,7 @@ hipError_t launch_unit(GemmArgs g, const UnitArgs& u, hipStream_t s) {
 template <int DT, int WM, int WN, int MT, int NT, bool AI, bool BI, bool SPLIT>
 hipError_t launch_gemm(GemmArgs g, void* c0, void* c1, hipStream_t s, int parts = 1, float* sums = nullptr) {
   using T = typename Elem<DT>::T;
-  using G = Gemm<DT, WM, WN, MT, NT, AI, BI, false, SPLIT>;
+  using G = Gemm<kGradType<DT>, WM, WN, MT, NT, AI, BI, false, SPLIT>;
   tiles(g, G::BM, G::BN);
   auto* f = k_unit_gemm<DT, WM, WN, MT, NT, AI, BI, SPLIT>;
   const hipError_t e = lds_for(f, G::kLds);
@@ -315,10 +318,11 @@ hipError_t launch_gemm(GemmArgs g, void* c0, void* c1, hipStream_t s, int parts 
 
 template <int DT>
 hipError_t forward(const UnitArgs& u, hipStream_t s) {
-  copies<DT>(u, s);
+  constexpr int np = DT == SEQ_FP32 ? 3 : 1;
+  copies<DT, np>(u, s);
   GemmArgs g = {};
   g.M = u.M, g.N = u.F, g.K = u.D;
-  g.planes = DT == SEQ_FP32 ? 3 : 1;
+  g.planes = np;
   g.lda = u.copy_x ? u.D8 : u.x_ld;
   g.ldb = u.copy_w ? u.F8 : u.w_ld;
   planes(g.a[0], u.copy_x, u.x, u.xp, u.M * u.D8);
@@ -333,13 +337,13 @@ hipError_t forward(const UnitArgs& u, hipStream_t s) {
 
 template <int DT>
 hipError_t backward(const UnitArgs& u, hipStream_t s) {
-  constexpr int np = DT == SEQ_FP32 ? 3 : 1;
+  constexpr int np = Elem<DT>::kPlanes;
   hipError_t e = !u.M ? hipSuccess : for_act(u.act, [&](auto act) {
     k_unit_back<DT, decltype(act)::value><<<blocks_for(u.M * u.F8 / 8), 256, 0, s>>>(u);
     return hipGetLastError();
   });
   if (e != hipSuccess) return e;
-  copies<DT>(u, s);
+  copies<DT, np>(u, s);
   if (u.dx) {
     GemmArgs g = {};
     g.M = u.M, g.N = u.D, g.K = u.F;
