@@ -62,6 +62,21 @@ __device__ __forceinline__ void planes8(f32x8 x, bf16x8 (&p)[NP]) {
   }
 }
 
+// The same of any finite values: the first plane of those above the largest bf16 value, which would be infinite, is that value.  An
+// infinity has NaN among its planes.
+template <int NP>
+__device__ __forceinline__ void planes8_whole(f32x8 x, bf16x8 (&p)[NP]) {
+  constexpr float kMost = 0x1.fep127f;
+  f32x8 c;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) c[i] = __builtin_amdgcn_fmed3f(x[i], -kMost, kMost);
+  p[0] = __builtin_convertvector(c, bf16x8);
+  static_assert(NP == 3, "two planes and a remainder");
+  const f32x8 r = x - admm::bf16_widen<f32x8>(p[0]);
+  p[1] = __builtin_convertvector(r, bf16x8);
+  p[2] = __builtin_convertvector(r - admm::bf16_widen<f32x8>(p[1]), bf16x8);
+}
+
 __device__ __forceinline__ f32x8 cat8(f32x4 a, f32x4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
 
 // acc += a b over the plane pairs i + j < L, the smallest terms first

@@ -4,7 +4,8 @@
 // A lane loads 8 rows of 8 neighbouring weights (rows 8 g..8 g + 7 of the inner axis, columns 8 x..8 x + 7) straight into
 // registers, 16 bytes a row whatever their alignment, and turns its 8 x 8 block over there (32 byte permutes): fragment j then has
 // the weights of columns 8 x + j as the matrix instruction wants them, and eight of those make 128 columns.  f32 weights need no
-// turning over: v_mfma_f32_16x16x4_f32 takes one weight a lane, at columns 4 x + j.  The rows of x are the other operand.
+// turning over: v_mfma_f32_16x16x4_f32 takes one weight a lane, at columns 4 x + j.  The rows of x are the other operand.  (An infinity
+// of f32 is made NaN, which it is as planes in the kernels of more rows: the result does not depend on the number of rows.)
 // The inner axis is split over the four waves of a workgroup and over workgroups, so that the loads in flight fill the memory
 // system; where it is split over workgroups their sums go through work memory and are joined by k_unit_sum, in order.
 #include "seq_dev.hpp"
@@ -27,6 +28,9 @@ __device__ __forceinline__ V load_any(const void* p) {   // of any alignment
   __builtin_memcpy(&v, p, sizeof v);
   return v;
 }
+
+// NaN for an infinity, any other value as it is
+__device__ __forceinline__ float finite_or_nan(float v) { return fmaf(v, 0.f, v); }
 
 // 16 bytes of a row of n values from value c on, zeros outside
 template <class T>
@@ -74,13 +78,15 @@ __global__ __launch_bounds__(64 * kWavesF) void k_unit_few(UnitArgs u, int split
         for (int i = 0; i < 4; ++i) {
           const int k = k0 + 4 * i + g;
           b[e][i] = __builtin_bit_cast(f32x4, k < u.D && col < u.F ? load_piece<T>(w[e] + k * ld[e], col, u.F) : u32x4{0, 0, 0, 0});
+#pragma unroll
+          for (int j = 0; j < 4; ++j) b[e][i][j] = finite_or_nan(b[e][i][j]);
         }
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int k = k0 + 4 * i + g;
-          const float xv = k < u.D ? xr[m][k] : 0.f;
+          const float xv = k < u.D ? finite_or_nan(xr[m][k]) : 0.f;
 #pragma unroll
           for (int e = 0; e < 2; ++e)
 #pragma unroll

@@ -62,7 +62,8 @@ __global__ __launch_bounds__(256) void k_unit_copy(CopyJobs jobs) {
       f32x8 v = {};
       if (left > 0) v = load8(s + r * ld + 8 * p, left, wide);
       bf16x8 pl[NP];
-      planes8<NP>(v, pl);
+      if constexpr (DT == SEQ_FP32) planes8_whole<NP>(v, pl);
+      else planes8<NP>(v, pl);
 #pragma unroll
       for (int j = 0; j < NP; ++j) *reinterpret_cast<bf16x8*>(d + j * plane) = pl[j];
     } else {
@@ -232,8 +233,13 @@ __global__ __launch_bounds__(256) void k_unit_back(UnitArgs u) {
     const int64_t at = r * u.F8 + 8 * p;
     constexpr int NP = Elem<DT>::kPlanes;
     bf16x8 pa[NP], pb[NP];
-    planes8<NP>(da, pa);
-    planes8<NP>(db, pb);
+    if constexpr (DT == SEQ_FP32) {
+      planes8_whole<NP>(da, pa);
+      planes8_whole<NP>(db, pb);
+    } else {
+      planes8<NP>(da, pa);
+      planes8<NP>(db, pb);
+    }
 #pragma unroll
     for (int j = 0; j < NP; ++j) {
       *reinterpret_cast<bf16x8*>(reinterpret_cast<__bf16*>(u.dap) + j * plane + at) = pa[j];

@@ -57,3 +57,39 @@ def test_gradients_of_fp16_whose_parts_are_beyond_it(unit):
 @pytest.mark.parametrize('shape', [(40, 33, 65), (2300, 320, 2052), (33001, 24, 33)])
 def test_gradients_of_fp16_in_every_tile_and_in_parts(unit, shape):
     _check_fp16(unit, *shape, 1.0, 1e-4, 'silu')
+
+
+def _fp32(M, D, F, x_size, w_size, dy_size):
+    gen = torch.Generator().manual_seed(112)
+    return [torch.randn(s, generator=gen) * f for s, f in (((M, D), x_size), ((D, F), w_size), ((D, F), w_size), ((M, F), dy_size))]
+
+
+@pytest.mark.parametrize('M', [5, 100])
+def test_the_largest_values_of_fp32(unit, M):
+    """Those above the largest bf16 value (3.39e38) would be infinities as bf16; weights and dy are so small that all results are in
+    range, with as much room below."""
+    D, F = 24, 40
+    x, wg, wu, dy = (t.cuda() for t in _fp32(M, D, F, 1.2e38, 1e-30, 1e-12))
+    x.clamp_(-torch.finfo(FP32).max, torch.finfo(FP32).max)
+    x[::2, 3], x[1::2, 5] = torch.finfo(FP32).max, -3.398e38
+    y = unit(x, wg, wu)
+    R.assert_close('y', y, R.gated_unit(x.cpu(), wg.cpu(), wu.cpu(), 'silu'), R.unit_atol(D))
+    got, want = _gradients(unit, x, wg, wu, dy, 'silu')
+    for n, a, b, (more, atol) in zip(('dx', 'dwg', 'dwu'), got, want, R.unit_grad_bounds(x, wg, wu, dy, 'silu')):
+        R.assert_close(n, a, b, atol, more)
+
+
+@pytest.mark.parametrize('M', [5, 100])
+def test_an_infinity_of_fp32_counts_as_nan(unit, M):
+    """Whichever kernel the number of rows leads to."""
+    x, wg, wu, _ = (t.cuda() for t in _fp32(M, 24, 40, 1.0, 0.2, 1.0))
+    clean = unit(x, wg, wu, activation='sigmoid')
+    for value in (float('inf'), -float('inf')):
+        for t, at, hit in ((x, (3, 7), (3, slice(None))), (wg, (23, 9), (slice(None), 9)), (wu, (0, 39), (slice(None), 39))):
+            was = t[at].clone()
+            t[at] = value
+            y = unit(x, wg, wu, activation='sigmoid')
+            t[at] = was
+            gone = torch.zeros_like(y, dtype=torch.bool)
+            gone[hit] = True
+            assert torch.equal(torch.isnan(y), gone) and torch.equal(y[~gone], clean[~gone])
