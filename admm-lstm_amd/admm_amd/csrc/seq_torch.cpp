@@ -52,10 +52,23 @@ void check(int rc, const char* what) {
   if (rc) throw SeqError(say(what, " failed (code ", rc, "): ", seq_last_error()), rc);
 }
 
+// Derivatives in forward mode would be lost: the kernels read the values alone.
+constexpr const char* kNoForwardMode = " carries a forward-mode derivative, which this operator does not propagate (use backward mode)";
+bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
+
 Tensor tensor(const py::handle& h, const char* name) {
   if (!THPVariable_Check(h.ptr()))
     throw py::type_error(say(name, " must be a tensor (got ", Py_TYPE(h.ptr())->tp_name, ")"));
-  return THPVariable_Unpack(h.ptr());
+  const Tensor& t = THPVariable_Unpack(h.ptr());
+  if (has_tangent(t)) {
+    PyErr_SetString(PyExc_NotImplementedError, say(name, kNoForwardMode).c_str());
+    throw py::error_already_set();
+  }
+  return t;
+}
+// the gradients that a backward pass begins with
+void check_given(const variable_list& d_out) {
+  for (const Tensor& t : d_out) TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent(t), "a gradient", kNoForwardMode);
 }
 Tensor maybe(const py::handle& h, const char* name) { return h.is_none() ? Tensor() : tensor(h, name); }
 
@@ -169,6 +182,7 @@ struct RuleFunction : torch::autograd::Function<RuleFunction> {
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& d_out) {
     const variable_list in = ctx->get_saved_variables();
+    check_given(d_out);
     RuleCall call(in[0], in[1], in[2], in[3], in[4], in[5], in[6], ctx->saved_data["scale"].toDouble());
     const Tensor work = in[7];
     Tensor d_o = d_out[0].defined() ? d_out[0].contiguous() : at::zeros(call.v.sizes(), call.v.options());
@@ -311,6 +325,7 @@ struct UnitFunction : torch::autograd::Function<UnitFunction> {
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& d_out) {
     const variable_list in = ctx->get_saved_variables();
+    check_given(d_out);
     UnitCall call(in[0], in[1], in[2], (int)ctx->saved_data["act"].toInt());
     const Tensor pre = in[3], dy = rows_last(d_out[0]), w = call.work(true);
     variable_list grads(4);
@@ -372,6 +387,7 @@ struct DropoutFunction : torch::autograd::Function<DropoutFunction> {
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& d_out) {
     const variable_list in = ctx->get_saved_variables();
+    check_given(d_out);
     variable_list grads(6);
     if (ctx->needs_input_grad(0))
       grads[0] = run_dropout(d_out[0].contiguous(), Tensor(), ctx->saved_data["below"].toInt(), ctx->saved_data["seed"].toInt(), in[0],

@@ -1,0 +1,34 @@
+"""What the sequence-layer operators refuse of PyTorch's transformations, which would otherwise lose their results without a word.
+Without a GPU: these are refused before anything is computed."""
+import pytest
+import torch
+
+
+def _calls():
+    """Each operator's arguments, and a call of them."""
+    from blocks.delta_rule import gated_delta_rule, gated_delta_step
+    from blocks.dropout import dropout
+    from blocks.gated_unit import gated_unit
+    rule = [torch.randn(2, 5, 1, 8), torch.randn(2, 5, 1, 8), torch.randn(2, 5, 2, 4), torch.randn(2, 5, 2), torch.randn(2, 5, 2)]
+    return {
+        'rule': (rule + [torch.randn(2, 2, 8, 4)], lambda *a: gated_delta_rule(*a[:5], initial_state=a[5])),
+        'step': ([x[:, 0] for x in rule] + [torch.randn(2, 2, 8, 4)], gated_delta_step),
+        'unit': ([torch.randn(3, 4), torch.randn(4, 5), torch.randn(4, 5)], gated_unit),
+        'dropout': ([torch.randn(3, 4), torch.randn(3, 4)], lambda x, r: dropout(x, 0.5, 1, residual=r)),
+    }
+
+
+ARGS = [('rule', i) for i in range(6)] + [('step', i) for i in range(6)] + [('unit', i) for i in range(3)] + [('dropout', i) for i in range(2)]
+
+
+@pytest.mark.parametrize('name, which', ARGS)
+@pytest.mark.parametrize('leaf', [False, True])
+def test_forward_mode_is_refused(name, which, leaf):
+    import torch.autograd.forward_ad as fw
+    args, call = _calls()[name]
+    if leaf:
+        args[which].requires_grad_()
+    with fw.dual_level():
+        args[which] = fw.make_dual(args[which], torch.ones_like(args[which]))
+        with pytest.raises(NotImplementedError, match='forward-mode'):
+            call(*args)
