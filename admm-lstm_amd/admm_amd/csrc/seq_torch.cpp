@@ -3,6 +3,7 @@
 // Python with ctypes took 25 us for a call without gradients, and 80 us for one with.
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <c10/hip/HIPStream.h>
 
@@ -60,6 +61,8 @@ Tensor tensor(const py::handle& h, const char* name) {
   if (!THPVariable_Check(h.ptr()))
     throw py::type_error(say(name, " must be a tensor (got ", Py_TYPE(h.ptr())->tp_name, ")"));
   const Tensor& t = THPVariable_Unpack(h.ptr());
+  // (a trace would have the allocation of the result and not the kernel that writes it)
+  if (torch::jit::tracer::isTracing()) throw std::runtime_error("the sequence-layer operators cannot be traced");
   if (has_tangent(t)) {
     PyErr_SetString(PyExc_NotImplementedError, say(name, kNoForwardMode).c_str());
     throw py::error_already_set();

@@ -32,3 +32,10 @@ def test_forward_mode_is_refused(name, which, leaf):
         args[which] = fw.make_dual(args[which], torch.ones_like(args[which]))
         with pytest.raises(NotImplementedError, match='forward-mode'):
             call(*args)
+
+
+@pytest.mark.parametrize('name', ['rule', 'step', 'unit', 'dropout'])
+def test_tracing_is_refused(name):
+    args, call = _calls()[name]
+    with pytest.raises(RuntimeError, match='traced'):
+        torch.jit.trace(call, tuple(args), check_trace=False)
