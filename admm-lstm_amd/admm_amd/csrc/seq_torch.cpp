@@ -63,6 +63,11 @@ Tensor tensor(const py::handle& h, const char* name) {
   const Tensor& t = THPVariable_Unpack(h.ptr());
   // (a trace would have the allocation of the result and not the kernel that writes it)
   if (torch::jit::tracer::isTracing()) throw std::runtime_error("the sequence-layer operators cannot be traced");
+  // batched, sparse and fake tensors, and subclasses that run PyTorch's operators in a way of their own (distributed ones): the values
+  // that a pointer leads to are none, or not what they stand for
+  const at::TensorImpl* impl = t.unsafeGetTensorImpl();
+  if (!impl->has_storage() || impl->is_python_dispatch() || t.layout() != at::kStrided)
+    throw py::type_error(say(name, " must be a dense tensor with memory of its own (got ", Py_TYPE(h.ptr())->tp_name, ", ", t.layout(), ")"));
   if (has_tangent(t)) {
     PyErr_SetString(PyExc_NotImplementedError, say(name, kNoForwardMode).c_str());
     throw py::error_already_set();

@@ -2,6 +2,7 @@
 Without a GPU: these are refused before anything is computed."""
 import pytest
 import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
 
 
 def _calls():
@@ -39,3 +40,21 @@ def test_tracing_is_refused(name):
     args, call = _calls()[name]
     with pytest.raises(RuntimeError, match='traced'):
         torch.jit.trace(call, tuple(args), check_trace=False)
+
+
+@pytest.mark.parametrize('name, which', ARGS)
+def test_tensors_without_memory_of_their_own_are_refused(name, which):
+    args, call = _calls()[name]
+    batched = list(args)
+    batched[which] = torch.stack([args[which]] * 3)
+    with pytest.raises(TypeError, match='memory of its own'):
+        torch.func.vmap(call, in_dims=tuple(0 if i == which else None for i in range(len(args))))(*batched)
+    sparse = list(args)
+    sparse[which] = args[which].to_sparse()
+    with pytest.raises(TypeError, match='memory of its own'):
+        call(*sparse)
+    with FakeTensorMode(allow_non_fake_inputs=True) as mode:
+        fake = list(args)
+        fake[which] = mode.from_tensor(args[which])
+        with pytest.raises(TypeError, match='memory of its own'):
+            call(*fake)
