@@ -72,7 +72,7 @@ Tensor tensor(const py::handle& h, const char* name) {
     PyErr_SetString(PyExc_NotImplementedError, say(name, kNoForwardMode).c_str());
     throw py::error_already_set();
   }
-  return t;
+  return t.resolve_neg();   // (the imaginary part of a conjugate is negated as it is read)
 }
 // the gradients that a backward pass begins with
 void check_given(const variable_list& d_out) {
@@ -193,8 +193,8 @@ struct RuleFunction : torch::autograd::Function<RuleFunction> {
     check_given(d_out);
     RuleCall call(in[0], in[1], in[2], in[3], in[4], in[5], in[6], ctx->saved_data["scale"].toDouble());
     const Tensor work = in[7];
-    Tensor d_o = d_out[0].defined() ? d_out[0].contiguous() : at::zeros(call.v.sizes(), call.v.options());
-    Tensor d_final = d_out[1].defined() ? d_out[1].contiguous() : Tensor();
+    Tensor d_o = d_out[0].defined() ? d_out[0].resolve_neg().contiguous() : at::zeros(call.v.sizes(), call.v.options());
+    Tensor d_final = d_out[1].defined() ? d_out[1].resolve_neg().contiguous() : Tensor();
     int64_t need = 0;
     check(seq_delta_backward_scratch(&call.d, &need), "gated_delta_rule");
     Tensor scratch = bytes(need, call.q);
@@ -256,6 +256,7 @@ Tensor gated_delta_step(const py::handle& q_, const py::handle& k_, const py::ha
   const at::NoGradGuard no_grad;
   Tensor q = tensor(q_, "q"), k = tensor(k_, "k"), v = tensor(v_, "v");
   const Tensor g = tensor(g_, "g"), beta = tensor(beta_, "beta"), state = tensor(state_, "state");
+  REQUIRE(!THPVariable_Unpack(state_.ptr()).is_neg(), "state must not be a view that is negated as it is read (it is updated in place)");
   Tensor slots = maybe(slots_, "slots");
   check_rows(q, k, v, g, beta, 1, "batch");
   const int64_t B = q.size(0), Hk = q.size(1), K = q.size(2), Hv = v.size(1), V = v.size(2);
@@ -335,7 +336,7 @@ struct UnitFunction : torch::autograd::Function<UnitFunction> {
     const variable_list in = ctx->get_saved_variables();
     check_given(d_out);
     UnitCall call(in[0], in[1], in[2], (int)ctx->saved_data["act"].toInt());
-    const Tensor pre = in[3], dy = rows_last(d_out[0]), w = call.work(true);
+    const Tensor pre = in[3], dy = rows_last(d_out[0].resolve_neg()), w = call.work(true);
     variable_list grads(4);
     if (ctx->needs_input_grad(0)) grads[0] = at::empty(in[0].sizes(), in[0].options());
     if (ctx->needs_input_grad(1) || ctx->needs_input_grad(2))
@@ -398,7 +399,7 @@ struct DropoutFunction : torch::autograd::Function<DropoutFunction> {
     check_given(d_out);
     variable_list grads(6);
     if (ctx->needs_input_grad(0))
-      grads[0] = run_dropout(d_out[0].contiguous(), Tensor(), ctx->saved_data["below"].toInt(), ctx->saved_data["seed"].toInt(), in[0],
+      grads[0] = run_dropout(d_out[0].resolve_neg().contiguous(), Tensor(), ctx->saved_data["below"].toInt(), ctx->saved_data["seed"].toInt(), in[0],
                              ctx->saved_data["offset"].toInt());
     if (ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(1)) grads[1] = d_out[0];
     return once(std::move(grads), "dropout");
@@ -425,7 +426,7 @@ Tensor dropout(const py::handle& x_, double p, const py::handle& seed_, const py
             shape(x.sizes()), " (got ", type(residual.scalar_type()), ", ", shape(residual.sizes()), ")");
   int64_t seed = 0;
   if (THPVariable_Check(seed_.ptr())) {
-    seed_device = THPVariable_Unpack(seed_.ptr());
+    seed_device = tensor(seed_, "seed");
     REQUIRE(seed_device.scalar_type() == at::kLong && seed_device.numel() == 1, "seed must be an integer or one int64 value (got ",
             type(seed_device.scalar_type()), ", shape ", shape(seed_device.sizes()), ")");
   } else {

@@ -29,3 +29,35 @@ def test_forward_mode_over_a_backward_pass_is_refused(name):
         dy = fw.make_dual(torch.ones_like(y), torch.ones_like(y))
         with pytest.raises(NotImplementedError, match='forward-mode'):
             torch.autograd.grad(y, leaves, dy)
+
+
+@pytest.mark.parametrize('name', ['rule', 'unit', 'dropout'])
+def test_views_with_the_sign_turned_are_read_with_it(name):
+    """The imaginary part of a conjugate is a view whose values PyTorch negates as they are read."""
+    args, call = _calls()[name]
+    dy = torch.randn_like(call(*args))
+    want = torch.autograd.grad(call(*(t.requires_grad_() for t in args)), args, dy)
+    y = call(*args).detach()
+    turned = [torch._neg_view(-t.detach()) for t in args]
+    assert all(t.is_neg() for t in turned)
+    assert torch.equal(call(*turned), y)
+    leaves = [(-t.detach()).requires_grad_() for t in args]
+    out = call(*(torch._neg_view(t) for t in leaves))
+    assert torch.equal(out.detach(), y)
+    got = torch.autograd.grad(out, leaves, torch._neg_view(-dy))
+    assert all(torch.equal(-a, b) for a, b in zip(got, want))
+    z = torch.complex(torch.zeros_like(args[0].detach()), -args[0].detach()).conj().imag   # as programs come by them
+    assert z.is_neg() and torch.equal(call(z, *args[1:]).detach(), y)
+
+
+def test_single_tokens_with_the_sign_turned():
+    from blocks.delta_rule import gated_delta_step
+    q, k, v, g, beta, s0 = R.delta_inputs(3, 1, 1, 2, 16, 24, torch.float32, seed=123)
+    args = [t[:, 0].contiguous() for t in (q, k, v, g, beta)]
+    state = s0.clone()
+    want = gated_delta_step(*args, state)
+    again = s0.clone()
+    assert torch.equal(gated_delta_step(*(torch._neg_view(-t) for t in args), again), want) and torch.equal(again, state)
+    turned = torch._neg_view(-s0)
+    with pytest.raises(ValueError, match='state'):
+        gated_delta_step(*args, turned)
