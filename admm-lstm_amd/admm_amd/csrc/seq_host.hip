@@ -189,7 +189,8 @@ int unit_sizes(const SeqUnit* u, bool backward, UnitSizes& z) {
   if (!u) return fail(SEQ_EINVAL, "NULL argument");
   if (u->dtype < SEQ_BF16 || u->dtype > SEQ_FP32) return fail(SEQ_EINVAL, "unknown dtype %d", u->dtype);
   if (u->act < SEQ_SILU || u->act > SEQ_SIGMOID) return fail(SEQ_EINVAL, "unknown activation %d", u->act);
-  if (u->M < 0 || u->M > kMaxBlocks) return fail(SEQ_EINVAL, "%lld rows: 0 to %lld are supported", (long long)u->M, (long long)kMaxBlocks);
+  if (u->M < 0) return fail(SEQ_EINVAL, "negative number of rows");
+  if (u->M > kUnitMaxRows) return fail(SEQ_EINVAL, "too many rows (%lld): up to %lld are supported", (long long)u->M, (long long)kUnitMaxRows);
   if (u->D < 1 || u->D > SEQ_UNIT_MAX || u->F < 1 || u->F > SEQ_UNIT_MAX)
     return fail(SEQ_EINVAL, "weights of %d x %d: 1 to %d are supported", u->D, u->F, SEQ_UNIT_MAX);
   if (u->M / 64 + 1 > kMaxBlocks / (u->F / 64 + 1) || u->M / 64 + 1 > kMaxBlocks / (u->D / 64 + 1))

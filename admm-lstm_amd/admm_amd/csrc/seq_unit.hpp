@@ -4,6 +4,8 @@
 
 namespace seq {
 
+constexpr int64_t kUnitMaxRows = 0x7fffffff - 255;   // row numbers up to the last tile's end are 32-bit integers
+
 struct UnitArgs {
   int M, D, F, act, dtype;
   const void *x, *wg, *wu;

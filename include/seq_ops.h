@@ -109,7 +109,7 @@ typedef struct SeqUnit {
   int64_t x_ld, wg_ld, wu_ld;
 } SeqUnit;
 
-#define SEQ_UNIT_MAX 1048576     /* largest D and F */
+#define SEQ_UNIT_MAX 1048576     /* largest D and F (M: up to 2^31 - 256) */
 
 /* Work memory of the forward (backward = 0) or the backward.  `pre` [2, M, F] float32 receives x Wg and x Wu for the
  * gradients, or is NULL.  dy [M, F] with the row stride dy_ld; dx [M, D], dwg and dwu [D, F] contiguous, dx and the pair dwg, dwu
