@@ -84,6 +84,9 @@ struct DeltaRows {
   }
 };
 
+// columns of a state that a workgroup of the single-token kernel takes (seq_step.hip has the measurements)
+inline int step_cols(int64_t heads, int V) { return V < 96 || heads < 1024 ? 32 : 128; }
+
 struct DeltaOutside {
   int n;
   void* p[5];

@@ -69,7 +69,7 @@ struct OnDevice {
 int elem_size(int dtype) { return dtype == SEQ_FP32 ? 4 : 2; }
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
-constexpr int64_t kMaxBlocks = 0x7fffffff;
+constexpr int64_t kMaxThreads = 0xffffffff;   // of a launch, along an axis
 
 // ----------------------------------------------------------------------------------------------- gated delta rule
 
@@ -118,7 +118,10 @@ int delta_sizes(const SeqDelta* d, bool saved, DeltaSizes& z) {
   // others (504 tiles of 9 sequences: 62 us and 91)
   z.wide_cols = tiles > (d->offsets ? 512 : 256);
   z.chunks = d->offsets ? (d->sequences && d->T ? d->T / z.C + d->sequences + 1 : 0) : z.per * d->batch;
-  if (z.chunks > kMaxBlocks / d->Hv || (d->sequences + 8) > kMaxBlocks / ((int64_t)d->Hv * (z.VP / 16) * 8))
+  // the largest launch of each kind: a sequence and head; a chunk and head; a sequence's column tiles (column_blocks)
+  const int64_t groups = (z.VP / 16 + (z.wide_cols ? 1 : 0)) / (z.wide_cols ? 2 : 1);
+  if (z.brief ? d->sequences > kMaxThreads / 256 / d->Hv
+              : z.chunks > kMaxThreads / (4 * z.C) / d->Hv || d->sequences + 7 > kMaxThreads / (8 * z.C) / (d->Hv * groups))
     return fail(SEQ_EINVAL, "too many sequences, rows or heads for one launch");
   // sizes of DeltaShape: K, Q, K^T (saved: Q^T), each z.C x KP planes; X, P (saved: their transposes) as fragments
   z.kq = up256(z.chunks * d->Hk * ((saved ? 4LL : 3LL) * NP * z.C * z.KP * 2));
@@ -193,7 +196,9 @@ int unit_sizes(const SeqUnit* u, bool backward, UnitSizes& z) {
   if (u->M > kUnitMaxRows) return fail(SEQ_EINVAL, "too many rows (%lld): up to %lld are supported", (long long)u->M, (long long)kUnitMaxRows);
   if (u->D < 1 || u->D > SEQ_UNIT_MAX || u->F < 1 || u->F > SEQ_UNIT_MAX)
     return fail(SEQ_EINVAL, "weights of %d x %d: 1 to %d are supported", u->D, u->F, SEQ_UNIT_MAX);
-  if (u->M / 64 + 1 > kMaxBlocks / (u->F / 64 + 1) || u->M / 64 + 1 > kMaxBlocks / (u->D / 64 + 1))
+  const UnitParts way = backward ? unit_parts(u->M, u->D, u->F, u->dtype) : UnitParts{0, 1};
+  const int64_t n = backward ? u->D : 2 * (int64_t)u->F;
+  if (tile_threads(tile_for(u->M, n, true, 1, nullptr), u->M, n) > kMaxThreads || (backward && tile_threads(way.tile, u->D, 2 * (int64_t)u->F) > kMaxThreads))
     return fail(SEQ_EINVAL, "too many rows for one launch");
   const int np = u->dtype == SEQ_FP32 ? 3 : backward && u->dtype == SEQ_FP16 ? 2 : 1;   // planes of x and the weights
   z.D8 = (u->D + 7) / 8 * 8;
@@ -204,8 +209,7 @@ int unit_sizes(const SeqUnit* u, bool backward, UnitSizes& z) {
   z.x = z.copy_x ? up256(u->M * z.D8 * 2 * np) : 0;
   z.w = z.copy_w ? up256(u->D * z.F8 * 2 * np) : 0;
   z.da = backward ? up256(u->M * z.F8 * 2 * np) : 0;
-  const int parts = backward ? unit_parts(u->M, u->D, u->F, u->dtype).parts : 1;
-  z.sums = parts > 1 ? up256(parts * 8LL * u->D * u->F) : 0;
+  z.sums = way.parts > 1 ? up256(way.parts * 8LL * u->D * u->F) : 0;
   z.need = z.x + 2 * z.w + 2 * z.da + z.sums;
   z.few = backward ? 0 : unit_few_splits(u->M, u->D, u->F, u->dtype);
   if (z.few) z.need = z.few > 1 ? up256(2LL * z.few * u->M * u->F * 4) : 0;
@@ -323,7 +327,9 @@ int seq_delta_step(const SeqDeltaStep* d, void* stream) {
   if (rc) return rc;
   if (d->batch < 0 || d->pool < 0) return fail(SEQ_EINVAL, "negative size");
   if (!d->slots && d->batch > d->pool) return fail(SEQ_EINVAL, "%lld rows and %lld states", (long long)d->batch, (long long)d->pool);
-  if (d->batch > kMaxBlocks / d->Hv / ((d->V + 31) / 32)) return fail(SEQ_EINVAL, "too many rows for one launch");
+  if (d->batch > kMaxThreads / d->Hv) return fail(SEQ_EINVAL, "too many rows for one launch");
+  const int64_t heads = d->batch * d->Hv, cols = step_cols(heads, d->V);
+  if (heads > kMaxThreads / 256 / ((d->V + cols - 1) / cols)) return fail(SEQ_EINVAL, "too many rows for one launch");
   if (!d->batch) return SEQ_OK;
   if (!d->q || !d->k || !d->v || !d->g || !d->beta || !d->o || (d->pool && !d->state)) return fail(SEQ_EINVAL, "NULL buffer");
   ON_DEVICE(d->device);

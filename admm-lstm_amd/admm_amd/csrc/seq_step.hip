@@ -135,7 +135,7 @@ void launch(const SeqDeltaStep& d, hipStream_t s) {
 template <int DT>
 void launch(const SeqDeltaStep& d, hipStream_t s) {
   const int64_t heads = d.batch * d.Hv;
-  if (d.V < 96 || heads < 1024) launch<DT, 32, false>(d, s);
+  if (step_cols(heads, d.V) == 32) launch<DT, 32, false>(d, s);
   else if (heads * d.K * d.V <= (32 << 20)) launch<DT, 128, false>(d, s);
   else launch<DT, 128, true>(d, s);
 }

@@ -41,6 +41,12 @@ inline int tile_for(int64_t m, int64_t n, bool with3, int parts, double* time) {
   return best;
 }
 
+// threads of a launch of such tiles, along its first axis
+inline int64_t tile_threads(int tile, int64_t m, int64_t n) {
+  constexpr int rows[4] = {256, 128, 64, 192}, cols[4] = {256, 128, 64, 256}, threads[4] = {512, 256, 256, 512};
+  return (m + rows[tile] - 1) / rows[tile] * ((n + cols[tile] - 1) / cols[tile]) * threads[tile];
+}
+
 // dWg and dWu have few tiles where the layer is narrow, and sum over all M rows: the sums are formed in parts, which a second
 // kernel adds up (in order), where that takes less time.  A round of 256 x 256 takes 30 ns a row (fp16: three times that, f32: six), the parts
 // are written and read at memory's rate, and another launch takes 5 us.  All gradients together, in us, and with one part:
