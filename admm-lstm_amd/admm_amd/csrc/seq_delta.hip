@@ -392,9 +392,8 @@ __global__ __launch_bounds__(8 * C, 2) void k_delta_scan(DeltaArgs a) {
       fnext.all = p[192];
       fnext.bad = p[193];
     };
-    // S as planes for Q S, and this wave's share of K S
+    // S as planes for Q S, and this wave's share of K S (where it has tiles of S)
     auto put_state = [&]() {
-      if (!holds) return;
 #pragma unroll
       for (int i = 0; i < NC; ++i) {
         f32x4 ks[S::RT];
@@ -419,7 +418,7 @@ __global__ __launch_bounds__(8 * C, 2) void k_delta_scan(DeltaArgs a) {
       load_vec();
       load_x();
       load_t();
-      put_state();
+      if (holds) put_state();
     }
     for (int ci = 0; ci < nc; ++ci) {
       const bool more = ci + 1 < nc;   // behind the last chunk its own values are loaded again, and not used
@@ -503,8 +502,8 @@ __global__ __launch_bounds__(8 * C, 2) void k_delta_scan(DeltaArgs a) {
             for (int t = 0; t < TW; ++t) st[i][t] = mfma_planes<NP, 3, 3>(ft[t][s], up, st[i][t]);
           }
         }
+        put_state();   // behind no branch: it reads the products' results first
       }
-      put_state();
       load_t();
       if (SAVE) {
         float* us = a.u + (ch * C + row0) * (int64_t)a.VP + col0;

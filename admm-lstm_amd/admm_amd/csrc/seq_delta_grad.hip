@@ -112,8 +112,7 @@ __global__ __launch_bounds__(8 * C, 2) void k_delta_back(DeltaGradArgs ga) {
       fnext.beta = *reinterpret_cast<const f32x4*>(p + 128 + row0);
       fnext.all = p[192];
     };
-    auto put_share = [&]() {
-      if (!holds) return;
+    auto put_share = [&]() {   // (where the wave has tiles of dS)
 #pragma unroll
       for (int i = 0; i < NC; ++i) {
         f32x4 ks[S::RT];
@@ -133,8 +132,10 @@ __global__ __launch_bounds__(8 * C, 2) void k_delta_back(DeltaGradArgs ga) {
       load_k();
       load_vec();
       load_x(S::pXT);
-      if (holds) load_t(S::fKT);
-      put_share();
+      if (holds) {
+        load_t(S::fKT);
+        put_share();
+      }
       lds_barrier();   // (the other waves exchange the last chunk's do)
       lds_barrier();
     }
@@ -191,9 +192,9 @@ __global__ __launch_bounds__(8 * C, 2) void k_delta_back(DeltaGradArgs ga) {
             mfma_rows<NP, 3, 3, TW>([&](int t) -> const bf16x8(&)[NP] { return ft[t][s]; }, rp, ds[i]);
           }
         }
+        put_share();   // behind no branch: it reads the products' results first
+        load_t(S::fKT);
       }
-      put_share();
-      if (holds) load_t(S::fKT);
 #pragma unroll
       for (int i = 0; i < NC; ++i) {
         float* p = ga.dr + (ch * C + row0) * (int64_t)a.VP + col0 + 16 * i;
@@ -456,6 +457,7 @@ __global__ __launch_bounds__(4 * C, C == 64 ? 2 : 1) void k_delta_grad(DeltaGrad
       }
     }
   }
+  mfma_settle();
   rdot += __shfl_xor(rdot, 1);
   rdot += __shfl_xor(rdot, 2);
   if ((tid & 3) == 0) rv[tid >> 2] = rdot;
@@ -484,6 +486,7 @@ __global__ __launch_bounds__(4 * C, C == 64 ? 2 : 1) void k_delta_grad(DeltaGrad
         kk[i] = mfma_planes<NP, NP, 3>(fa, kb, kk[i]);
       }
     }
+    mfma_settle();
     float csum = 0.f;
 #pragma unroll
     for (int i = 0; i < RT; ++i)
@@ -573,6 +576,7 @@ __global__ __launch_bounds__(4 * C, C == 64 ? 2 : 1) void k_delta_grad(DeltaGrad
         }
       }
     }
+    mfma_settle();
     const int64_t first = bt * a.rows.T + r0;
 #pragma unroll
     for (int i = 0; i < RT; ++i)
