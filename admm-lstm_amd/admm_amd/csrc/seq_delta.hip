@@ -41,7 +41,7 @@ __device__ __forceinline__ void tile_planes(const float* m, int ld, int r, int c
 
 // Bound by the chain of small products, exchanges and barriers of a chunk: several workgroups on a compute unit cover for each
 // other, so the f32 tiles lie where K and Q were, and fragments are cut straight from them.
-// 128 chunks of 16 query/key and 32 value heads of 128, bf16: 75 us, about 15 us of it one workgroup's way through; 230 MB written.
+// 128 chunks of 16 query/key and 32 value heads of 128, bf16: 73 us, about 15 us of it one workgroup's way through; 230 MB written.
 template <int DT, int KP, int C, bool SAVE>
 __global__ __launch_bounds__(4 * C, DT == SEQ_FP32 ? 2 : 3) void k_delta_prep(DeltaArgs a) {
   using S = DeltaShape<DT, KP, C, SAVE>;
@@ -288,7 +288,7 @@ __global__ __launch_bounds__(4 * C, DT == SEQ_FP32 ? 2 : 3) void k_delta_prep(De
 //
 // Bound by a chunk's chain of products and exchanges (few heads) or by loads and issue (many).  T 8192 of 128 x 128, bf16: one
 // wave for all rows and products took 6.3 us a chunk, four waves 2.5 us, eight with all of S handed through LDS 2.0 us, with
-// shares of K S instead 1.9 us.
+// shares of K S instead 1.9 us (1.7 us, 222 us in all, at the clocks of a program that goes on).
 template <int DT, int KP, int C, int NC, bool SAVE>
 struct Scan {
   using S = DeltaShape<DT, KP, C, SAVE>;

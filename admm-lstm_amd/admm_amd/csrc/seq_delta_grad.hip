@@ -23,7 +23,7 @@ namespace {
 // perm_row(w, .) of du and dR.  As many more waves form what does not depend on dS, P^T do and scale Q^T (exp(G_i) do), one
 // chunk ahead.
 //
-// Bound as k_delta_scan is: 3.3 us a chunk (32 chunks, 256 column tiles of 128 x 128, bf16: 104 us).
+// Bound as k_delta_scan is: 3.2 us a chunk (32 chunks, 256 column tiles of 128 x 128, bf16: 102 us).
 template <int DT, int KP, int C, int NC>
 struct Back {
   using S = DeltaShape<DT, KP, C, true>;
@@ -310,7 +310,8 @@ __device__ __forceinline__ float whole(const __bf16* p) {
 
 // A workgroup takes one chunk and value head: 32 columns of v at a time into LDS as planes, a wave for 16 rows of M and N and a
 // share of K's columns.  Bound by the latency of its products; at 64 rows it keeps to 256 registers, so that two workgroups of four
-// waves are on a unit (1024 chunks and heads of 128 x 128, bf16: 126 us, one at a time 171 us; the 295 MB that it moves would take 58 us).
+// waves are on a unit, though heads of 128 spill 47 registers a lane for that (f32: 67).  1024 chunks and heads of 128 x 128, bf16: 119
+// us (one workgroup at a time took 1.36 times as long); the 295 MB that it moves would take 58 us.
 template <int DT, int KP, int C>
 __global__ __launch_bounds__(4 * C, C == 64 ? 2 : 1) void k_delta_grad(DeltaGradArgs ga, bool wide_v, bool wide_o) {
   using S = DeltaShape<DT, KP, C, true>;

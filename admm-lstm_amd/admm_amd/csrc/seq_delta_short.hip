@@ -10,7 +10,8 @@
 // scratch memory (offsets that the compiler worked out before the loops).  f32, forward and forward with backward, in us, against
 // the kernels over chunks of 32 rows with their work memory: 2048 sequences of 32 rows, 4 heads of 64 x 64: 144 and 550 (321 and
 // 1024); 1024 of 32 rows, 4 heads of 128 x 128: 210 and 946 (493 and 1565); 256 of them, V = 512: 184 and 736 (405 and 1333);
-// 1024 of 8 rows: 184 and 887 (475 and 1517); 8 sequences: 10 (14).  At memory's rate the first would take 50 and 210.
+// 1024 of 8 rows: 184 and 887 (475 and 1517); 8 sequences: 10 (14).  At memory's rate the first would take 50 and 210; at the clocks
+// of a program that goes on it takes 135 and 523.
 #include "seq_delta_dev.hpp"
 
 namespace seq {

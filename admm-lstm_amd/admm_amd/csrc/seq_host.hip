@@ -114,8 +114,11 @@ int delta_sizes(const SeqDelta* d, bool saved, DeltaSizes& z) {
   z.VP = (d->V + 15) / 16 * 16;
   // Two column tiles a workgroup, which share its loads, where one each would be more than a round.  In us, one and two, forward
   // alone and with gradients, 1024 rows of 128 x 128, bf16: 256 tiles 48, 159 and 65, 187; 512: 79, 355 and 69, 303; 768: 111, 530
-  // and 117, 501; 1024: 162, 695 and 144, 583.  Packed sequences are of uneven length, and the short ones' units are soon free for
-  // others (504 tiles of 9 sequences: 62 us and 91)
+  // and 117, 501; 1024: 162, 695 and 144, 583.  Packed sequences are of uneven length as a rule: the time is the longest one's, whose
+  // chunks take longer with two, and the short ones' units are soon free for others.  8192 to 12288 rows cut at random, bf16: 320
+  // tiles (10 sequences, 4 heads of 128 x 128) 73, 236 and 105, 306; 384 (12, 8 of 64 x 64) 96, 332 and 135, 391; 448 (14, 4 of 128 x
+  // 128) 69, 227 and 85, 263; 512 (4, 16 of 128 x 128) 186, 775 and 196, 761; cut evenly, which the host cannot know: 64, 215 and 57,
+  // 198; 80, 278 and 74, 250; 57, 200 and 51, 187; 163, 703 and 144, 597
   z.wide_cols = tiles > (d->offsets ? 512 : 256);
   z.chunks = d->offsets ? (d->sequences && d->T ? d->T / z.C + d->sequences + 1 : 0) : z.per * d->batch;
   // the largest launch of each kind: a sequence and head; a chunk and head; a sequence's column tiles (column_blocks)

@@ -48,10 +48,10 @@ inline int64_t tile_threads(int tile, int64_t m, int64_t n) {
 }
 
 // dWg and dWu have few tiles where the layer is narrow, and sum over all M rows: the sums are formed in parts, which a second
-// kernel adds up (in order), where that takes less time.  A round of 256 x 256 takes 30 ns a row (fp16: three times that, f32: six), the parts
-// are written and read at memory's rate, and another launch takes 5 us.  All gradients together, in us, and with one part:
+// kernel adds up (in order), where that takes less time.  A round of 256 x 256 takes 30 ns a row (fp16: three times that, f32: six
+// times), the parts are written and read at memory's rate, and another launch takes 5 us.  All gradients together, in us, and with one part:
 //   f32: 262144 x 256 x 512: 2431 (19342), 65536 x 128 x 256: 351 (3723), 8192 x 512 x 1365: 621 (790), 1500 x 256 x 512: 102 (130);
-//   bf16: 724 (3483), 111 (561), 174 (190), 61 (57).
+//   fp16: 1404 (9751), 209 (1583), 331 (404), 63 (74);  bf16: 724 (3483), 111 (561), 174 (190), 61 (57).
 struct UnitParts {
   int tile, parts;
 };

@@ -16,8 +16,8 @@
 // rows.  Planes of the operands are formed by a pass before, and 16-bit operands whose rows are not 16-byte aligned are copied to
 // padded rows.
 //
-// 8192 x 2048 x 8192, bf16: forward with the projections kept 635 us (865 TFLOP/s; without them 550), dx 500 us and dWg, dWu 530 us
-// (1.1 and 1.04 PFLOP/s; a large library product reaches 1.2 to 1.3), the elementwise pass 204 us (4.6 TB/s).
+// 8192 x 2048 x 8192, bf16: forward with the projections kept 557 us (0.99 PFLOP/s; without them 465, 1.18), dx 434 us and dWg, dWu
+// 450 us (1.27 and 1.22 PFLOP/s; a large library product reaches 1.41), the elementwise pass 203 us (4.6 TB/s).
 //
 // Compiled by one source for each type (seq_unit_bf16.hip, _fp16, _fp32), so that they compile side by side.
 #pragma once

@@ -35,10 +35,12 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     B = 1: sequence n is rows ``offsets[n]:offsets[n + 1]``, and states are [len(offsets) - 1, Hv, K, V].  A sequence may
     be empty; rows outside every sequence get zeros.
 
-    Products and states are float32 throughout (operands split into bf16 pieces); only o and gradients of q, k, v are
-    rounded to the inputs' type.  A row whose g is -inf starts its sequence's state afresh.  Any other value that is not
-    finite makes NaN what depends on it, and nothing before its row (in q: o of that row; in v: its column from that row on;
-    in k, g and beta: all columns from that row on).
+    Sums and states are float32, and products accurate to float32 (operands split into three bf16 pieces), but for what only
+    results of 16 bits are made of: o of such inputs takes 16 bits (two pieces) of the state and of the rows written, and dq and dk
+    16 bits of the rows' weights.  o and the gradients of q, k, v are rounded to the inputs' type.  A row whose g is -inf starts its
+    sequence's state afresh.  Where rows grow (g > 0), exp of their sum over 64 rows has to be within float32.  Any other value that
+    is not finite (or is above 3.39e38) makes NaN what depends on it, and nothing before its row (in q: o of that row; in v: its
+    column from that row on; in k, g and beta: all columns from that row on).
     """
     return _E.gated_delta_rule(q, k, v, g, beta, scale, initial_state, offsets)
 

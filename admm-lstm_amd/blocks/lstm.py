@@ -10,7 +10,7 @@ gfx950 time-step kernel of libadmmlstm.so (``admm_forward``); they require HIP
 device tensors.  ``with_grad=True`` (``blocks/lstm.py:48-63``) is the autograd
 path the reference uses for its gradient-descent baselines; it is plain PyTorch.
 There ``dropout=p`` drops part of h_T before the output layer while the model trains
-(``blocks/dropout.py``); 0, the default, changes nothing.
+(``blocks/dropout.py``, for HIP device tensors); 0, the default, changes nothing.
 """
 from __future__ import annotations
 

@@ -4,7 +4,8 @@
  * They are what a recurrent model is built from next to the LSTM of blocks/lstm.py: the gated delta rule (a gated
  * recurrence with a matrix state), the gated unit (two projections, an activation and a product) and dropout whose
  * mask is recomputed from a counter instead of stored.  The Python entry points are blocks/delta_rule.py,
- * blocks/gated_unit.py and blocks/dropout.py, which bind these calls with ctypes (admm_amd/_seq_native.py).
+ * blocks/gated_unit.py and blocks/dropout.py, which call these through the extension _seq_torch (csrc/seq_torch.cpp);
+ * admm_amd/_seq_native.py loads the library and declares the calls for ctypes.
  *
  * Conventions (those of admm_lstm.h)
  *  - Plain C types: device pointers, sizes, a hipStream_t passed as void*; strides are in elements.
@@ -13,6 +14,7 @@
  *    memory is the caller's (seq_*_workspace gives its size); two calls that may overlap need two.
  *  - `device` is the HIP device that every pointer belongs to; the caller's current device is restored.
  *  - Every call may be captured into a HIP graph.
+ *  - A call larger than a launch takes (2^32 threads along an axis) is refused before anything is enqueued.
  */
 #ifndef SEQ_OPS_H
 #define SEQ_OPS_H
